@@ -57,7 +57,13 @@ enum {
  * truncating fp32_to_fp16 of src/quant.cpp:906-925 (not round-to-nearest).
  * JX_BF16 rounds with fp32_to_bf16 (src/quant.cpp:934-939).  JX_F32 stores the
  * rotated values unchanged. */
-typedef enum { JX_F32 = 0, JX_BF16 = 1, JX_F16_TRUNC = 2 } jx_dtype;
+typedef enum {
+    JX_F32 = 0,
+    JX_BF16 = 1,
+    JX_F16_TRUNC = 2,
+    JX_I8 = 3,   /* paged cache only (jx_pkv): 8-bit integers, scaled per block of rows */
+    JX_E4M3 = 4  /* paged cache only: 8-bit floats (4 exponent, 3 mantissa bits), scaled likewise */
+} jx_dtype;
 
 typedef struct jx_kv jx_kv;
 
@@ -237,6 +243,104 @@ JX_API int jx_noalloc_check_device_error(int device, int* code, void* stream);
  * later jx_attn_step_noalloc call in the process): "wait_limit_ms" and
  * "test_wait_cta" as in jx_kv_set_option.  No counterpart in the reference. */
 JX_API int jx_noalloc_set_option(const char* key, int value);
+
+/* ---- paged 8-bit cache ------------------------------------------------------
+ * No counterpart in the reference (its cache is fp16 or fp32, one contiguous
+ * slot per sequence).  Rows of K and V are held as 8-bit codes -- JX_I8:
+ * integers in [-127, 127]; JX_E4M3: 8-bit floats up to 448 -- with one
+ * power-of-two scale for each block of 16 rows and kv head, in pages of 32
+ * rows that sequences take from one pool, share after a fork and give back.
+ *
+ * What a row is held as: the key is rotated (angle = position * frequency in
+ * 64 bits, cosine and sine rounded to fp32, products and sums each rounded to
+ * fp32); NaN counts as 0 and magnitudes are cut at 2^62.  The scale is 2^k with
+ * the smallest k in [-40, 56] that holds the block's largest magnitude (-40 for
+ * a block of zeros); a code is the nearest one to value / 2^k, ties to even.
+ * Rows that join a block in a later call raise its scale where they have to,
+ * the codes already there are then re-rounded; it is never lowered.
+ *
+ * A sequence holds the rows [0, seq_pos).  A call that writes rows may begin at
+ * any position up to seq_pos; the sequence then ends at the row after the last
+ * one written.  Calls on one jx_pkv are ordered on one stream, like those on a
+ * jx_kv.  None of them can be captured into a CUDA graph (JX_ERR_UNSUPPORTED):
+ * which page a row goes to is decided on the host, call by call. */
+typedef struct jx_pkv jx_pkv;
+
+typedef struct {
+    uint32_t n_seqs;     /* sequences (slots) of the handle */
+    uint32_t n_layers;   /* cache layers */
+    uint32_t capacity;   /* rows a sequence may hold */
+    uint32_t n_kv_heads;
+    uint32_t head_dim;   /* 32, 64, 128 or 256, the same in every layer */
+    uint32_t n_pages;    /* pages of the pool, 32 rows of all layers each */
+    int32_t dtype;       /* JX_I8 or JX_E4M3 */
+    int32_t device;      /* CUDA device ordinal */
+} jx_pkv_desc;
+
+JX_API int jx_pkv_create(const jx_pkv_desc* desc, jx_pkv** out);
+JX_API int jx_pkv_destroy(jx_pkv* kv);
+JX_API int jx_pkv_get_desc(const jx_pkv* kv, jx_pkv_desc* desc);
+/* Rows held by a sequence.  set_seq_pos lowers it (as jx_pkv_rollback does) or
+ * confirms it; rows that were not written cannot be claimed (JX_ERR_RANGE). */
+JX_API int jx_pkv_get_seq_pos(const jx_pkv* kv, uint32_t seq, uint32_t* seq_pos);
+JX_API int jx_pkv_set_seq_pos(jx_pkv* kv, uint32_t seq, uint32_t seq_pos);
+/* Pages that are free, and pages a sequence holds (shared ones included). */
+JX_API int jx_pkv_free_pages(const jx_pkv* kv, uint32_t* n);
+JX_API int jx_pkv_held_pages(const jx_pkv* kv, uint32_t seq, uint32_t* n);
+
+/* Page operations.  clear gives a sequence's pages back; rollback drops the
+ * rows from new_seq_pos on and the pages that held only those. */
+JX_API int jx_pkv_clear(jx_pkv* kv, uint32_t seq);
+JX_API int jx_pkv_rollback(jx_pkv* kv, uint32_t seq, uint32_t new_seq_pos);
+/* dst becomes the first n_rows rows of src without moving any (dst's earlier
+ * rows are dropped): both read the same pages, and the one that writes into a
+ * shared page first gets its own copy of it. */
+JX_API int jx_pkv_fork(jx_pkv* kv, uint32_t src, uint32_t dst, uint32_t n_rows, void* stream);
+/* dst becomes a copy of src with pages of its own. */
+JX_API int jx_pkv_copy(jx_pkv* kv, uint32_t src, uint32_t dst, void* stream);
+/* Cuts a sequence down to the given rows (HOST array, ascending, each below
+ * seq_pos): row i of the result is row rows[i], for every layer.  Blocks that
+ * change are scaled and rounded anew from the values held.  Leading pages whose
+ * rows all stay in place are kept as they are.  Needs free pages for the others,
+ * or none where the pool has too few and the sequence shares none of them (the
+ * rows are then moved in place, which is slower). */
+JX_API int jx_pkv_keep(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, void* stream);
+/* jx_kv_compact's rule: rows [0, 4) and the last keep_recent rows stay; no-op
+ * when the sequence holds no more than those. */
+JX_API int jx_pkv_compact(jx_pkv* kv, uint32_t seq, uint32_t keep_recent, void* stream);
+
+/* Rows [row0, row0 + n_rows) of a sequence from codes and scales (DEVICE):
+ * codes [n_layers][n_rows][n_kv_heads][head_dim] bytes, scales [n_layers]
+ * [ceil(n_rows / 16)][n_kv_heads] fp32.  row0 is a multiple of 16.  A scale is
+ * taken down to a power of two in the format's range, the int8 code -128 as
+ * -127, an e4m3 NaN code as 0. */
+JX_API int jx_pkv_load_rows(jx_pkv* kv, uint32_t seq, uint32_t row0, uint32_t n_rows,
+                            const void* k_codes, const float* k_scales, const void* v_codes,
+                            const float* v_scales, void* stream);
+/* The values of n_rows rows of each listed sequence from row0[i] on (HOST
+ * arrays): out (DEVICE) [n][n_layers][2][n_rows][n_kv_heads][head_dim], K then
+ * V, of JX_F32 or JX_BF16 (both hold every value exactly). */
+JX_API int jx_pkv_read_rows(jx_pkv* kv, const int32_t* seq_ids, const int32_t* row0, uint32_t n,
+                            uint32_t n_rows, int32_t dtype, void* out, void* stream);
+
+/* jx_attn_step and jx_attn_prefill over a paged cache: the same arguments and
+ * the same attention, over the rows as they are held (a row of this call
+ * included).  q, k, v and out are memory of the cache's device; every layer has
+ * the cache's head_dim, the call its n_kv_heads; at most 8 RoPE settings per
+ * handle (rope_dim, base, factors, yarn_scale).  In a prompt, the rows of one sequence
+ * stand together and ascend by one.  New pages come from the pool; with too few
+ * left, JX_ERR_NOMEM and nothing is changed. */
+JX_API int jx_pkv_attn_step(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers,
+                            const jx_step_args* args, void* stream);
+JX_API int jx_pkv_attn_prefill(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers,
+                               const jx_step_args* args, void* stream);
+
+/* As jx_kv_check_device_error. */
+JX_API int jx_pkv_check_device_error(jx_pkv* kv, int* code, void* stream);
+/* "wait_limit_ms": as in jx_kv_set_option. */
+JX_API int jx_pkv_set_option(jx_pkv* kv, const char* key, int value);
+/* Kernels the last jx_pkv_attn_step / jx_pkv_attn_prefill launched. */
+JX_API int jx_pkv_last_launch_count(const jx_pkv* kv, int* count);
 
 /* ---- diagnostics, tuning, harness helpers --------------------------------- */
 

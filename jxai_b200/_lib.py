@@ -22,6 +22,7 @@ JX_ERR_TIMEOUT = -7
 JX_ERR_COMM = -8
 
 JX_F32, JX_BF16, JX_F16_TRUNC = 0, 1, 2
+JX_I8, JX_E4M3 = 3, 4  # paged cache only
 
 # symbols include/jx_attn.h declares (checked by the tests)
 EXPORTS = (
@@ -32,6 +33,11 @@ EXPORTS = (
     "jx_kv_fill_normal", "jx_fill_normal_f32", "jx_last_error_string", "jx_version",
     "jx_attn_step_noalloc", "jx_attn_step_sharded", "jx_kv_last_step_ms", "jx_attn_prefill",
     "jx_noalloc_check_device_error", "jx_noalloc_set_option",
+    "jx_pkv_create", "jx_pkv_destroy", "jx_pkv_get_desc", "jx_pkv_get_seq_pos",
+    "jx_pkv_set_seq_pos", "jx_pkv_free_pages", "jx_pkv_held_pages", "jx_pkv_clear",
+    "jx_pkv_rollback", "jx_pkv_fork", "jx_pkv_copy", "jx_pkv_keep", "jx_pkv_compact",
+    "jx_pkv_load_rows", "jx_pkv_read_rows", "jx_pkv_attn_step", "jx_pkv_attn_prefill",
+    "jx_pkv_check_device_error", "jx_pkv_set_option", "jx_pkv_last_launch_count",
 )
 
 
@@ -45,6 +51,12 @@ class KvDesc(C.Structure):
     _fields_ = [("n_seqs", C.c_uint32), ("n_layers", C.c_uint32), ("capacity", C.c_uint32),
                 ("row_stride", C.c_uint32), ("dtype", C.c_int32), ("device", C.c_int32),
                 ("pos_base", C.c_uint32)]
+
+
+class PkvDesc(C.Structure):
+    _fields_ = [("n_seqs", C.c_uint32), ("n_layers", C.c_uint32), ("capacity", C.c_uint32),
+                ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("n_pages", C.c_uint32),
+                ("dtype", C.c_int32), ("device", C.c_int32)]
 
 
 class LayerDesc(C.Structure):
@@ -95,6 +107,26 @@ def _declare(lib: C.CDLL) -> None:
         "jx_attn_prefill": [vp, C.POINTER(LayerDesc), u32, C.POINTER(StepArgs), vp],
         "jx_noalloc_check_device_error": [C.c_int, C.POINTER(C.c_int), vp],
         "jx_noalloc_set_option": [C.c_char_p, C.c_int],
+        "jx_pkv_create": [C.POINTER(PkvDesc), C.POINTER(vp)],
+        "jx_pkv_destroy": [vp],
+        "jx_pkv_get_desc": [vp, C.POINTER(PkvDesc)],
+        "jx_pkv_get_seq_pos": [vp, u32, C.POINTER(u32)],
+        "jx_pkv_set_seq_pos": [vp, u32, u32],
+        "jx_pkv_free_pages": [vp, C.POINTER(u32)],
+        "jx_pkv_held_pages": [vp, u32, C.POINTER(u32)],
+        "jx_pkv_clear": [vp, u32],
+        "jx_pkv_rollback": [vp, u32, u32],
+        "jx_pkv_fork": [vp, u32, u32, u32, vp],
+        "jx_pkv_copy": [vp, u32, u32, vp],
+        "jx_pkv_keep": [vp, u32, C.POINTER(i32), u32, vp],
+        "jx_pkv_compact": [vp, u32, u32, vp],
+        "jx_pkv_load_rows": [vp, u32, u32, u32, vp, vp, vp, vp, vp],
+        "jx_pkv_read_rows": [vp, C.POINTER(i32), C.POINTER(i32), u32, u32, i32, vp, vp],
+        "jx_pkv_attn_step": [vp, C.POINTER(LayerDesc), u32, C.POINTER(StepArgs), vp],
+        "jx_pkv_attn_prefill": [vp, C.POINTER(LayerDesc), u32, C.POINTER(StepArgs), vp],
+        "jx_pkv_check_device_error": [vp, C.POINTER(C.c_int), vp],
+        "jx_pkv_set_option": [vp, C.c_char_p, C.c_int],
+        "jx_pkv_last_launch_count": [vp, C.POINTER(C.c_int)],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)

@@ -71,8 +71,26 @@ class Layer:
     rope_freqs: Optional[np.ndarray] = None
 
 
+def _i32_array(x):
+    """A C array of int32 from integers; arrays are taken as a whole (a prompt lists one position
+    per token)."""
+    if isinstance(x, np.ndarray):
+        a = x
+    elif isinstance(x, range):
+        a = np.arange(x.start, x.stop, x.step)
+    else:
+        return (C.c_int32 * len(x))(*[int(v) for v in x])
+    if a.ndim != 1 or a.dtype.kind not in "iu":
+        raise JxError(-1, "expected a one-dimensional array of integers")
+    if a.size and (int(a.min()) < -(1 << 31) or int(a.max()) >= 1 << 31):
+        raise JxError(-1, "an integer does not fit 32 bits")
+    return (C.c_int32 * a.size).from_buffer_copy(np.ascontiguousarray(a, dtype=np.int32))
+
+
 class KVCache:
     """Device KV cache: K and V each [n_seqs][n_layers][capacity][row_stride]."""
+
+    entry_prefix = "jx_attn_"
 
     def __init__(self, n_seqs: int, n_layers: int, capacity: int, row_stride: int,
                  dtype="f32", device: int = 0, pos_base: int = 0):
@@ -264,10 +282,12 @@ def _step_args(cache, layers, q, k, v, out, pos, n_heads, n_kv_heads, scale, sof
     rows = n * len(layers)
     if scale is None:
         scale = 1.0 / math.sqrt(hd)
-    pos_a = (C.c_int32 * n)(*[int(p) for p in pos])
+    pos_a = _i32_array(pos)
     sid = None
     if seq_ids is not None:
-        sid = (C.c_int32 * n)(*[int(s) for s in seq_ids])
+        sid = _i32_array(seq_ids)
+        if len(sid) != n:
+            raise JxError(-1, "seq_ids: one sequence per row")
     a = StepArgs()
     a.n_heads, a.n_kv_heads, a.n_seqs = n_heads, n_kv_heads, n
     a.seq_ids = C.cast(sid, C.POINTER(C.c_int32)) if sid is not None else None
@@ -282,6 +302,14 @@ def _step_args(cache, layers, q, k, v, out, pos, n_heads, n_kv_heads, scale, sof
     return a, (pos_a, sid)
 
 
+def _entry(cache, name: str):
+    """The library call `name` for this kind of cache."""
+    fn = getattr(cache.lib, cache.entry_prefix + name, None)
+    if fn is None:
+        raise JxError(-4, f"{type(cache).__name__} has no {name}")
+    return fn
+
+
 def attn_step(cache: KVCache, layers: Sequence[Layer], q, k, v, out, pos: Sequence[int],
               n_heads: int, n_kv_heads: int, scale: Optional[float] = None, softcap: float = 0.0,
               sliding_window: int = 0, yarn_scale: float = 1.0, neox: bool = True,
@@ -289,12 +317,13 @@ def attn_step(cache: KVCache, layers: Sequence[Layer], q, k, v, out, pos: Sequen
     """RoPE + KV append + GQA decode attention for len(pos) slots x len(layers) layers.
 
     q/out: [n_seqs, n_layers, q_stride] float32 CUDA tensors;
-    k/v: [n_seqs, n_layers, kv_stride].  Asynchronous on `stream`.
+    k/v: [n_seqs, n_layers, kv_stride].  Asynchronous on `stream`.  `cache` is a
+    KVCache or a PagedKVCache.
     """
     arr, keep = _layer_array(layers)
     a, keep2 = _step_args(cache, layers, q, k, v, out, pos, n_heads, n_kv_heads, scale, softcap,
                           sliding_window, yarn_scale, neox, seq_ids, 0)
-    check(cache.lib.jx_attn_step(cache.handle, arr, len(layers), C.byref(a), _stream_ptr(stream)))
+    check(_entry(cache, "step")(cache.handle, arr, len(layers), C.byref(a), _stream_ptr(stream)))
 
 
 def attn_prefill(cache: KVCache, layers: Sequence[Layer], q, k, v, out, pos: Sequence[int],
@@ -303,14 +332,15 @@ def attn_prefill(cache: KVCache, layers: Sequence[Layer], q, k, v, out, pos: Seq
                  yarn_scale: float = 1.0, neox: bool = True, stream=None) -> None:
     """Many tokens per call: row i is a token of sequence seq_ids[i] (default 0)
     at position pos[i]; all rows are appended, then each attends causally.
+    On a PagedKVCache the rows of one sequence stand together and ascend by one.
     q/out: [n_rows, n_layers, q_stride]; k/v: [n_rows, n_layers, kv_stride]."""
     if seq_ids is None:
         seq_ids = [0] * len(pos)
     arr, keep = _layer_array(layers)
     a, keep2 = _step_args(cache, layers, q, k, v, out, pos, n_heads, n_kv_heads, scale, softcap,
                           sliding_window, yarn_scale, neox, seq_ids, 0)
-    check(cache.lib.jx_attn_prefill(cache.handle, arr, len(layers), C.byref(a),
-                                    _stream_ptr(stream)))
+    check(_entry(cache, "prefill")(cache.handle, arr, len(layers), C.byref(a),
+                                   _stream_ptr(stream)))
 
 
 def attn_step_partial(cache: KVCache, layers: Sequence[Layer], q, k, v, partials,
@@ -325,8 +355,8 @@ def attn_step_partial(cache: KVCache, layers: Sequence[Layer], q, k, v, partials
     arr, keep = _layer_array(layers)
     a, keep2 = _step_args(cache, layers, q, k, v, None, pos, n_heads, n_kv_heads, scale, softcap,
                           sliding_window, yarn_scale, neox, seq_ids, n)
-    check(cache.lib.jx_attn_step_partial(cache.handle, arr, len(layers), C.byref(a), pp,
-                                         _stream_ptr(stream)))
+    check(_entry(cache, "step_partial")(cache.handle, arr, len(layers), C.byref(a), pp,
+                                        _stream_ptr(stream)))
 
 
 def attn_step_sharded(cache: KVCache, layers: Sequence[Layer], q, k, v, out, pos: Sequence[int],
@@ -352,14 +382,14 @@ def attn_step_sharded(cache: KVCache, layers: Sequence[Layer], q, k, v, out, pos
     arr, keep = _layer_array(layers)
     a, keep2 = _step_args(cache, layers, q, k, v, out, pos, n_heads, n_kv_heads, scale, softcap,
                           sliding_window, yarn_scale, neox, seq_ids, 0)
-    check(cache.lib.jx_attn_step_sharded(cache.handle, arr, len(layers), C.byref(a),
-                                         C.c_void_p(int(comm)), int(timeout_ms),
-                                         _stream_ptr(stream)))
+    check(_entry(cache, "step_sharded")(cache.handle, arr, len(layers), C.byref(a),
+                                        C.c_void_p(int(comm)), int(timeout_ms),
+                                        _stream_ptr(stream)))
 
 
 class StepPlan:
-    """One attn_step (or attn_step_partial, or attn_step_sharded) call with its
-    C arguments built once.
+    """One attn_step (or attn_step_partial, or attn_step_sharded, or with
+    `prefill` attn_prefill) call with its C arguments built once.
 
     For callers that repeat the step on the same buffers (a decode loop whose
     inputs are rewritten in place, or a benchmark): run() costs one foreign
@@ -373,7 +403,11 @@ class StepPlan:
                  n_heads: int, n_kv_heads: int, scale: Optional[float] = None,
                  softcap: float = 0.0, sliding_window: int = 0, yarn_scale: float = 1.0,
                  neox: bool = True, seq_ids: Optional[Sequence[int]] = None, partials=None,
-                 comm=None, timeout_ms: int = 0):
+                 comm=None, timeout_ms: int = 0, prefill: bool = False):
+        if prefill and (comm is not None or partials is not None):
+            raise JxError(-1, "a prompt is neither partial nor sharded")
+        if prefill and seq_ids is None:
+            seq_ids = [0] * len(pos)
         self.cache = cache
         self.arr, self._keep = _layer_array(layers)
         self.args, self._keep2 = _step_args(cache, layers, q, k, v, out if partials is None else None,
@@ -385,16 +419,16 @@ class StepPlan:
         if comm is not None:
             if partials is not None:
                 raise JxError(-1, "a sharded step writes out, not partials")
-            self._call = cache.lib.jx_attn_step_sharded
+            self._call = _entry(cache, "step_sharded")
             self._head = (cache.handle, self.arr, self.n_layers, C.byref(self.args),
                           C.c_void_p(int(comm)), int(timeout_ms))
         elif partials is None:
-            self._call = cache.lib.jx_attn_step
+            self._call = _entry(cache, "prefill" if prefill else "step")
             self._head = (cache.handle, self.arr, self.n_layers, C.byref(self.args))
         else:
             hd = layers[0].head_dim
             pp = _dev_ptr(partials, "partials", len(pos) * len(layers) * n_heads * (hd + 2))
-            self._call = cache.lib.jx_attn_step_partial
+            self._call = _entry(cache, "step_partial")
             self._head = (cache.handle, self.arr, self.n_layers, C.byref(self.args), pp)
 
     def set_positions(self, pos: Sequence[int]) -> None:

@@ -1,0 +1,1259 @@
+// jx_paged.cu -- the paged 8-bit KV cache: its host side (pages, page tables,
+// argument checks, launch plans) and the kernels that write, move and read rows.
+//
+// Pages, their reference counts and the page table live on the host; a device
+// copy of the table ([n_seqs][max_pages]) is brought up to date by small kernels
+// on the caller's stream.  A launch's plan (which sequences, positions and
+// layers) travels in the kernel's parameters: nothing is uploaded, and no buffer
+// has to outlive the call.
+#include "jx_paged.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+#include <mutex>
+#include <new>
+#include <string>
+#include <vector>
+
+#include "jx_attn.h"
+#include "jx_device.cuh"
+#include "jx_internal.h"
+
+using namespace jx;
+
+namespace {
+
+int pfail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int pfail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    set_last_error(buf);
+    return code;
+}
+
+#define PKV_CUDA(call)                                                                    \
+    do {                                                                                  \
+        cudaError_t e_ = (call);                                                          \
+        if (e_ != cudaSuccess)                                                            \
+            return pfail(JX_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(e_));    \
+    } while (0)
+
+struct OnDevice {  // the handle's device for the duration of a call
+    int prev = -1;
+    bool ok = false;
+    explicit OnDevice(int dev) {
+        if (cudaGetDevice(&prev) != cudaSuccess) return;
+        ok = prev == dev || cudaSetDevice(dev) == cudaSuccess;
+    }
+    ~OnDevice() {
+        if (ok && prev >= 0) cudaSetDevice(prev);
+    }
+};
+
+// ------------------------------------------------------------------ kernels
+
+constexpr int kTableBatch = 480;
+struct TableSet {
+    int* table;
+    int n;
+    int at[kTableBatch];
+    int page[kTableBatch];
+};
+static_assert(sizeof(TableSet) <= 4096, "kernel parameters");
+
+__global__ void table_set_kernel(const __grid_constant__ TableSet t) {
+    for (int i = threadIdx.x; i < t.n; i += blockDim.x) t.table[t.at[i]] = t.page[i];
+}
+
+__global__ void table_copy_kernel(int* dst, const int* src, int n) {
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x)
+        dst[i] = src[i];
+}
+
+constexpr int kCopyBatch = 480;
+struct PageCopies {
+    unsigned char* pool;
+    long long page_bytes;
+    int n;
+    int src[kCopyBatch];
+    int dst[kCopyBatch];
+};
+static_assert(sizeof(PageCopies) <= 4096, "kernel parameters");
+
+// Whole pages, 16 bytes per thread and turn: a page is one contiguous run, so
+// this is a plain copy at memory speed whatever the layers and heads are.
+__global__ void page_copy_kernel(const __grid_constant__ PageCopies c) {
+    const long long n16 = c.page_bytes / 16;
+    for (int p = blockIdx.y; p < c.n; p += gridDim.y) {
+        const uint4* s = reinterpret_cast<const uint4*>(c.pool + c.src[p] * c.page_bytes);
+        uint4* d = reinterpret_cast<uint4*>(c.pool + c.dst[p] * c.page_bytes);
+        for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n16;
+             i += static_cast<long long>(gridDim.x) * blockDim.x)
+            d[i] = s[i];
+    }
+}
+
+// (cos, sin) of every rotated pair at every position of the cache, from angles
+// in 64 bits: at position 100000 an fp32 angle is off by up to 4e-3.
+struct RopeTable {
+    float2* out;
+    int rows, width, half;
+    double freq[128];
+};
+__global__ void rope_table_kernel(const __grid_constant__ RopeTable t) {
+    const long long n = static_cast<long long>(t.rows) * t.width;
+    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n;
+         i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const int j = static_cast<int>(i % t.width);
+        float2 r = make_float2(1.0f, 0.0f);
+        if (j < t.half) {
+            const double a = static_cast<double>(i / t.width) * t.freq[j];
+            r = make_float2(static_cast<float>(cos(a)), static_cast<float>(sin(a)));
+        }
+        t.out[i] = r;
+    }
+}
+
+// Largest value over the `n` threads (a multiple of 32, starting at a warp) of
+// one half of the CTA: `red` has one slot per warp.
+__device__ __forceinline__ float half_max(float v, float* red, int n) {
+    v = warp_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int w0 = threadIdx.x / n * (n / 32);
+    float m = 0.0f;
+    for (int w = 0; w < n / 32; ++w) m = fmaxf(m, red[w0 + w]);
+    return m;
+}
+
+template <int DT>
+__device__ __forceinline__ uint4 pack_codes(const float (&x)[16], float inv) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = to_code<DT>(x[4 * i] * inv) | to_code<DT>(x[4 * i + 1] * inv) << 8 |
+               to_code<DT>(x[4 * i + 2] * inv) << 16 | to_code<DT>(x[4 * i + 3] * inv) << 24;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack_codes(const uint4& c, float (&x)[16]) {
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = from_code<DT>((w[i / 4] >> (8 * (i % 4))) & 0xFFu);
+}
+
+// Rows of a call written to the cache.  One CTA per (block of 16 rows, layer,
+// kv head): its first half takes K, its second V, one thread per 16 values of
+// a row.  The block's largest magnitude gives the scale; rows that were in the
+// block before the call are re-rounded where the scale grows.
+template <int HD, int DT>
+__global__ void __launch_bounds__(2 * HD) append_kernel(const __grid_constant__ PagedArgs a) {
+    constexpr int CPR = HD / 16;  // threads per row
+    __shared__ float red[2 * HD / 32];
+    const int which = threadIdx.x / HD, tid = threadIdx.x % HD;
+    const int row = tid / CPR, d0 = tid % CPR * 16;
+    int r = 0;
+    while (r + 1 < a.n_runs && a.runs[r + 1].off <= static_cast<int>(blockIdx.x)) ++r;
+    const PagedRun run = a.runs[r];
+    const int h = blockIdx.y % a.n_kv;
+    const PagedLayer L = a.layers[blockIdx.y / a.n_kv];
+    const int blk = run.pos0 / kBlockRows + (static_cast<int>(blockIdx.x) - run.off);
+    const int t = blk * kBlockRows + row;
+    const bool is_new = t >= run.pos0 && t < run.pos0 + run.n;
+    const bool kept = t < run.pos0;
+    const int page = a.table[static_cast<long long>(run.seq) * a.max_pages + blk / 2];
+    unsigned char* rec = a.pool + page * a.page_bytes + L.cache_layer * a.layer_bytes +
+                         static_cast<long long>(h) * record_bytes(HD);
+    unsigned char* dst = rec + which * kPageRows * HD +
+                         tile_byte(HD, (blk & 1) * kBlockRows + row, d0);
+    float* scale = reinterpret_cast<float*>(rec + 2 * kPageRows * HD) + which * 2 + (blk & 1);
+    float x[16];
+    float m = 0.0f;
+    if (is_new) {
+        const long long io = static_cast<long long>(run.io0 + t - run.pos0) * a.n_io_layers + L.io;
+        if (which == 0) {
+            const float* src = a.k_in + io * a.kv_stride + h * HD;
+            const float2* cs = a.rope[L.cfg] + static_cast<long long>(t) * (HD / 2);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                x[i] = cache_value(rope_plain(src, d0 + i, L.half, cs, a.neox != 0));
+        } else {
+            const float* src = a.v_in + io * a.kv_stride + h * HD + d0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = cache_value(src[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(x[i]));
+    }
+    m = half_max(m, red, HD);
+    int k = block_exp<DT>(m);
+    const bool joins = blk * kBlockRows < run.pos0;  // earlier rows stay in the block
+    const int k_old = joins ? max(kMinExp, scale_exp(*scale)) : kMinExp;
+    k = max(k, k_old);
+    __syncthreads();  // the old scale is read by all before one thread replaces it
+    if (is_new) *reinterpret_cast<uint4*>(dst) = pack_codes<DT>(x, exp2_int(-k));
+    if (kept && k > k_old) {
+        unpack_codes<DT>(*reinterpret_cast<const uint4*>(dst), x);
+        *reinterpret_cast<uint4*>(dst) = pack_codes<DT>(x, exp2_int(k_old - k));
+    }
+    if (tid == 0) *scale = exp2_int(k);
+}
+
+struct KeepArgs {
+    unsigned char* pool;
+    const int* src_table;  // [pages] of the sequence as it is
+    const int* dst_table;  // [pages] of the result
+    const int* rows;       // [n_rows] kept rows, ascending
+    long long page_bytes;
+    int n_rec;             // records of a page
+    int n_rows;
+    int blk0;              // first block to write
+    int n_blk;             // blocks to write
+    int serial;            // one CTA per record, block after block (in place)
+};
+
+// Kept rows gathered into dense blocks: each is scaled and rounded anew from
+// the values held.  Same thread layout as append_kernel.  Row i of the result
+// comes from a row >= i, and a CTA reads all of a block before it writes it: in
+// place (serial) no row is overwritten before it has been read.
+template <int HD, int DT>
+__global__ void __launch_bounds__(2 * HD) keep_kernel(const KeepArgs a) {
+    constexpr int CPR = HD / 16;
+    __shared__ float red[2 * HD / 32];
+    const int which = threadIdx.x / HD, tid = threadIdx.x % HD;
+    const int row = tid / CPR, d0 = tid % CPR * 16;
+    const long long rec_off = static_cast<long long>(blockIdx.y) * record_bytes(HD);
+    const int last = a.serial ? a.n_blk : static_cast<int>(blockIdx.x) + 1;
+    for (int b = a.serial ? 0 : static_cast<int>(blockIdx.x); b < last; ++b) {
+        const int blk = a.blk0 + b;
+        const int i = blk * kBlockRows + row;
+        float x[16];
+        float m = 0.0f;
+        if (i < a.n_rows) {
+            const int t = a.rows[i];
+            const unsigned char* rec = a.pool + a.src_table[t / kPageRows] * a.page_bytes + rec_off;
+            const float s = reinterpret_cast<const float*>(rec + 2 * kPageRows * HD)
+                [which * 2 + (t / kBlockRows & 1)];
+            unpack_codes<DT>(*reinterpret_cast<const uint4*>(rec + which * kPageRows * HD +
+                                                             tile_byte(HD, t % kPageRows, d0)), x);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                x[j] *= s;
+                m = fmaxf(m, fabsf(x[j]));
+            }
+        }
+        m = half_max(m, red, HD);  // its barriers also order this block's reads before its writes
+        const int k = block_exp<DT>(m);
+        unsigned char* rec = a.pool + a.dst_table[blk / 2] * a.page_bytes + rec_off;
+        if (i < a.n_rows)
+            *reinterpret_cast<uint4*>(rec + which * kPageRows * HD +
+                                      tile_byte(HD, (blk & 1) * kBlockRows + row, d0)) =
+                pack_codes<DT>(x, exp2_int(-k));
+        if (tid == 0)
+            reinterpret_cast<float*>(rec + 2 * kPageRows * HD)[which * 2 + (blk & 1)] = exp2_int(k);
+        __syncthreads();  // this block's writes before the next one's reads
+    }
+}
+
+struct LoadArgs {
+    unsigned char* pool;
+    const int* table;  // of the sequence
+    const unsigned char* codes[2];
+    const float* scales[2];
+    long long page_bytes;
+    int row0, n_rows, n_kv, n_layers;
+};
+
+template <int HD, int DT>
+__global__ void load_kernel(const LoadArgs a) {
+    constexpr int CPR = HD / 16;
+    const int n_blk = (a.n_rows + kBlockRows - 1) / kBlockRows;
+    const long long n = static_cast<long long>(a.n_layers) * a.n_rows * a.n_kv * CPR;
+    const int which = blockIdx.y;
+    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < n;
+         i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const int c = static_cast<int>(i % CPR);
+        const int h = static_cast<int>(i / CPR % a.n_kv);
+        const long long lr = i / CPR / a.n_kv;
+        const int r = static_cast<int>(lr % a.n_rows), l = static_cast<int>(lr / a.n_rows);
+        const int t = a.row0 + r;
+        unsigned char* rec = a.pool + a.table[t / kPageRows] * a.page_bytes +
+                             (static_cast<long long>(l) * a.n_kv + h) * record_bytes(HD);
+        const uint4 v = *reinterpret_cast<const uint4*>(a.codes[which] + i * 16);
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t o = 0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                uint32_t u = (w[j] >> (8 * b)) & 0xFFu;
+                if constexpr (DT == DT_I8) u = max(u ^ 0x80u, 1u);  // offset by 128; -128 -> -127
+                else u = (u & 0x7Fu) == 0x7Fu ? 0u : u;             // NaN -> 0
+                o |= u << (8 * b);
+            }
+            w[j] = o;
+        }
+        *reinterpret_cast<uint4*>(rec + which * kPageRows * HD +
+                                  tile_byte(HD, t % kPageRows, c * 16)) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+        if (c == 0 && r % kBlockRows == 0) {
+            const float s = a.scales[which][(static_cast<long long>(l) * n_blk + r / kBlockRows) * a.n_kv + h];
+            reinterpret_cast<float*>(rec + 2 * kPageRows * HD)[which * 2 + (t / kBlockRows & 1)] =
+                exp2_int(min(kMaxExp, max(kMinExp, scale_exp(fabsf(s)))));
+        }
+    }
+}
+
+struct ReadArgs {
+    const unsigned char* pool;
+    const int* table;
+    void* out;
+    long long page_bytes;
+    int max_pages, n_kv, n_layers, n_rows, n;
+    int seq[kMaxRuns];
+    int row0[kMaxRuns];
+};
+
+template <int HD, int DT, bool F32>
+__global__ void read_kernel(const __grid_constant__ ReadArgs a) {
+    constexpr int CPR = HD / 16;
+    const long long per = static_cast<long long>(a.n_layers) * 2 * a.n_rows * a.n_kv * CPR;
+    const int s = blockIdx.y;
+    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < per;
+         i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const int c = static_cast<int>(i % CPR);
+        const int h = static_cast<int>(i / CPR % a.n_kv);
+        long long q = i / CPR / a.n_kv;
+        const int t = a.row0[s] + static_cast<int>(q % a.n_rows);
+        q /= a.n_rows;
+        const int which = static_cast<int>(q & 1), l = static_cast<int>(q >> 1);
+        const unsigned char* rec =
+            a.pool + a.table[static_cast<long long>(a.seq[s]) * a.max_pages + t / kPageRows] * a.page_bytes +
+            (static_cast<long long>(l) * a.n_kv + h) * record_bytes(HD);
+        const float sc = reinterpret_cast<const float*>(rec + 2 * kPageRows * HD)
+            [which * 2 + (t / kBlockRows & 1)];
+        float x[16];
+        unpack_codes<DT>(*reinterpret_cast<const uint4*>(rec + which * kPageRows * HD +
+                                                         tile_byte(HD, t % kPageRows, c * 16)), x);
+        const long long o = (s * per + i) * 16;
+        if constexpr (F32) {
+            float4* dst = reinterpret_cast<float4*>(static_cast<float*>(a.out) + o);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                dst[j] = make_float4(x[4 * j] * sc, x[4 * j + 1] * sc, x[4 * j + 2] * sc, x[4 * j + 3] * sc);
+        } else {
+            // a code has at most 7 significant bits: its value is a bf16 number,
+            // the upper half of the fp32 one
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                w[j] = __byte_perm(__float_as_uint(x[2 * j] * sc), __float_as_uint(x[2 * j + 1] * sc), 0x7632);
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + o);
+            dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+    }
+}
+
+// Attention of one token and kv head: a CTA of 128 threads walks its rows page
+// by page with the running maximum and sum of the softmax.
+template <int HD, int DT>
+__global__ void __launch_bounds__(128) attend_kernel(const __grid_constant__ PagedArgs a) {
+    __shared__ float q_s[8][HD];
+    __shared__ float p_s[8][kPageRows];
+    __shared__ float f_s[8];
+    const int tid = threadIdx.x;
+    int r = 0;
+    while (r + 1 < a.n_runs && a.runs[r + 1].off <= static_cast<int>(blockIdx.x)) ++r;
+    const PagedRun run = a.runs[r];
+    const int j = static_cast<int>(blockIdx.x) - run.off;
+    const int pos = run.pos0 + j;
+    const int h = blockIdx.y % a.n_kv;
+    const PagedLayer L = a.layers[blockIdx.y / a.n_kv];
+    const long long io = static_cast<long long>(run.io0 + j) * a.n_io_layers + L.io;
+    const float2* cs = a.rope[L.cfg] + static_cast<long long>(pos) * (HD / 2);
+    for (int i = tid; i < a.G * HD; i += 128)
+        q_s[i / HD][i % HD] = rope_plain(a.q + io * a.q_stride + (h * a.G + i / HD) * HD, i % HD, L.half,
+                                         cs, a.neox != 0);
+    const int lo = (L.flags & kLayerWindow) ? max(0, pos - a.window + 1) : 0;
+    float o[8][(HD + 127) / 128];
+    for (int g = 0; g < 8; ++g)
+        for (int e = 0; e < (HD + 127) / 128; ++e) o[g][e] = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // of head tid / 16 (16 threads per head)
+    const int hg = tid / 16;
+    __syncthreads();
+    for (int p = lo / kPageRows; p <= pos / kPageRows; ++p) {
+        const unsigned char* rec =
+            a.pool + a.table[static_cast<long long>(run.seq) * a.max_pages + p] * a.page_bytes +
+            L.cache_layer * a.layer_bytes + static_cast<long long>(h) * record_bytes(HD);
+        const float* sc = reinterpret_cast<const float*>(rec + 2 * kPageRows * HD);
+        const int row = tid / 4, part = tid % 4, t = p * kPageRows + row;
+        float dot[8];
+        for (int g = 0; g < 8; ++g) dot[g] = 0.0f;
+        for (int d = part * (HD / 4); d < (part + 1) * (HD / 4); ++d) {
+            const float kv = from_code<DT>(rec[tile_byte(HD, row, d)]);
+            for (int g = 0; g < a.G; ++g) dot[g] += q_s[g][d] * kv;
+        }
+        for (int g = 0; g < 8; ++g) {
+            float s = dot[g];
+            s += __shfl_xor_sync(0xffffffffu, s, 1);
+            s += __shfl_xor_sync(0xffffffffu, s, 2);
+            s = s * sc[row / kBlockRows] * a.scale;
+            if (a.softcap > 0.0f) s = a.softcap * tanhf(s * a.inv_softcap);
+            if (part == 0) p_s[g][row] = (t >= lo && t <= pos) ? s : -INFINITY;
+        }
+        __syncthreads();
+        float s0 = p_s[hg][tid % 16], s1 = p_s[hg][tid % 16 + 16];
+        float mt = fmaxf(s0, s1);
+        for (int x = 8; x > 0; x >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
+        const float mn = fmaxf(m, mt);
+        const float f = m == -INFINITY ? 0.0f : __expf(m - mn);
+        s0 = s0 == -INFINITY ? 0.0f : expf(s0 - mn);
+        s1 = s1 == -INFINITY ? 0.0f : expf(s1 - mn);
+        float ls = s0 + s1;
+        for (int x = 8; x > 0; x >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
+        l = l * f + ls;
+        m = mn;
+        __syncwarp();
+        p_s[hg][tid % 16] = s0 * sc[2];
+        p_s[hg][tid % 16 + 16] = s1 * sc[3];
+        if (tid % 16 == 0) f_s[hg] = f;
+        __syncthreads();
+        for (int e = 0; e < (HD + 127) / 128; ++e) {
+            const int d = tid + e * 128;
+            if (d >= HD) break;
+            for (int g = 0; g < a.G; ++g) o[g][e] *= f_s[g];
+            for (int rr = 0; rr < kPageRows; ++rr) {
+                const float v = from_code<DT>(rec[kPageRows * HD + tile_byte(HD, rr, d)]);
+                for (int g = 0; g < a.G; ++g) o[g][e] += p_s[g][rr] * v;
+            }
+        }
+        __syncthreads();
+    }
+    if (tid % 16 == 0) f_s[hg] = l;
+    __syncthreads();
+    for (int e = 0; e < (HD + 127) / 128; ++e) {
+        const int d = tid + e * 128;
+        if (d >= HD) break;
+        for (int g = 0; g < a.G; ++g)
+            a.out[io * a.q_stride + (h * a.G + g) * HD + d] = o[g][e] / f_s[g];
+    }
+}
+
+// Calls f(integral_constant<HD>, integral_constant<DT>) for a cache's format.
+template <int V>
+using Int = std::integral_constant<int, V>;
+template <typename F>
+void dispatch(const jx_pkv_desc& d, F&& f) {
+    auto with_hd = [&](auto dt) {
+        switch (d.head_dim) {
+            case 32: f(Int<32>{}, dt); break;
+            case 64: f(Int<64>{}, dt); break;
+            case 128: f(Int<128>{}, dt); break;
+            default: f(Int<256>{}, dt); break;
+        }
+    };
+    if (d.dtype == JX_I8) with_hd(Int<DT_I8>{});
+    else with_hd(Int<DT_E4M3>{});
+}
+
+struct RopeCfg {
+    uint32_t rdim, base_bits, yarn_bits;
+    std::vector<float> factors;
+    float2* d_tab;
+};
+
+}  // namespace
+
+struct jx_pkv {
+    jx_pkv_desc d{};
+    long long page_bytes = 0, layer_bytes = 0;
+    uint32_t max_pages = 0;
+    unsigned char* pool = nullptr;
+    int* d_table = nullptr;
+    std::vector<int> free_pages;          // a stack
+    std::vector<int> refs;                // sequences that hold the page
+    std::vector<std::vector<int>> pages;  // of each sequence
+    std::vector<uint32_t> rows;           // rows held by each sequence
+    std::vector<RopeCfg> ropes;
+    int* d_err = nullptr;
+    int* d_dbg = nullptr;
+    int* d_rows = nullptr;                // keep: row list and source page table
+    size_t d_rows_n = 0;
+    int* h_rows = nullptr;                // pinned
+    size_t h_rows_n = 0;
+    cudaEvent_t ev_rows = nullptr;        // the copy out of h_rows
+    int num_sms = 0;
+    int opt_wait_limit_ms = 0;
+    int last_launches = 0;
+};
+
+namespace {
+
+int launched(const char* what) {
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? JX_OK : pfail(JX_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+}
+
+int refuse_capture(cudaStream_t st) {
+    cudaStreamCaptureStatus c = cudaStreamCaptureStatusNone;
+    PKV_CUDA(cudaStreamIsCapturing(st, &c));
+    return c == cudaStreamCaptureStatusNone
+               ? JX_OK
+               : pfail(JX_ERR_UNSUPPORTED,
+                       "calls on a paged cache cannot be captured into a graph (pages are "
+                       "assigned on the host, call by call)");
+}
+
+uint32_t pages_for(uint32_t rows) { return (rows + kPageRows - 1) / kPageRows; }
+
+void give_back(jx_pkv* kv, int page) {
+    if (--kv->refs[page] == 0) kv->free_pages.push_back(page);
+}
+
+int take_page(jx_pkv* kv) {  // the caller has checked that one is free
+    const int p = kv->free_pages.back();
+    kv->free_pages.pop_back();
+    kv->refs[p] = 1;
+    return p;
+}
+
+void drop_rows(jx_pkv* kv, uint32_t seq, uint32_t rows) {
+    auto& pg = kv->pages[seq];
+    while (pg.size() > pages_for(rows)) {
+        give_back(kv, pg.back());
+        pg.pop_back();
+    }
+    kv->rows[seq] = std::min(kv->rows[seq], rows);
+}
+
+struct TableEntry {
+    uint32_t seq, idx;
+    int page;
+};
+
+int set_table(jx_pkv* kv, const std::vector<TableEntry>& e, cudaStream_t st) {
+    for (size_t i = 0; i < e.size();) {
+        TableSet t;
+        t.table = kv->d_table;
+        t.n = 0;
+        for (; i < e.size() && t.n < kTableBatch; ++i, ++t.n) {
+            t.at[t.n] = static_cast<int>(e[i].seq * kv->max_pages + e[i].idx);
+            t.page[t.n] = e[i].page;
+        }
+        table_set_kernel<<<1, 128, 0, st>>>(t);
+        if (int rc = launched("page table")) return rc;
+    }
+    return JX_OK;
+}
+
+int copy_pages(jx_pkv* kv, const std::vector<std::pair<int, int>>& c, cudaStream_t st) {
+    for (size_t i = 0; i < c.size();) {
+        PageCopies p;
+        p.pool = kv->pool;
+        p.page_bytes = kv->page_bytes;
+        p.n = 0;
+        for (; i < c.size() && p.n < kCopyBatch; ++i, ++p.n) {
+            p.src[p.n] = c[i].first;
+            p.dst[p.n] = c[i].second;
+        }
+        const long long per = std::max<long long>(1, (kv->page_bytes / 16 + 255) / 256);
+        const dim3 grid(static_cast<unsigned>(std::min<long long>(per, 64)), p.n);
+        page_copy_kernel<<<grid, 256, 0, st>>>(p);
+        if (int rc = launched("page copy")) return rc;
+    }
+    return JX_OK;
+}
+
+struct Span {  // rows [begin, end) of a sequence that a call writes
+    uint32_t seq, begin, end;
+};
+
+// Pages for the rows that a call writes: new ones, and copies of shared ones
+// (the page is shared by a fork: the writer gets its own).  All or nothing.
+int make_room(jx_pkv* kv, const std::vector<Span>& spans, cudaStream_t st) {
+    size_t need = 0;
+    for (const Span& s : spans) {
+        const auto& pg = kv->pages[s.seq];
+        for (uint32_t i = s.begin / kPageRows; i < pages_for(s.end); ++i)
+            if (i >= pg.size() || kv->refs[pg[i]] > 1) ++need;
+    }
+    if (need > kv->free_pages.size())
+        return pfail(JX_ERR_NOMEM, "%zu pages are needed, %zu of %u are free", need,
+                     kv->free_pages.size(), kv->d.n_pages);
+    std::vector<TableEntry> table;
+    std::vector<std::pair<int, int>> copies;
+    for (const Span& s : spans) {
+        auto& pg = kv->pages[s.seq];
+        for (uint32_t i = s.begin / kPageRows; i < pages_for(s.end); ++i) {
+            if (i < pg.size() && kv->refs[pg[i]] == 1) continue;
+            const int p = take_page(kv);
+            if (i < pg.size()) {
+                copies.emplace_back(pg[i], p);
+                give_back(kv, pg[i]);
+                pg[i] = p;
+            } else {
+                pg.push_back(p);
+            }
+            table.push_back({s.seq, i, p});
+        }
+    }
+    if (int rc = copy_pages(kv, copies, st)) return rc;
+    return set_table(kv, table, st);
+}
+
+// The table of (cos, sin) rows for a layer's RoPE setting, built on first use.
+int rope_table(jx_pkv* kv, const jx_layer_desc& L, float yarn, bool neox, cudaStream_t st, int* cfg) {
+    const uint32_t rdim = std::min(L.head_dim, L.rope_dim) / 2 * 2;
+    const float* rf = neox && !L.is_swa ? L.rope_freqs : nullptr;
+    uint32_t bb, yb;
+    std::memcpy(&bb, &L.rope_freq_base, 4);
+    std::memcpy(&yb, &yarn, 4);
+    for (size_t i = 0; i < kv->ropes.size(); ++i) {
+        const RopeCfg& r = kv->ropes[i];
+        if (r.rdim == rdim && r.base_bits == bb && r.yarn_bits == yb &&
+            r.factors.size() == (rf ? rdim / 2 : 0) &&
+            (!rf || std::memcmp(r.factors.data(), rf, rdim / 2 * sizeof(float)) == 0)) {
+            *cfg = static_cast<int>(i);
+            return JX_OK;
+        }
+    }
+    if (kv->ropes.size() == kMaxRopeCfgs)
+        return pfail(JX_ERR_UNSUPPORTED, "more than %d RoPE settings on one paged cache", kMaxRopeCfgs);
+    RopeCfg r{rdim, bb, yb, {}, nullptr};
+    if (rf) r.factors.assign(rf, rf + rdim / 2);
+    RopeTable t;
+    t.rows = static_cast<int>(kv->d.capacity);
+    t.width = static_cast<int>(kv->d.head_dim / 2);
+    t.half = static_cast<int>(rdim / 2);
+    for (int j = 0; j < t.half; ++j) {
+        t.freq[j] = std::pow(static_cast<double>(L.rope_freq_base), -2.0 * j / rdim) /
+                    static_cast<double>(std::max(1e-4f, yarn));
+        if (rf) t.freq[j] /= static_cast<double>(rf[j]);
+    }
+    const size_t n = static_cast<size_t>(t.rows) * t.width;
+    if (cudaMalloc(&r.d_tab, n * sizeof(float2)) != cudaSuccess) {
+        cudaGetLastError();
+        return pfail(JX_ERR_NOMEM, "RoPE table of %zu bytes failed", n * sizeof(float2));
+    }
+    t.out = r.d_tab;
+    rope_table_kernel<<<static_cast<unsigned>(std::min<size_t>((n + 255) / 256, 4096)), 256, 0, st>>>(t);
+    if (int rc = launched("RoPE table")) {
+        cudaFree(r.d_tab);
+        return rc;
+    }
+    kv->ropes.push_back(std::move(r));
+    *cfg = static_cast<int>(kv->ropes.size()) - 1;
+    return JX_OK;
+}
+
+int check_device_ptr(const void* p, const char* name, int device) {
+    cudaPointerAttributes at{};
+    const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return pfail(JX_ERR_INVALID, "%s: not a CUDA-visible pointer (%s)", name, cudaGetErrorString(e));
+    }
+    if ((at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged) && at.device == device)
+        return JX_OK;
+    return pfail(JX_ERR_INVALID, "%s must be memory of device %d", name, device);
+}
+
+int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const jx_step_args* a,
+              cudaStream_t st, bool prompt) {
+    if (!kv || !layers || !a) return pfail(JX_ERR_INVALID, "null handle, layers or args");
+    if (n_layers == 0 || a->n_seqs == 0) return pfail(JX_ERR_INVALID, "empty step");
+    if (n_layers > 65535) return pfail(JX_ERR_INVALID, "more than 65535 layers");
+    if (!a->pos || !a->q || !a->k || !a->v || !a->out)
+        return pfail(JX_ERR_INVALID, "null pos/q/k/v/out");
+    const jx_pkv_desc& D = kv->d;
+    if (a->n_kv_heads != D.n_kv_heads || a->n_heads == 0 || a->n_heads % a->n_kv_heads != 0)
+        return pfail(JX_ERR_INVALID, "n_kv_heads %u (the cache has %u) must match and divide n_heads %u",
+                     a->n_kv_heads, D.n_kv_heads, a->n_heads);
+    const uint32_t G = a->n_heads / a->n_kv_heads;
+    if (G > 8) return pfail(JX_ERR_UNSUPPORTED, "query group of %u heads exceeds 8", G);
+    if (!(a->yarn_scale >= 0.0f)) return pfail(JX_ERR_INVALID, "yarn_scale must not be negative or NaN");
+    const uint64_t q_row = static_cast<uint64_t>(a->n_heads) * D.head_dim;
+    const uint64_t kv_row = static_cast<uint64_t>(a->n_kv_heads) * D.head_dim;
+    if (a->q_stride < q_row || a->kv_stride < kv_row)
+        return pfail(JX_ERR_INVALID, "q_stride/kv_stride smaller than the layer's rows");
+    if (static_cast<uint64_t>(a->n_seqs) * n_layers > 0x7FFFFFFFull)
+        return pfail(JX_ERR_INVALID, "too many rows");
+    std::vector<int> writer(D.n_layers, -1);
+    for (uint32_t l = 0; l < n_layers; ++l) {
+        const jx_layer_desc& L = layers[l];
+        if (L.head_dim != D.head_dim)
+            return pfail(JX_ERR_UNSUPPORTED, "layer %u: head_dim %u, the cache has %u", l, L.head_dim, D.head_dim);
+        if (L.kv_source_layer >= D.n_layers)
+            return pfail(JX_ERR_INVALID, "layer %u: kv_source_layer %u >= %u", l, L.kv_source_layer, D.n_layers);
+        if (!(L.rope_freq_base > 0.0f) || !std::isfinite(L.rope_freq_base))
+            return pfail(JX_ERR_INVALID, "layer %u: rope_freq_base must be positive", l);
+        if (!L.shares_kv) {
+            if (writer[L.kv_source_layer] >= 0)
+                return pfail(JX_ERR_INVALID, "layers %d and %u both write cache layer %u",
+                             writer[L.kv_source_layer], l, L.kv_source_layer);
+            writer[L.kv_source_layer] = static_cast<int>(l);
+        }
+    }
+    // runs: rows of one sequence at consecutive positions
+    std::vector<PagedRun> runs;
+    std::vector<char> seen(D.n_seqs, 0);
+    bool any_write = false;
+    for (uint32_t l = 0; l < n_layers; ++l) any_write = any_write || !layers[l].shares_kv;
+    for (uint32_t i = 0; i < a->n_seqs; ++i) {
+        const int sid = a->seq_ids ? a->seq_ids[i] : (prompt ? 0 : static_cast<int>(i));
+        if (sid < 0 || static_cast<uint32_t>(sid) >= D.n_seqs)
+            return pfail(JX_ERR_INVALID, "sequence id %d outside [0, %u)", sid, D.n_seqs);
+        const int p = a->pos[i];
+        if (p < 0) return pfail(JX_ERR_INVALID, "negative position");
+        if (static_cast<uint32_t>(p) >= D.capacity)
+            return pfail(JX_ERR_RANGE, "position %d is beyond the capacity of %u rows", p, D.capacity);
+        if (!runs.empty() && runs.back().seq == sid) {
+            if (!prompt) return pfail(JX_ERR_INVALID, "sequence id %d listed twice", sid);
+            PagedRun& r = runs.back();
+            if (p != r.pos0 + r.n)
+                return pfail(JX_ERR_INVALID, "a prompt's rows of one sequence must ascend by one "
+                             "(sequence %d: position %d after %d)", sid, p, r.pos0 + r.n - 1);
+            ++r.n;
+            continue;
+        }
+        if (seen[sid]) return pfail(JX_ERR_INVALID, prompt ? "the rows of sequence %d must stand together"
+                                                           : "sequence id %d listed twice", sid);
+        seen[sid] = 1;
+        runs.push_back(PagedRun{sid, p, 1, static_cast<int>(i), 0, 0});
+    }
+    std::vector<Span> spans;
+    for (const PagedRun& r : runs) {
+        const uint32_t held = kv->rows[r.seq], end = static_cast<uint32_t>(r.pos0 + r.n);
+        if (any_write ? static_cast<uint32_t>(r.pos0) > held : end > held)
+            return pfail(JX_ERR_RANGE, "sequence %d holds %u rows: position %d leaves a gap", r.seq, held, r.pos0);
+        spans.push_back(Span{static_cast<uint32_t>(r.seq), static_cast<uint32_t>(r.pos0), end});
+    }
+    const void* ptrs[4] = {a->q, a->k, a->v, a->out};
+    const char* names[4] = {"q", "k", "v", "out"};
+    OnDevice on(D.device);
+    if (!on.ok) return pfail(JX_ERR_CUDA, "cannot select device %d", D.device);
+    for (int i = 0; i < 4; ++i)
+        if (int rc = check_device_ptr(ptrs[i], names[i], D.device)) return rc;
+    if (int rc = refuse_capture(st)) return rc;
+    std::vector<PagedLayer> all(n_layers);
+    PagedArgs A{};
+    for (uint32_t l = 0; l < n_layers; ++l) {
+        const jx_layer_desc& L = layers[l];
+        int cfg = 0;
+        if (int rc = rope_table(kv, L, a->yarn_scale, a->rope_neox != 0, st, &cfg)) return rc;
+        all[l].cache_layer = static_cast<uint16_t>(L.kv_source_layer);
+        all[l].io = static_cast<uint16_t>(l);
+        all[l].half = static_cast<uint16_t>(std::min(L.head_dim, L.rope_dim) / 2);
+        all[l].cfg = static_cast<uint8_t>(cfg);
+        all[l].flags = static_cast<uint8_t>((L.is_swa && a->sliding_window > 0 ? kLayerWindow : 0) |
+                                            (L.shares_kv ? 0 : kLayerAppend));
+    }
+    if (any_write) {
+        if (int rc = make_room(kv, spans, st)) return rc;
+        for (const Span& s : spans) {
+            drop_rows(kv, s.seq, s.end);
+            kv->rows[s.seq] = s.end;
+        }
+    }
+    for (size_t i = 0; i < kv->ropes.size(); ++i) A.rope[i] = kv->ropes[i].d_tab;
+    A.pool = kv->pool;
+    A.table = kv->d_table;
+    A.page_bytes = kv->page_bytes;
+    A.layer_bytes = kv->layer_bytes;
+    A.max_pages = static_cast<int>(kv->max_pages);
+    A.n_kv = static_cast<int>(D.n_kv_heads);
+    A.G = static_cast<int>(G);
+    A.n_io_layers = static_cast<int>(n_layers);
+    A.q = a->q;
+    A.k_in = a->k;
+    A.v_in = a->v;
+    A.out = a->out;
+    A.q_stride = a->q_stride;
+    A.kv_stride = a->kv_stride;
+    A.scale = a->scale;
+    A.softcap = a->softcap;
+    A.inv_softcap = a->softcap > 0.0f ? 1.0f / a->softcap : 0.0f;
+    A.window = static_cast<int>(std::min<uint32_t>(a->sliding_window, 0x7FFFFFFFu));
+    A.neox = a->rope_neox != 0 ? 1 : 0;
+    A.err = kv->d_err;
+    A.dbg = kv->d_dbg;
+    A.wait_limit = wait_limit_cycles(kv->opt_wait_limit_ms);
+    int launches = 0;
+    // the rows of every layer first, then attention
+    for (int pass = 0; pass < 2; ++pass) {
+        std::vector<PagedLayer> part;
+        for (const PagedLayer& L : all)
+            if (pass == 1 || (L.flags & kLayerAppend)) part.push_back(L);
+        for (size_t l0 = 0; l0 < part.size(); l0 += kMaxCallLayers) {
+            A.n_layers = static_cast<int>(std::min<size_t>(kMaxCallLayers, part.size() - l0));
+            std::copy_n(part.begin() + l0, A.n_layers, A.layers);
+            for (size_t r0 = 0; r0 < runs.size(); r0 += kMaxRuns) {
+                A.n_runs = static_cast<int>(std::min<size_t>(kMaxRuns, runs.size() - r0));
+                int total = 0;
+                for (int i = 0; i < A.n_runs; ++i) {
+                    PagedRun r = runs[r0 + i];
+                    r.off = total;
+                    total += pass == 0 ? (r.pos0 + r.n - 1) / kBlockRows - r.pos0 / kBlockRows + 1 : r.n;
+                    A.runs[i] = r;
+                }
+                const dim3 grid(total, static_cast<unsigned>(A.n_layers * A.n_kv));
+                dispatch(D, [&](auto hd, auto dt) {
+                    if (pass == 0) append_kernel<hd.value, dt.value><<<grid, 2 * hd.value, 0, st>>>(A);
+                    else attend_kernel<hd.value, dt.value><<<grid, 128, 0, st>>>(A);
+                });
+                ++launches;
+                if (int rc = launched(pass == 0 ? "append" : "attention")) return rc;
+            }
+        }
+    }
+    kv->last_launches = launches;
+    return JX_OK;
+}
+
+// Device and pinned buffers of at least n ints for keep's row list.
+int ensure_rows(jx_pkv* kv, size_t n) {
+    if (!kv->ev_rows) PKV_CUDA(cudaEventCreateWithFlags(&kv->ev_rows, cudaEventDisableTiming));
+    else PKV_CUDA(cudaEventSynchronize(kv->ev_rows));  // the last list has left the pinned buffer
+    if (kv->h_rows_n < n) {
+        if (kv->h_rows) PKV_CUDA(cudaFreeHost(kv->h_rows));
+        kv->h_rows = nullptr;
+        kv->h_rows_n = 0;
+        if (cudaHostAlloc(reinterpret_cast<void**>(&kv->h_rows), 2 * n * sizeof(int), cudaHostAllocDefault) != cudaSuccess) {
+            cudaGetLastError();
+            return pfail(JX_ERR_NOMEM, "pinned buffer of %zu bytes failed", 2 * n * sizeof(int));
+        }
+        kv->h_rows_n = 2 * n;
+    }
+    if (kv->d_rows_n < n) {
+        if (kv->d_rows) PKV_CUDA(cudaFree(kv->d_rows));  // (waits for the device)
+        kv->d_rows = nullptr;
+        kv->d_rows_n = 0;
+        if (cudaMalloc(&kv->d_rows, 2 * n * sizeof(int)) != cudaSuccess) {
+            cudaGetLastError();
+            return pfail(JX_ERR_NOMEM, "row list of %zu bytes failed", 2 * n * sizeof(int));
+        }
+        kv->d_rows_n = 2 * n;
+    }
+    return JX_OK;
+}
+
+int keep_impl(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, cudaStream_t st) {
+    const jx_pkv_desc& D = kv->d;
+    OnDevice on(D.device);
+    if (!on.ok) return pfail(JX_ERR_CUDA, "cannot select device %d", D.device);
+    if (int rc = refuse_capture(st)) return rc;
+    uint32_t same = 0;  // leading rows that stay in place
+    while (same < n_rows && rows[same] == static_cast<int32_t>(same)) ++same;
+    if (same == n_rows) {  // nothing moves
+        drop_rows(kv, seq, n_rows);
+        return JX_OK;
+    }
+    auto& pg = kv->pages[seq];
+    const uint32_t keep_pages = same / kPageRows, n_pages = pages_for(n_rows);
+    const uint32_t fresh = n_pages - keep_pages;
+    bool shared = false;
+    for (uint32_t i = keep_pages; i < n_pages; ++i) shared = shared || kv->refs[pg[i]] > 1;
+    const bool in_place = fresh > kv->free_pages.size();
+    if (in_place && shared)
+        return pfail(JX_ERR_NOMEM, "%u pages are needed (the sequence shares its own), %zu of %u are free",
+                     fresh, kv->free_pages.size(), D.n_pages);
+    // [rows][source pages][result pages]
+    const size_t n_src = pg.size(), n_list = n_rows + n_src + n_pages;
+    if (int rc = ensure_rows(kv, n_list)) return rc;
+    std::memcpy(kv->h_rows, rows, n_rows * sizeof(int));
+    std::memcpy(kv->h_rows + n_rows, pg.data(), n_src * sizeof(int));
+    std::vector<int> result(pg.begin(), pg.begin() + n_pages);
+    if (!in_place)
+        for (uint32_t i = keep_pages; i < n_pages; ++i) result[i] = take_page(kv);
+    std::memcpy(kv->h_rows + n_rows + n_src, result.data(), n_pages * sizeof(int));
+    PKV_CUDA(cudaMemcpyAsync(kv->d_rows, kv->h_rows, n_list * sizeof(int), cudaMemcpyHostToDevice, st));
+    PKV_CUDA(cudaEventRecord(kv->ev_rows, st));
+    KeepArgs k{};
+    k.pool = kv->pool;
+    k.rows = kv->d_rows;
+    k.src_table = kv->d_rows + n_rows;
+    k.dst_table = kv->d_rows + n_rows + n_src;
+    k.page_bytes = kv->page_bytes;
+    k.n_rec = static_cast<int>(D.n_layers * D.n_kv_heads);
+    k.n_rows = static_cast<int>(n_rows);
+    k.blk0 = static_cast<int>(keep_pages * (kPageRows / kBlockRows));
+    k.n_blk = static_cast<int>((n_rows + kBlockRows - 1) / kBlockRows) - k.blk0;
+    k.serial = in_place ? 1 : 0;
+    const dim3 grid(in_place ? 1 : k.n_blk, k.n_rec);
+    dispatch(D, [&](auto hd, auto dt) {
+        keep_kernel<hd.value, dt.value><<<grid, 2 * hd.value, 0, st>>>(k);
+    });
+    if (int rc = launched("keep")) return rc;
+    if (in_place) {
+        drop_rows(kv, seq, n_rows);
+        return JX_OK;
+    }
+    std::vector<TableEntry> table;
+    for (uint32_t i = keep_pages; i < n_pages; ++i) table.push_back({seq, i, result[i]});
+    for (size_t i = keep_pages; i < pg.size(); ++i) give_back(kv, pg[i]);
+    pg = std::move(result);
+    kv->rows[seq] = n_rows;
+    return set_table(kv, table, st);
+}
+
+bool bad_seq(const jx_pkv* kv, uint32_t seq) { return !kv || seq >= kv->d.n_seqs; }
+
+// No C++ exception crosses the C boundary.
+template <typename F>
+int guarded(F&& f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc&) {
+        return pfail(JX_ERR_NOMEM, "out of host memory");
+    } catch (...) {
+        return pfail(JX_ERR_INVALID, "unexpected exception");
+    }
+}
+
+}  // namespace
+
+// ================================================================== C ABI
+
+extern "C" {
+
+int jx_pkv_create(const jx_pkv_desc* desc, jx_pkv** out) {
+    return guarded([&]() -> int {
+        if (!desc || !out) return pfail(JX_ERR_INVALID, "null desc/out");
+        *out = nullptr;
+        const jx_pkv_desc& d = *desc;
+        if (d.n_seqs == 0 || d.n_layers == 0 || d.capacity == 0 || d.n_kv_heads == 0 || d.n_pages == 0)
+            return pfail(JX_ERR_INVALID, "n_seqs, n_layers, capacity, n_kv_heads and n_pages must be positive");
+        if (d.dtype != JX_I8 && d.dtype != JX_E4M3)
+            return pfail(JX_ERR_INVALID, "dtype %d: a paged cache holds JX_I8 or JX_E4M3", d.dtype);
+        if (d.head_dim != 32 && d.head_dim != 64 && d.head_dim != 128 && d.head_dim != 256)
+            return pfail(JX_ERR_UNSUPPORTED, "head_dim %u (compiled: 32, 64, 128, 256)", d.head_dim);
+        if (d.n_layers > 65535 || d.n_kv_heads > 512 ||
+            static_cast<uint64_t>(d.n_layers) * d.n_kv_heads > 65535)
+            return pfail(JX_ERR_UNSUPPORTED, "n_kv_heads must be at most 512, n_layers * n_kv_heads at most 65535");
+        if (d.capacity > (1u << 30) || d.n_pages > (1u << 30) ||
+            static_cast<uint64_t>(d.n_seqs) * ((d.capacity + kPageRows - 1) / kPageRows) > (1ull << 30))
+            return pfail(JX_ERR_INVALID, "capacity, n_pages and the page table must stay below 2^30 entries");
+        int ndev = 0;
+        if (cudaGetDeviceCount(&ndev) != cudaSuccess || ndev == 0) {
+            cudaGetLastError();
+            return pfail(JX_ERR_CUDA, "no CUDA device (this library has no CPU path)");
+        }
+        if (d.device < 0 || d.device >= ndev) return pfail(JX_ERR_INVALID, "device %d absent", d.device);
+        OnDevice on(d.device);
+        if (!on.ok) return pfail(JX_ERR_CUDA, "cannot select device %d", d.device);
+        int major = 0, sms = 0;
+        PKV_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, d.device));
+        PKV_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d.device));
+        if (major < 10) return pfail(JX_ERR_UNSUPPORTED, "device %d is older than this build's target, sm_100a", d.device);
+        jx_pkv* kv = new jx_pkv();
+        auto undo = [&](int code) {
+            jx_pkv_destroy(kv);
+            return code;
+        };
+        kv->d = d;
+        kv->num_sms = sms;
+        kv->layer_bytes = static_cast<long long>(d.n_kv_heads) * record_bytes(static_cast<int>(d.head_dim));
+        kv->page_bytes = kv->layer_bytes * d.n_layers;
+        kv->max_pages = pages_for(d.capacity);
+        kv->refs.assign(d.n_pages, 0);
+        kv->pages.resize(d.n_seqs);
+        kv->rows.assign(d.n_seqs, 0);
+        kv->free_pages.resize(d.n_pages);
+        for (uint32_t i = 0; i < d.n_pages; ++i) kv->free_pages[i] = static_cast<int>(d.n_pages - 1 - i);
+        const size_t bytes = static_cast<size_t>(kv->page_bytes) * d.n_pages;
+        const size_t tb = static_cast<size_t>(d.n_seqs) * kv->max_pages * sizeof(int);
+        if (cudaMalloc(&kv->pool, bytes) != cudaSuccess || cudaMalloc(&kv->d_table, tb) != cudaSuccess) {
+            cudaGetLastError();
+            return undo(pfail(JX_ERR_NOMEM, "page pool of %zu bytes failed", bytes));
+        }
+        if (cudaMemset(kv->pool, 0, bytes) != cudaSuccess || cudaMemset(kv->d_table, 0, tb) != cudaSuccess ||
+            cudaMalloc(&kv->d_err, sizeof(int)) != cudaSuccess || cudaMemset(kv->d_err, 0, sizeof(int)) != cudaSuccess ||
+            cudaMalloc(&kv->d_dbg, 8 * sizeof(int)) != cudaSuccess ||
+            cudaMemset(kv->d_dbg, 0, 8 * sizeof(int)) != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) {
+            cudaGetLastError();
+            return undo(pfail(JX_ERR_CUDA, "cache initialisation failed"));
+        }
+        *out = kv;
+        return JX_OK;
+    });
+}
+
+int jx_pkv_destroy(jx_pkv* kv) {
+    if (!kv) return JX_OK;
+    OnDevice on(kv->d.device);
+    cudaDeviceSynchronize();
+    cudaFree(kv->pool);
+    cudaFree(kv->d_table);
+    cudaFree(kv->d_err);
+    cudaFree(kv->d_dbg);
+    cudaFree(kv->d_rows);
+    if (kv->h_rows) cudaFreeHost(kv->h_rows);
+    if (kv->ev_rows) cudaEventDestroy(kv->ev_rows);
+    for (RopeCfg& r : kv->ropes) cudaFree(r.d_tab);
+    delete kv;
+    return JX_OK;
+}
+
+int jx_pkv_get_desc(const jx_pkv* kv, jx_pkv_desc* desc) {
+    if (!kv || !desc) return pfail(JX_ERR_INVALID, "null argument");
+    *desc = kv->d;
+    return JX_OK;
+}
+
+int jx_pkv_get_seq_pos(const jx_pkv* kv, uint32_t seq, uint32_t* seq_pos) {
+    if (bad_seq(kv, seq) || !seq_pos) return pfail(JX_ERR_INVALID, "bad handle/sequence");
+    *seq_pos = kv->rows[seq];
+    return JX_OK;
+}
+
+int jx_pkv_set_seq_pos(jx_pkv* kv, uint32_t seq, uint32_t seq_pos) {
+    if (bad_seq(kv, seq)) return pfail(JX_ERR_INVALID, "bad handle/sequence");
+    if (seq_pos > kv->rows[seq])
+        return pfail(JX_ERR_RANGE, "sequence %u holds %u rows, not %u", seq, kv->rows[seq], seq_pos);
+    return jx_pkv_rollback(kv, seq, seq_pos);
+}
+
+int jx_pkv_free_pages(const jx_pkv* kv, uint32_t* n) {
+    if (!kv || !n) return pfail(JX_ERR_INVALID, "null argument");
+    *n = static_cast<uint32_t>(kv->free_pages.size());
+    return JX_OK;
+}
+
+int jx_pkv_held_pages(const jx_pkv* kv, uint32_t seq, uint32_t* n) {
+    if (bad_seq(kv, seq) || !n) return pfail(JX_ERR_INVALID, "bad handle/sequence");
+    *n = static_cast<uint32_t>(kv->pages[seq].size());
+    return JX_OK;
+}
+
+int jx_pkv_clear(jx_pkv* kv, uint32_t seq) { return jx_pkv_rollback(kv, seq, 0); }
+
+int jx_pkv_rollback(jx_pkv* kv, uint32_t seq, uint32_t new_seq_pos) {
+    return guarded([&]() -> int {
+        if (bad_seq(kv, seq)) return pfail(JX_ERR_INVALID, "bad handle/sequence");
+        if (new_seq_pos < kv->rows[seq]) drop_rows(kv, seq, new_seq_pos);
+        return JX_OK;
+    });
+}
+
+int jx_pkv_fork(jx_pkv* kv, uint32_t src, uint32_t dst, uint32_t n_rows, void* stream) {
+    return guarded([&]() -> int {
+        if (bad_seq(kv, src) || bad_seq(kv, dst) || src == dst)
+            return pfail(JX_ERR_INVALID, "bad handle/sequence, or a sequence forked into itself");
+        if (n_rows > kv->rows[src])
+            return pfail(JX_ERR_RANGE, "sequence %u holds %u rows, not %u", src, kv->rows[src], n_rows);
+        OnDevice on(kv->d.device);
+        if (!on.ok) return pfail(JX_ERR_CUDA, "cannot select device %d", kv->d.device);
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (int rc = refuse_capture(st)) return rc;
+        const uint32_t n = pages_for(n_rows);
+        std::vector<int> pg(kv->pages[src].begin(), kv->pages[src].begin() + n);
+        for (int p : pg) ++kv->refs[p];  // before dst's are given back: it may hold the same pages
+        drop_rows(kv, dst, 0);
+        kv->pages[dst] = std::move(pg);
+        kv->rows[dst] = n_rows;
+        if (n == 0) return JX_OK;
+        table_copy_kernel<<<std::min<uint32_t>((n + 255) / 256, 148), 256, 0, st>>>(
+            kv->d_table + static_cast<size_t>(dst) * kv->max_pages,
+            kv->d_table + static_cast<size_t>(src) * kv->max_pages, static_cast<int>(n));
+        return launched("page table copy");
+    });
+}
+
+int jx_pkv_copy(jx_pkv* kv, uint32_t src, uint32_t dst, void* stream) {
+    return guarded([&]() -> int {
+        if (bad_seq(kv, src) || bad_seq(kv, dst) || src == dst)
+            return pfail(JX_ERR_INVALID, "bad handle/sequence, or a sequence copied into itself");
+        OnDevice on(kv->d.device);
+        if (!on.ok) return pfail(JX_ERR_CUDA, "cannot select device %d", kv->d.device);
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (int rc = refuse_capture(st)) return rc;
+        const auto& from = kv->pages[src];
+        size_t freed = 0;  // pages that only dst holds come free first
+        for (int p : kv->pages[dst]) freed += kv->refs[p] == 1;
+        if (from.size() > kv->free_pages.size() + freed)
+            return pfail(JX_ERR_NOMEM, "%zu pages are needed, %zu of %u are free", from.size(),
+                         kv->free_pages.size() + freed, kv->d.n_pages);
+        drop_rows(kv, dst, 0);
+        std::vector<TableEntry> table;
+        std::vector<std::pair<int, int>> copies;
+        for (size_t i = 0; i < from.size(); ++i) {
+            const int p = take_page(kv);
+            kv->pages[dst].push_back(p);
+            copies.emplace_back(from[i], p);
+            table.push_back({dst, static_cast<uint32_t>(i), p});
+        }
+        kv->rows[dst] = kv->rows[src];
+        if (int rc = copy_pages(kv, copies, st)) return rc;
+        return set_table(kv, table, st);
+    });
+}
+
+int jx_pkv_keep(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, void* stream) {
+    return guarded([&]() -> int {
+        if (bad_seq(kv, seq) || (!rows && n_rows > 0)) return pfail(JX_ERR_INVALID, "bad handle/sequence/rows");
+        for (uint32_t i = 0; i < n_rows; ++i)
+            if (rows[i] < 0 || static_cast<uint32_t>(rows[i]) >= kv->rows[seq] || (i > 0 && rows[i] <= rows[i - 1]))
+                return pfail(JX_ERR_INVALID, "rows must ascend and stay below %u (entry %u is %d)", kv->rows[seq], i, rows[i]);
+        return keep_impl(kv, seq, rows, n_rows, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int jx_pkv_compact(jx_pkv* kv, uint32_t seq, uint32_t keep_recent, void* stream) {
+    return guarded([&]() -> int {
+        if (bad_seq(kv, seq)) return pfail(JX_ERR_INVALID, "bad handle/sequence");
+        const uint32_t sink = 4, sp = kv->rows[seq];
+        if (static_cast<uint64_t>(sp) <= static_cast<uint64_t>(sink) + keep_recent) return JX_OK;
+        std::vector<int32_t> rows;
+        rows.reserve(sink + keep_recent);
+        for (uint32_t i = 0; i < sink; ++i) rows.push_back(static_cast<int32_t>(i));
+        for (uint32_t i = sp - keep_recent; i < sp; ++i) rows.push_back(static_cast<int32_t>(i));
+        return keep_impl(kv, seq, rows.data(), static_cast<uint32_t>(rows.size()), static_cast<cudaStream_t>(stream));
+    });
+}
+
+int jx_pkv_load_rows(jx_pkv* kv, uint32_t seq, uint32_t row0, uint32_t n_rows, const void* k_codes,
+                     const float* k_scales, const void* v_codes, const float* v_scales, void* stream) {
+    return guarded([&]() -> int {
+        if (bad_seq(kv, seq)) return pfail(JX_ERR_INVALID, "bad handle/sequence");
+        const jx_pkv_desc& D = kv->d;
+        if (n_rows == 0) return JX_OK;
+        if (row0 % kBlockRows != 0) return pfail(JX_ERR_INVALID, "row0 must be a multiple of %d", kBlockRows);
+        if (static_cast<uint64_t>(row0) + n_rows > D.capacity || row0 > kv->rows[seq])
+            return pfail(JX_ERR_RANGE, "rows [%u, %llu): the sequence holds %u, its capacity is %u", row0,
+                         static_cast<unsigned long long>(row0) + n_rows, kv->rows[seq], D.capacity);
+        OnDevice on(D.device);
+        if (!on.ok) return pfail(JX_ERR_CUDA, "cannot select device %d", D.device);
+        const void* ptrs[4] = {k_codes, k_scales, v_codes, v_scales};
+        const char* names[4] = {"k_codes", "k_scales", "v_codes", "v_scales"};
+        for (int i = 0; i < 4; ++i) {
+            if (int rc = check_device_ptr(ptrs[i], names[i], D.device)) return rc;
+            if (reinterpret_cast<uintptr_t>(ptrs[i]) % (i % 2 ? 4 : 16) != 0)
+                return pfail(JX_ERR_INVALID, "%s must be aligned to %d bytes", names[i], i % 2 ? 4 : 16);
+        }
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (int rc = refuse_capture(st)) return rc;
+        if (int rc = make_room(kv, {Span{seq, row0, row0 + n_rows}}, st)) return rc;
+        drop_rows(kv, seq, row0 + n_rows);
+        kv->rows[seq] = row0 + n_rows;
+        LoadArgs a{};
+        a.pool = kv->pool;
+        a.table = kv->d_table + static_cast<size_t>(seq) * kv->max_pages;
+        a.codes[0] = static_cast<const unsigned char*>(k_codes);
+        a.codes[1] = static_cast<const unsigned char*>(v_codes);
+        a.scales[0] = k_scales;
+        a.scales[1] = v_scales;
+        a.page_bytes = kv->page_bytes;
+        a.row0 = static_cast<int>(row0);
+        a.n_rows = static_cast<int>(n_rows);
+        a.n_kv = static_cast<int>(D.n_kv_heads);
+        a.n_layers = static_cast<int>(D.n_layers);
+        const long long n = static_cast<long long>(D.n_layers) * n_rows * D.n_kv_heads * (D.head_dim / 16);
+        const dim3 grid(static_cast<unsigned>(std::min<long long>((n + 255) / 256, 8ll * kv->num_sms)), 2);
+        dispatch(D, [&](auto hd, auto dt) { load_kernel<hd.value, dt.value><<<grid, 256, 0, st>>>(a); });
+        return launched("load");
+    });
+}
+
+int jx_pkv_read_rows(jx_pkv* kv, const int32_t* seq_ids, const int32_t* row0, uint32_t n, uint32_t n_rows,
+                     int32_t dtype, void* out, void* stream) {
+    return guarded([&]() -> int {
+        if (!kv || !seq_ids || !row0) return pfail(JX_ERR_INVALID, "null argument");
+        const jx_pkv_desc& D = kv->d;
+        if (dtype != JX_F32 && dtype != JX_BF16) return pfail(JX_ERR_INVALID, "rows are read as JX_F32 or JX_BF16");
+        for (uint32_t i = 0; i < n; ++i) {
+            if (seq_ids[i] < 0 || bad_seq(kv, static_cast<uint32_t>(seq_ids[i])))
+                return pfail(JX_ERR_INVALID, "sequence id %d outside [0, %u)", seq_ids[i], D.n_seqs);
+            if (row0[i] < 0 || static_cast<uint64_t>(row0[i]) + n_rows > kv->rows[seq_ids[i]])
+                return pfail(JX_ERR_RANGE, "sequence %d holds %u rows, not [%d, %lld)", seq_ids[i],
+                             kv->rows[seq_ids[i]], row0[i], static_cast<long long>(row0[i]) + n_rows);
+        }
+        if (n == 0 || n_rows == 0) return JX_OK;
+        OnDevice on(D.device);
+        if (!on.ok) return pfail(JX_ERR_CUDA, "cannot select device %d", D.device);
+        if (int rc = check_device_ptr(out, "out", D.device)) return rc;
+        if (reinterpret_cast<uintptr_t>(out) % 16 != 0) return pfail(JX_ERR_INVALID, "out must be aligned to 16 bytes");
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        if (int rc = refuse_capture(st)) return rc;
+        ReadArgs a{};
+        a.pool = kv->pool;
+        a.table = kv->d_table;
+        a.page_bytes = kv->page_bytes;
+        a.max_pages = static_cast<int>(kv->max_pages);
+        a.n_kv = static_cast<int>(D.n_kv_heads);
+        a.n_layers = static_cast<int>(D.n_layers);
+        a.n_rows = static_cast<int>(n_rows);
+        const long long per = static_cast<long long>(D.n_layers) * 2 * n_rows * D.n_kv_heads * (D.head_dim / 16);
+        for (uint32_t s0 = 0; s0 < n; s0 += kMaxRuns) {
+            a.n = static_cast<int>(std::min<uint32_t>(kMaxRuns, n - s0));
+            std::copy_n(seq_ids + s0, a.n, a.seq);
+            std::copy_n(row0 + s0, a.n, a.row0);
+            a.out = static_cast<char*>(out) + static_cast<size_t>(s0) * per * 16 * (dtype == JX_F32 ? 4 : 2);
+            const dim3 grid(static_cast<unsigned>(std::min<long long>((per + 255) / 256, 16ll * kv->num_sms)), a.n);
+            dispatch(D, [&](auto hd, auto dt) {
+                if (dtype == JX_F32) read_kernel<hd.value, dt.value, true><<<grid, 256, 0, st>>>(a);
+                else read_kernel<hd.value, dt.value, false><<<grid, 256, 0, st>>>(a);
+            });
+            if (int rc = launched("read")) return rc;
+        }
+        return JX_OK;
+    });
+}
+
+int jx_pkv_attn_step(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const jx_step_args* args,
+                     void* stream) {
+    return guarded([&]() -> int {
+        return attn_call(kv, layers, n_layers, args, static_cast<cudaStream_t>(stream), false);
+    });
+}
+
+int jx_pkv_attn_prefill(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const jx_step_args* args,
+                        void* stream) {
+    return guarded([&]() -> int {
+        return attn_call(kv, layers, n_layers, args, static_cast<cudaStream_t>(stream), true);
+    });
+}
+
+int jx_pkv_check_device_error(jx_pkv* kv, int* code, void* stream) {
+    if (!kv || !code) return pfail(JX_ERR_INVALID, "null argument");
+    OnDevice on(kv->d.device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int h = 0, dbg[8] = {0};
+    PKV_CUDA(cudaMemcpyAsync(&h, kv->d_err, sizeof(int), cudaMemcpyDeviceToHost, st));
+    PKV_CUDA(cudaMemcpyAsync(dbg, kv->d_dbg, sizeof dbg, cudaMemcpyDeviceToHost, st));
+    PKV_CUDA(cudaStreamSynchronize(st));
+    PKV_CUDA(cudaMemsetAsync(kv->d_err, 0, sizeof(int), st));
+    PKV_CUDA(cudaMemsetAsync(kv->d_dbg, 0, sizeof dbg, st));
+    PKV_CUDA(cudaStreamSynchronize(st));
+    *code = h;
+    if (h)
+        return pfail(JX_ERR_DEVICE, "a kernel's bounded wait ran out: site %d block %d thread %d index %d (error %d)",
+                     dbg[0] - 100, dbg[1], dbg[2], dbg[5], h);
+    return JX_OK;
+}
+
+int jx_pkv_set_option(jx_pkv* kv, const char* key, int value) {
+    if (!kv || !key) return pfail(JX_ERR_INVALID, "null argument");
+    if (std::strcmp(key, "wait_limit_ms") == 0) {
+        if (value < 0) return pfail(JX_ERR_INVALID, "wait_limit_ms must not be negative");
+        kv->opt_wait_limit_ms = value;
+        return JX_OK;
+    }
+    return pfail(JX_ERR_INVALID, "unknown option '%s'", key);
+}
+
+int jx_pkv_last_launch_count(const jx_pkv* kv, int* count) {
+    if (!kv || !count) return pfail(JX_ERR_INVALID, "null argument");
+    *count = kv->last_launches;
+    return JX_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,159 @@
+// jx_paged.h -- types and device helpers of the paged 8-bit KV cache, shared by
+// its host side and its kernels.
+//
+// A page holds kPageRows consecutive rows of one sequence for every layer.  It
+// is a run of records, one per (layer, kv head):
+//   K codes [32][HD] bytes, V codes [32][HD] bytes, scales {K0, K1, V0, V1}
+// where K0 / V0 scale rows 0-15 and K1 / V1 rows 16-31 (fp32 powers of two).
+// Inside a 32-row tile the 16-byte chunks of each 128-byte line are permuted
+// (chunk ^= line & 7), so that both the row-wise reads of K and the 8x8 matrix
+// loads of V are free of bank conflicts once a record lies in shared memory.
+// A record is one contiguous, 16-byte aligned run (HD*64 + 16 bytes): one bulk
+// copy brings everything attention needs of 32 rows, scales included.
+// int8 codes are stored offset by 128 (one byte permute then builds the fp16
+// number 1024 + u); e4m3 codes as they are.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace jx {
+
+enum { DT_I8 = 3, DT_E4M3 = 4 };  // = jx_dtype JX_I8, JX_E4M3
+
+constexpr int kPageRows = 32;
+constexpr int kBlockRows = 16;     // rows that share a scale
+constexpr int kMinExp = -40;       // scale exponents: a block of zeros has the smallest
+constexpr int kMaxExp = 56;
+constexpr float kClip = 4.611686018427387904e18f;  // 2^62: larger magnitudes are held as this one
+
+constexpr int kMaxRuns = 128;      // runs and layers of one launch: its plan travels in the
+constexpr int kMaxCallLayers = 64; // kernel's parameters (no upload, nothing to outlive the call)
+constexpr int kMaxRopeCfgs = 8;
+
+// Consecutive tokens of one sequence: rows io0 .. io0+n-1 of the call, at
+// positions pos0 .. pos0+n-1.
+struct PagedRun {
+    int seq;
+    int pos0;
+    int n;
+    int io0;
+    int off;  // first work unit of the run (meaning: the kernel's)
+    int off1;
+};
+
+struct PagedLayer {
+    uint16_t cache_layer;
+    uint16_t io;    // layer index within the call's rows
+    uint16_t half;  // rotated pairs per head
+    uint8_t cfg;    // rope table
+    uint8_t flags;  // kLayerWindow | kLayerAppend
+};
+constexpr int kLayerWindow = 1, kLayerAppend = 2;
+
+struct PagedArgs {
+    unsigned char* pool;
+    const int* table;       // [n_seqs][max_pages] page of every 32 rows
+    long long page_bytes;
+    long long layer_bytes;  // n_kv * record
+    int max_pages;
+    int n_kv;
+    int G;
+    int n_io_layers;        // layers of the call: row r, layer l is io row r*n_io_layers + l
+    const float* q;
+    const float* k_in;
+    const float* v_in;
+    float* out;
+    long long q_stride;
+    long long kv_stride;
+    float scale;
+    float softcap;
+    float inv_softcap;
+    int window;
+    int neox;
+    int n_runs;
+    int n_layers;
+    int total;              // work units
+    const float2* rope[kMaxRopeCfgs];  // [capacity][HD/2] (cos, sin)
+    float* scratch;
+    int* counters;
+    int* err;
+    int* dbg;
+    long long wait_limit;
+    PagedLayer layers[kMaxCallLayers];
+    PagedRun runs[kMaxRuns];
+};
+static_assert(sizeof(PagedArgs) <= 4096, "kernel parameters");
+
+__host__ __device__ constexpr int record_bytes(int hd) { return 2 * kPageRows * hd + 16; }
+
+// Byte of (row, dim) inside a K or V tile of a record.
+__host__ __device__ __forceinline__ uint32_t tile_byte(int hd, int row, int d) {
+    const uint32_t off = static_cast<uint32_t>(row * hd + d);
+    return off ^ (((off >> 7) & 7u) << 4);
+}
+
+#ifdef __CUDACC__
+
+// ---------------------------------------------------------------- the format
+// A value as the cache takes it: NaN is 0, magnitudes are cut at 2^62.
+__device__ __forceinline__ float cache_value(float x) {
+    return x != x ? 0.0f : fminf(fmaxf(x, -kClip), kClip);
+}
+
+// Exponent k of a block whose largest magnitude is `amax`: the smallest with
+// amax <= M * 2^k (M = 127: 1.984375 * 2^6; 448: 1.75 * 2^8), cut to the range.
+template <int DT>
+__device__ __forceinline__ int block_exp(float amax) {
+    if (!(amax > 0.0f)) return kMinExp;
+    const uint32_t u = __float_as_uint(amax);
+    const int e = static_cast<int>(u >> 23) - 127;  // subnormals end up below kMinExp all the same
+    const uint32_t man = u & 0x7FFFFFu;
+    const int k = DT == DT_I8 ? e - 6 + (man > 0x7E0000u ? 1 : 0) : e - 8 + (man > 0x600000u ? 1 : 0);
+    return min(kMaxExp, max(kMinExp, k));
+}
+
+__device__ __forceinline__ float exp2_int(int k) {  // 2^k, k in the normal range
+    return __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
+}
+__device__ __forceinline__ int scale_exp(float s) {  // k of a stored scale 2^k
+    return static_cast<int>(__float_as_uint(s) >> 23) - 127;
+}
+
+// Nearest code of y = x * 2^-k (ties to even), as the stored byte, and back.
+template <int DT>
+__device__ __forceinline__ uint32_t to_code(float y) {
+    if constexpr (DT == DT_I8) {
+        return static_cast<uint32_t>(min(127, max(-127, __float2int_rn(y))) + 128);
+    } else {
+        return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+    }
+}
+template <int DT>
+__device__ __forceinline__ float from_code(uint32_t b) {
+    if constexpr (DT == DT_I8) {
+        return static_cast<float>(static_cast<int>(b) - 128);
+    } else {
+        return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(b), __NV_E4M3)));
+    }
+}
+
+// One element of a rotated head; each operation's result is an fp32 number
+// (no fused multiply-add), so that what the cache holds does not depend on
+// how the compiler contracts.  cs[j] = (cos, sin).
+__device__ __forceinline__ float rope_plain(const float* x, int d, int half, const float2* cs,
+                                            bool neox) {
+    if (d >= 2 * half) return x[d];
+    const int j = neox ? (d < half ? d : d - half) : d >> 1;
+    const bool first = neox ? d < half : (d & 1) == 0;
+    const float a = x[neox ? j : 2 * j], b = x[neox ? j + half : 2 * j + 1];
+    const float2 t = cs[j];
+    return first ? __fsub_rn(__fmul_rn(a, t.x), __fmul_rn(b, t.y))
+                 : __fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
+}
+
+#endif  // __CUDACC__
+
+}  // namespace jx
