@@ -133,23 +133,6 @@ __device__ __forceinline__ float half_max(float v, float* red, int n) {
     return m;
 }
 
-template <int DT>
-__device__ __forceinline__ uint4 pack_codes(const float (&x)[16], float inv) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        w[i] = to_code<DT>(x[4 * i] * inv) | to_code<DT>(x[4 * i + 1] * inv) << 8 |
-               to_code<DT>(x[4 * i + 2] * inv) << 16 | to_code<DT>(x[4 * i + 3] * inv) << 24;
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-template <int DT>
-__device__ __forceinline__ void unpack_codes(const uint4& c, float (&x)[16]) {
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = from_code<DT>((w[i / 4] >> (8 * (i % 4))) & 0xFFu);
-}
-
 // Rows of a call written to the cache.  One CTA per (block of 16 rows, layer,
 // kv head): its first half takes K, its second V, one thread per 16 values of
 // a row.  The block's largest magnitude gives the scale; rows that were in the
@@ -363,91 +346,6 @@ __global__ void read_kernel(const __grid_constant__ ReadArgs a) {
     }
 }
 
-// Attention of one token and kv head: a CTA of 128 threads walks its rows page
-// by page with the running maximum and sum of the softmax.
-template <int HD, int DT>
-__global__ void __launch_bounds__(128) attend_kernel(const __grid_constant__ PagedArgs a) {
-    __shared__ float q_s[8][HD];
-    __shared__ float p_s[8][kPageRows];
-    __shared__ float f_s[8];
-    const int tid = threadIdx.x;
-    int r = 0;
-    while (r + 1 < a.n_runs && a.runs[r + 1].off <= static_cast<int>(blockIdx.x)) ++r;
-    const PagedRun run = a.runs[r];
-    const int j = static_cast<int>(blockIdx.x) - run.off;
-    const int pos = run.pos0 + j;
-    const int h = blockIdx.y % a.n_kv;
-    const PagedLayer L = a.layers[blockIdx.y / a.n_kv];
-    const long long io = static_cast<long long>(run.io0 + j) * a.n_io_layers + L.io;
-    const float2* cs = a.rope[L.cfg] + static_cast<long long>(pos) * (HD / 2);
-    for (int i = tid; i < a.G * HD; i += 128)
-        q_s[i / HD][i % HD] = rope_plain(a.q + io * a.q_stride + (h * a.G + i / HD) * HD, i % HD, L.half,
-                                         cs, a.neox != 0);
-    const int lo = (L.flags & kLayerWindow) ? max(0, pos - a.window + 1) : 0;
-    float o[8][(HD + 127) / 128];
-    for (int g = 0; g < 8; ++g)
-        for (int e = 0; e < (HD + 127) / 128; ++e) o[g][e] = 0.0f;
-    float m = -INFINITY, l = 0.0f;  // of head tid / 16 (16 threads per head)
-    const int hg = tid / 16;
-    __syncthreads();
-    for (int p = lo / kPageRows; p <= pos / kPageRows; ++p) {
-        const unsigned char* rec =
-            a.pool + a.table[static_cast<long long>(run.seq) * a.max_pages + p] * a.page_bytes +
-            L.cache_layer * a.layer_bytes + static_cast<long long>(h) * record_bytes(HD);
-        const float* sc = reinterpret_cast<const float*>(rec + 2 * kPageRows * HD);
-        const int row = tid / 4, part = tid % 4, t = p * kPageRows + row;
-        float dot[8];
-        for (int g = 0; g < 8; ++g) dot[g] = 0.0f;
-        for (int d = part * (HD / 4); d < (part + 1) * (HD / 4); ++d) {
-            const float kv = from_code<DT>(rec[tile_byte(HD, row, d)]);
-            for (int g = 0; g < a.G; ++g) dot[g] += q_s[g][d] * kv;
-        }
-        for (int g = 0; g < 8; ++g) {
-            float s = dot[g];
-            s += __shfl_xor_sync(0xffffffffu, s, 1);
-            s += __shfl_xor_sync(0xffffffffu, s, 2);
-            s = s * sc[row / kBlockRows] * a.scale;
-            if (a.softcap > 0.0f) s = a.softcap * tanhf(s * a.inv_softcap);
-            if (part == 0) p_s[g][row] = (t >= lo && t <= pos) ? s : -INFINITY;
-        }
-        __syncthreads();
-        float s0 = p_s[hg][tid % 16], s1 = p_s[hg][tid % 16 + 16];
-        float mt = fmaxf(s0, s1);
-        for (int x = 8; x > 0; x >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
-        const float mn = fmaxf(m, mt);
-        const float f = m == -INFINITY ? 0.0f : __expf(m - mn);
-        s0 = s0 == -INFINITY ? 0.0f : expf(s0 - mn);
-        s1 = s1 == -INFINITY ? 0.0f : expf(s1 - mn);
-        float ls = s0 + s1;
-        for (int x = 8; x > 0; x >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, x);
-        l = l * f + ls;
-        m = mn;
-        __syncwarp();
-        p_s[hg][tid % 16] = s0 * sc[2];
-        p_s[hg][tid % 16 + 16] = s1 * sc[3];
-        if (tid % 16 == 0) f_s[hg] = f;
-        __syncthreads();
-        for (int e = 0; e < (HD + 127) / 128; ++e) {
-            const int d = tid + e * 128;
-            if (d >= HD) break;
-            for (int g = 0; g < a.G; ++g) o[g][e] *= f_s[g];
-            for (int rr = 0; rr < kPageRows; ++rr) {
-                const float v = from_code<DT>(rec[kPageRows * HD + tile_byte(HD, rr, d)]);
-                for (int g = 0; g < a.G; ++g) o[g][e] += p_s[g][rr] * v;
-            }
-        }
-        __syncthreads();
-    }
-    if (tid % 16 == 0) f_s[hg] = l;
-    __syncthreads();
-    for (int e = 0; e < (HD + 127) / 128; ++e) {
-        const int d = tid + e * 128;
-        if (d >= HD) break;
-        for (int g = 0; g < a.G; ++g)
-            a.out[io * a.q_stride + (h * a.G + g) * HD + d] = o[g][e] / f_s[g];
-    }
-}
-
 // Calls f(integral_constant<HD>, integral_constant<DT>) for a cache's format.
 template <int V>
 using Int = std::integral_constant<int, V>;
@@ -484,6 +382,8 @@ struct jx_pkv {
     std::vector<std::vector<int>> pages;  // of each sequence
     std::vector<uint32_t> rows;           // rows held by each sequence
     std::vector<RopeCfg> ropes;
+    float* d_scratch = nullptr;           // two partial results per CTA of the step kernel
+    int* d_counters = nullptr;
     int* d_err = nullptr;
     int* d_dbg = nullptr;
     int* d_rows = nullptr;                // keep: row list and source page table
@@ -667,6 +567,80 @@ int check_device_ptr(const void* p, const char* name, int device) {
     return pfail(JX_ERR_INVALID, "%s must be memory of device %d", name, device);
 }
 
+// The rows of a call written to the given layers.
+int append_rows(jx_pkv* kv, PagedArgs& A, const std::vector<PagedLayer>& part, const std::vector<PagedRun>& runs,
+                cudaStream_t st, int* launches) {
+    for (size_t l0 = 0; l0 < part.size(); l0 += kMaxCallLayers) {
+        A.n_layers = static_cast<int>(std::min<size_t>(kMaxCallLayers, part.size() - l0));
+        std::copy_n(part.begin() + l0, A.n_layers, A.layers);
+        for (size_t r0 = 0; r0 < runs.size(); r0 += kMaxRuns) {
+            A.n_runs = static_cast<int>(std::min<size_t>(kMaxRuns, runs.size() - r0));
+            A.total = 0;
+            for (int i = 0; i < A.n_runs; ++i) {
+                PagedRun r = runs[r0 + i];
+                r.off = A.total;
+                A.total += (r.pos0 + r.n - 1) / kBlockRows - r.pos0 / kBlockRows + 1;
+                A.runs[i] = r;
+            }
+            const dim3 grid(A.total, static_cast<unsigned>(A.n_layers * A.n_kv));
+            dispatch(kv->d, [&](auto hd, auto dt) {
+                append_kernel<hd.value, dt.value><<<grid, 2 * hd.value, 0, st>>>(A);
+            });
+            ++*launches;
+            if (int rc = launched("append")) return rc;
+        }
+    }
+    return JX_OK;
+}
+
+// The step kernel over the given layers and runs (of at most 8 / G tokens),
+// in as many launches as their plan takes.
+int step_rows(jx_pkv* kv, PagedArgs& A, const std::vector<PagedLayer>& part, const std::vector<PagedRun>& runs,
+              cudaStream_t st, int* launches) {
+    constexpr long long kMaxUnits = 1ll << 30;
+    for (size_t l0 = 0; l0 < part.size(); l0 += kMaxCallLayers) {
+        A.n_layers = static_cast<int>(std::min<size_t>(kMaxCallLayers, part.size() - l0));
+        std::copy_n(part.begin() + l0, A.n_layers, A.layers);
+        std::stable_partition(A.layers, A.layers + A.n_layers,
+                              [](const PagedLayer& L) { return !(L.flags & kLayerWindow); });
+        A.n_full = static_cast<int>(std::count_if(A.layers, A.layers + A.n_layers, [](const PagedLayer& L) {
+            return !(L.flags & kLayerWindow);
+        }));
+        const long long seg0 = static_cast<long long>(A.n_full) * A.n_kv;
+        const long long seg1 = static_cast<long long>(A.n_layers - A.n_full) * A.n_kv;
+        for (size_t r0 = 0; r0 < runs.size();) {
+            long long p0 = 0, p1 = 0;
+            int cols = 1;
+            A.n_runs = 0;
+            for (; A.n_runs < kMaxRuns && r0 < runs.size(); ++r0) {
+                PagedRun r = runs[r0];
+                const int last = r.pos0 + r.n - 1;
+                const int n0 = last / kPageRows + 1;
+                const int n1 = last / kPageRows - std::max(0, r.pos0 - A.window + 1) / kPageRows + 1;
+                if ((p0 + n0) * seg0 + (p1 + n1) * seg1 > kMaxUnits) {
+                    if (A.n_runs > 0) break;
+                    return pfail(JX_ERR_UNSUPPORTED, "a step over %d rows of %d layers is too large", last + 1, A.n_layers);
+                }
+                r.off = static_cast<int>(p0);
+                r.off1 = static_cast<int>(p1);
+                p0 += n0;
+                p1 += n1;
+                cols = std::max(cols, r.n * A.G);
+                A.runs[A.n_runs++] = r;
+            }
+            A.pages0 = static_cast<int>(p0);
+            A.pages1 = static_cast<int>(p1);
+            A.total0 = static_cast<int>(p0 * seg0);
+            A.total = static_cast<int>(p0 * seg0 + p1 * seg1);
+            const auto launch = kv->d.dtype == JX_I8 ? paged_step_i8 : paged_step_e4m3;
+            const cudaError_t e = launch(A, static_cast<int>(kv->d.head_dim), cols, kv->num_sms, st);
+            if (e != cudaSuccess) return pfail(JX_ERR_CUDA, "step launch failed: %s", cudaGetErrorString(e));
+            ++*launches;
+        }
+    }
+    return JX_OK;
+}
+
 int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const jx_step_args* a,
               cudaStream_t st, bool prompt) {
     if (!kv || !layers || !a) return pfail(JX_ERR_INVALID, "null handle, layers or args");
@@ -787,32 +761,35 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
     A.err = kv->d_err;
     A.dbg = kv->d_dbg;
     A.wait_limit = wait_limit_cycles(kv->opt_wait_limit_ms);
+    A.q_vec = reinterpret_cast<uintptr_t>(a->q) % 16 == 0 && a->q_stride % 4 == 0;
+    A.kv_vec = reinterpret_cast<uintptr_t>(a->k) % 16 == 0 && reinterpret_cast<uintptr_t>(a->v) % 16 == 0 &&
+               a->kv_stride % 4 == 0;
+    A.scratch = kv->d_scratch;
+    A.counters = kv->d_counters;
     int launches = 0;
-    // the rows of every layer first, then attention
-    for (int pass = 0; pass < 2; ++pass) {
+    if (prompt) {
+        // all rows of the call first
         std::vector<PagedLayer> part;
         for (const PagedLayer& L : all)
-            if (pass == 1 || (L.flags & kLayerAppend)) part.push_back(L);
-        for (size_t l0 = 0; l0 < part.size(); l0 += kMaxCallLayers) {
-            A.n_layers = static_cast<int>(std::min<size_t>(kMaxCallLayers, part.size() - l0));
-            std::copy_n(part.begin() + l0, A.n_layers, A.layers);
-            for (size_t r0 = 0; r0 < runs.size(); r0 += kMaxRuns) {
-                A.n_runs = static_cast<int>(std::min<size_t>(kMaxRuns, runs.size() - r0));
-                int total = 0;
-                for (int i = 0; i < A.n_runs; ++i) {
-                    PagedRun r = runs[r0 + i];
-                    r.off = total;
-                    total += pass == 0 ? (r.pos0 + r.n - 1) / kBlockRows - r.pos0 / kBlockRows + 1 : r.n;
-                    A.runs[i] = r;
-                }
-                const dim3 grid(total, static_cast<unsigned>(A.n_layers * A.n_kv));
-                dispatch(D, [&](auto hd, auto dt) {
-                    if (pass == 0) append_kernel<hd.value, dt.value><<<grid, 2 * hd.value, 0, st>>>(A);
-                    else attend_kernel<hd.value, dt.value><<<grid, 128, 0, st>>>(A);
-                });
-                ++launches;
-                if (int rc = launched(pass == 0 ? "append" : "attention")) return rc;
+            if (L.flags & kLayerAppend) part.push_back(L);
+        if (int rc = append_rows(kv, A, part, runs, st, &launches)) return rc;
+        // then attention, for blocks of as many tokens as fill the kernel's columns
+        const int nq = std::max(1, kStepCols / static_cast<int>(G));
+        std::vector<PagedRun> blocks;
+        for (const PagedRun& r : runs)
+            for (int j = 0; j < r.n; j += nq)
+                blocks.push_back(PagedRun{r.seq, r.pos0 + j, std::min(nq, r.n - j), r.io0 + j, 0, 0});
+        if (int rc = step_rows(kv, A, all, blocks, st, &launches)) return rc;
+    } else {
+        // a layer that reads rows another layer of the call writes goes second
+        A.append = 1;
+        for (int wave = 0; wave < 2; ++wave) {
+            std::vector<PagedLayer> part;
+            for (const PagedLayer& L : all) {
+                const bool later = !(L.flags & kLayerAppend) && writer[L.cache_layer] >= 0;
+                if (later == (wave == 1)) part.push_back(L);
             }
+            if (int rc = step_rows(kv, A, part, runs, st, &launches)) return rc;
         }
     }
     kv->last_launches = launches;
@@ -975,6 +952,13 @@ int jx_pkv_create(const jx_pkv_desc* desc, jx_pkv** out) {
             cudaGetLastError();
             return undo(pfail(JX_ERR_NOMEM, "page pool of %zu bytes failed", bytes));
         }
+        const size_t ctas = static_cast<size_t>(sms) * kStepCtasPerSm;
+        const size_t part = 2 * ctas * kStepCols * (d.head_dim + 2) * sizeof(float);
+        if (cudaMalloc(&kv->d_scratch, part) != cudaSuccess || cudaMalloc(&kv->d_counters, ctas * sizeof(int)) != cudaSuccess ||
+            cudaMemset(kv->d_counters, 0, ctas * sizeof(int)) != cudaSuccess) {
+            cudaGetLastError();
+            return undo(pfail(JX_ERR_NOMEM, "scratch of %zu bytes failed", part));
+        }
         if (cudaMemset(kv->pool, 0, bytes) != cudaSuccess || cudaMemset(kv->d_table, 0, tb) != cudaSuccess ||
             cudaMalloc(&kv->d_err, sizeof(int)) != cudaSuccess || cudaMemset(kv->d_err, 0, sizeof(int)) != cudaSuccess ||
             cudaMalloc(&kv->d_dbg, 8 * sizeof(int)) != cudaSuccess ||
@@ -993,6 +977,8 @@ int jx_pkv_destroy(jx_pkv* kv) {
     cudaDeviceSynchronize();
     cudaFree(kv->pool);
     cudaFree(kv->d_table);
+    cudaFree(kv->d_scratch);
+    cudaFree(kv->d_counters);
     cudaFree(kv->d_err);
     cudaFree(kv->d_dbg);
     cudaFree(kv->d_rows);

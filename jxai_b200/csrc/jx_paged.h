@@ -6,8 +6,9 @@
 //   K codes [32][HD] bytes, V codes [32][HD] bytes, scales {K0, K1, V0, V1}
 // where K0 / V0 scale rows 0-15 and K1 / V1 rows 16-31 (fp32 powers of two).
 // Inside a 32-row tile the 16-byte chunks of each 128-byte line are permuted
-// (chunk ^= line & 7), so that both the row-wise reads of K and the 8x8 matrix
-// loads of V are free of bank conflicts once a record lies in shared memory.
+// (chunk ^= line & 7; by row at head_dim 256), so that both the row-wise reads
+// of K and the 8x8 matrix loads of V are free of bank conflicts once a record
+// lies in shared memory.
 // A record is one contiguous, 16-byte aligned run (HD*64 + 16 bytes): one bulk
 // copy brings everything attention needs of 32 rows, scales included.
 // int8 codes are stored offset by 128 (one byte permute then builds the fp16
@@ -32,6 +33,8 @@ constexpr float kClip = 4.611686018427387904e18f;  // 2^62: larger magnitudes ar
 constexpr int kMaxRuns = 128;      // runs and layers of one launch: its plan travels in the
 constexpr int kMaxCallLayers = 64; // kernel's parameters (no upload, nothing to outlive the call)
 constexpr int kMaxRopeCfgs = 8;
+constexpr int kStepCtasPerSm = 2;  // at most
+constexpr int kStepCols = 8;       // columns of the step kernel
 
 // Consecutive tokens of one sequence: rows io0 .. io0+n-1 of the call, at
 // positions pos0 .. pos0+n-1.
@@ -75,7 +78,12 @@ struct PagedArgs {
     int neox;
     int n_runs;
     int n_layers;
+    int n_full;             // step: layers without a window stand first
     int total;              // work units
+    int total0;             // step: units of those layers
+    int pages0, pages1;     // step: pages of all runs, without and with the window
+    int append;             // step: write the run's row, too
+    int q_vec, kv_vec;      // 16-byte loads of q / of k and v are possible
     const float2* rope[kMaxRopeCfgs];  // [capacity][HD/2] (cos, sin)
     float* scratch;
     int* counters;
@@ -92,7 +100,7 @@ __host__ __device__ constexpr int record_bytes(int hd) { return 2 * kPageRows * 
 // Byte of (row, dim) inside a K or V tile of a record.
 __host__ __device__ __forceinline__ uint32_t tile_byte(int hd, int row, int d) {
     const uint32_t off = static_cast<uint32_t>(row * hd + d);
-    return off ^ (((off >> 7) & 7u) << 4);
+    return off ^ (((off >> (hd == 256 ? 8 : 7)) & 7u) << 4);
 }
 
 #ifdef __CUDACC__
@@ -154,6 +162,34 @@ __device__ __forceinline__ float rope_plain(const float* x, int d, int half, con
                  : __fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
 }
 
+// 16 values to codes (x * inv) and back.
+template <int DT>
+__device__ __forceinline__ uint4 pack_codes(const float (&x)[16], float inv) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = to_code<DT>(x[4 * i] * inv) | to_code<DT>(x[4 * i + 1] * inv) << 8 |
+               to_code<DT>(x[4 * i + 2] * inv) << 16 | to_code<DT>(x[4 * i + 3] * inv) << 24;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack_codes(const uint4& c, float (&x)[16]) {
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = from_code<DT>((w[i / 4] >> (8 * (i % 4))) & 0xFFu);
+}
+
+// CTA that owns unit x when CTA c of P takes units [c*total/P, (c+1)*total/P).
+__device__ __forceinline__ long long owner_of(long long x, long long total, long long P) {
+    return ((x + 1) * P - 1) / total;
+}
+
 #endif  // __CUDACC__
+
+// The step kernel (jx_paged_step.cuh) for `cols` columns: query heads of a kv
+// head, times the tokens of a block.
+cudaError_t paged_step_i8(const PagedArgs& a, int hd, int cols, int num_sms, cudaStream_t st);
+cudaError_t paged_step_e4m3(const PagedArgs& a, int hd, int cols, int num_sms, cudaStream_t st);
 
 }  // namespace jx
