@@ -31,16 +31,26 @@ DTYPES = {"f32": JX_F32, "bf16": JX_BF16, "f16": JX_F16_TRUNC, "f16_trunc": JX_F
 ELEM_SIZE = {JX_F32: 4, JX_BF16: 2, JX_F16_TRUNC: 2}
 
 
-def _stream_ptr(stream) -> Optional[int]:
+_raw_stream = None  # torch's (device) -> address of its current stream, once a GPU was seen
+
+
+def _stream_ptr(stream, device: Optional[int] = None) -> Optional[int]:
+    """Address of `stream`, or of torch's current stream (of `device`, or the current device)."""
+    global _raw_stream
     if stream is not None:
         return int(getattr(stream, "cuda_stream", stream))
-    try:
-        import torch
-        if torch.cuda.is_available():
-            return int(torch.cuda.current_stream().cuda_stream)
-    except ImportError:
-        pass
-    return None
+    if _raw_stream is None:
+        try:
+            import torch
+        except ImportError:
+            return None
+        if not torch.cuda.is_available():
+            return None
+        torch.cuda.init()
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _raw_stream = (lambda d: int(torch.cuda.current_stream(d).cuda_stream)) if raw is None else (
+            lambda d: raw(torch._C._cuda_getDevice() if d is None else d))
+    return _raw_stream(device)
 
 
 def _dev_ptr(t, name: str, min_elems: int, host_ok: bool = False) -> int:
@@ -76,7 +86,7 @@ def _i32_array(x):
     per token)."""
     if isinstance(x, np.ndarray):
         a = x
-    elif isinstance(x, range):
+    elif isinstance(x, range) and len(x) > 64:
         a = np.arange(x.start, x.stop, x.step)
     else:
         return (C.c_int32 * len(x))(*[int(v) for v in x])
@@ -323,7 +333,7 @@ def attn_step(cache: KVCache, layers: Sequence[Layer], q, k, v, out, pos: Sequen
     arr, keep = _layer_array(layers)
     a, keep2 = _step_args(cache, layers, q, k, v, out, pos, n_heads, n_kv_heads, scale, softcap,
                           sliding_window, yarn_scale, neox, seq_ids, 0)
-    check(_entry(cache, "step")(cache.handle, arr, len(layers), C.byref(a), _stream_ptr(stream)))
+    check(_entry(cache, "step")(cache.handle, arr, len(layers), C.byref(a), _stream_ptr(stream, cache.device)))
 
 
 def attn_prefill(cache: KVCache, layers: Sequence[Layer], q, k, v, out, pos: Sequence[int],
@@ -340,7 +350,7 @@ def attn_prefill(cache: KVCache, layers: Sequence[Layer], q, k, v, out, pos: Seq
     a, keep2 = _step_args(cache, layers, q, k, v, out, pos, n_heads, n_kv_heads, scale, softcap,
                           sliding_window, yarn_scale, neox, seq_ids, 0)
     check(_entry(cache, "prefill")(cache.handle, arr, len(layers), C.byref(a),
-                                   _stream_ptr(stream)))
+                                   _stream_ptr(stream, cache.device)))
 
 
 def attn_step_partial(cache: KVCache, layers: Sequence[Layer], q, k, v, partials,
@@ -356,7 +366,7 @@ def attn_step_partial(cache: KVCache, layers: Sequence[Layer], q, k, v, partials
     a, keep2 = _step_args(cache, layers, q, k, v, None, pos, n_heads, n_kv_heads, scale, softcap,
                           sliding_window, yarn_scale, neox, seq_ids, n)
     check(_entry(cache, "step_partial")(cache.handle, arr, len(layers), C.byref(a), pp,
-                                        _stream_ptr(stream)))
+                                        _stream_ptr(stream, cache.device)))
 
 
 def attn_step_sharded(cache: KVCache, layers: Sequence[Layer], q, k, v, out, pos: Sequence[int],
@@ -384,7 +394,7 @@ def attn_step_sharded(cache: KVCache, layers: Sequence[Layer], q, k, v, out, pos
                           sliding_window, yarn_scale, neox, seq_ids, 0)
     check(_entry(cache, "step_sharded")(cache.handle, arr, len(layers), C.byref(a),
                                         C.c_void_p(int(comm)), int(timeout_ms),
-                                        _stream_ptr(stream)))
+                                        _stream_ptr(stream, cache.device)))
 
 
 class StepPlan:
@@ -441,7 +451,7 @@ class StepPlan:
             self._pos[i] = int(p)
 
     def run(self, stream=None) -> None:
-        rc = self._call(*self._head, _stream_ptr(stream))
+        rc = self._call(*self._head, _stream_ptr(stream, self.cache.device))
         if rc:
             check(rc)
 

@@ -155,9 +155,8 @@ __global__ void __launch_bounds__(2 * HD) append_kernel(const __grid_constant__ 
     const int page = a.table[static_cast<long long>(run.seq) * a.max_pages + blk / 2];
     unsigned char* rec = a.pool + page * a.page_bytes + L.cache_layer * a.layer_bytes +
                          static_cast<long long>(h) * record_bytes(HD);
-    unsigned char* dst = rec + which * kPageRows * HD +
-                         tile_byte(HD, (blk & 1) * kBlockRows + row, d0);
-    float* scale = reinterpret_cast<float*>(rec + 2 * kPageRows * HD) + which * 2 + (blk & 1);
+    unsigned char* dst = rec + tile_at(HD, which) + tile_byte(HD, (blk & 1) * kBlockRows + row, d0);
+    float* scale = reinterpret_cast<float*>(rec) + which * 2 + (blk & 1);
     float x[16];
     float m = 0.0f;
     if (is_new) {
@@ -223,9 +222,8 @@ __global__ void __launch_bounds__(2 * HD) keep_kernel(const KeepArgs a) {
         if (i < a.n_rows) {
             const int t = a.rows[i];
             const unsigned char* rec = a.pool + a.src_table[t / kPageRows] * a.page_bytes + rec_off;
-            const float s = reinterpret_cast<const float*>(rec + 2 * kPageRows * HD)
-                [which * 2 + (t / kBlockRows & 1)];
-            unpack_codes<DT>(*reinterpret_cast<const uint4*>(rec + which * kPageRows * HD +
+            const float s = reinterpret_cast<const float*>(rec)[which * 2 + (t / kBlockRows & 1)];
+            unpack_codes<DT>(*reinterpret_cast<const uint4*>(rec + tile_at(HD, which) +
                                                              tile_byte(HD, t % kPageRows, d0)), x);
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -237,11 +235,10 @@ __global__ void __launch_bounds__(2 * HD) keep_kernel(const KeepArgs a) {
         const int k = block_exp<DT>(m);
         unsigned char* rec = a.pool + a.dst_table[blk / 2] * a.page_bytes + rec_off;
         if (i < a.n_rows)
-            *reinterpret_cast<uint4*>(rec + which * kPageRows * HD +
+            *reinterpret_cast<uint4*>(rec + tile_at(HD, which) +
                                       tile_byte(HD, (blk & 1) * kBlockRows + row, d0)) =
                 pack_codes<DT>(x, exp2_int(-k));
-        if (tid == 0)
-            reinterpret_cast<float*>(rec + 2 * kPageRows * HD)[which * 2 + (blk & 1)] = exp2_int(k);
+        if (tid == 0) reinterpret_cast<float*>(rec)[which * 2 + (blk & 1)] = exp2_int(k);
         __syncthreads();  // this block's writes before the next one's reads
     }
 }
@@ -284,12 +281,11 @@ __global__ void load_kernel(const LoadArgs a) {
             }
             w[j] = o;
         }
-        *reinterpret_cast<uint4*>(rec + which * kPageRows * HD +
-                                  tile_byte(HD, t % kPageRows, c * 16)) =
+        *reinterpret_cast<uint4*>(rec + tile_at(HD, which) + tile_byte(HD, t % kPageRows, c * 16)) =
             make_uint4(w[0], w[1], w[2], w[3]);
         if (c == 0 && r % kBlockRows == 0) {
             const float s = a.scales[which][(static_cast<long long>(l) * n_blk + r / kBlockRows) * a.n_kv + h];
-            reinterpret_cast<float*>(rec + 2 * kPageRows * HD)[which * 2 + (t / kBlockRows & 1)] =
+            reinterpret_cast<float*>(rec)[which * 2 + (t / kBlockRows & 1)] =
                 exp2_int(min(kMaxExp, max(kMinExp, scale_exp(fabsf(s)))));
         }
     }
@@ -321,10 +317,9 @@ __global__ void read_kernel(const __grid_constant__ ReadArgs a) {
         const unsigned char* rec =
             a.pool + a.table[static_cast<long long>(a.seq[s]) * a.max_pages + t / kPageRows] * a.page_bytes +
             (static_cast<long long>(l) * a.n_kv + h) * record_bytes(HD);
-        const float sc = reinterpret_cast<const float*>(rec + 2 * kPageRows * HD)
-            [which * 2 + (t / kBlockRows & 1)];
+        const float sc = reinterpret_cast<const float*>(rec)[which * 2 + (t / kBlockRows & 1)];
         float x[16];
-        unpack_codes<DT>(*reinterpret_cast<const uint4*>(rec + which * kPageRows * HD +
+        unpack_codes<DT>(*reinterpret_cast<const uint4*>(rec + tile_at(HD, which) +
                                                          tile_byte(HD, t % kPageRows, c * 16)), x);
         const long long o = (s * per + i) * 16;
         if constexpr (F32) {
@@ -615,8 +610,8 @@ int step_rows(jx_pkv* kv, PagedArgs& A, const std::vector<PagedLayer>& part, con
             for (; A.n_runs < kMaxRuns && r0 < runs.size(); ++r0) {
                 PagedRun r = runs[r0];
                 const int last = r.pos0 + r.n - 1;
-                const int n0 = last / kPageRows + 1;
-                const int n1 = last / kPageRows - std::max(0, r.pos0 - A.window + 1) / kPageRows + 1;
+                const int n0 = last / kPageRows + 1 + kPieceCost;
+                const int n1 = last / kPageRows - std::max(0, r.pos0 - A.window + 1) / kPageRows + 1 + kPieceCost;
                 if ((p0 + n0) * seg0 + (p1 + n1) * seg1 > kMaxUnits) {
                     if (A.n_runs > 0) break;
                     return pfail(JX_ERR_UNSUPPORTED, "a step over %d rows of %d layers is too large", last + 1, A.n_layers);
@@ -628,8 +623,8 @@ int step_rows(jx_pkv* kv, PagedArgs& A, const std::vector<PagedLayer>& part, con
                 cols = std::max(cols, r.n * A.G);
                 A.runs[A.n_runs++] = r;
             }
-            A.pages0 = static_cast<int>(p0);
-            A.pages1 = static_cast<int>(p1);
+            A.units0 = static_cast<int>(p0);
+            A.units1 = static_cast<int>(p1);
             A.total0 = static_cast<int>(p0 * seg0);
             A.total = static_cast<int>(p0 * seg0 + p1 * seg1);
             const auto launch = kv->d.dtype == JX_I8 ? paged_step_i8 : paged_step_e4m3;
@@ -755,7 +750,8 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
     A.kv_stride = a->kv_stride;
     A.scale = a->scale;
     A.softcap = a->softcap;
-    A.inv_softcap = a->softcap > 0.0f ? 1.0f / a->softcap : 0.0f;
+    A.cap_out = a->softcap * 1.4426950408889634f;
+    A.cap_in = a->softcap > 0.0f ? 1.0f / A.cap_out : 0.0f;
     A.window = static_cast<int>(std::min<uint32_t>(a->sliding_window, 0x7FFFFFFFu));
     A.neox = a->rope_neox != 0 ? 1 : 0;
     A.err = kv->d_err;

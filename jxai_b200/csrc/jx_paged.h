@@ -3,14 +3,14 @@
 //
 // A page holds kPageRows consecutive rows of one sequence for every layer.  It
 // is a run of records, one per (layer, kv head):
-//   K codes [32][HD] bytes, V codes [32][HD] bytes, scales {K0, K1, V0, V1}
+//   scales {K0, K1, V0, V1}, K codes [32][HD] bytes, V codes [32][HD] bytes
 // where K0 / V0 scale rows 0-15 and K1 / V1 rows 16-31 (fp32 powers of two).
 // Inside a 32-row tile the 16-byte chunks of each 128-byte line are permuted
 // (chunk ^= line & 7; by row at head_dim 256), so that both the row-wise reads
 // of K and the 8x8 matrix loads of V are free of bank conflicts once a record
 // lies in shared memory.
 // A record is one contiguous, 16-byte aligned run (HD*64 + 16 bytes): one bulk
-// copy brings everything attention needs of 32 rows, scales included.
+// copy, or two (scales and K, then V), bring all that attention needs of 32 rows.
 // int8 codes are stored offset by 128 (one byte permute then builds the fp16
 // number 1024 + u); e4m3 codes as they are.
 #pragma once
@@ -33,7 +33,8 @@ constexpr float kClip = 4.611686018427387904e18f;  // 2^62: larger magnitudes ar
 constexpr int kMaxRuns = 128;      // runs and layers of one launch: its plan travels in the
 constexpr int kMaxCallLayers = 64; // kernel's parameters (no upload, nothing to outlive the call)
 constexpr int kMaxRopeCfgs = 8;
-constexpr int kStepCtasPerSm = 2;  // at most
+constexpr int kStepCtasPerSm = 4;  // at most
+constexpr int kPieceCost = 16;      // what a segment costs a CTA beside its pages, in pages
 constexpr int kStepCols = 8;       // columns of the step kernel
 
 // Consecutive tokens of one sequence: rows io0 .. io0+n-1 of the call, at
@@ -73,7 +74,7 @@ struct PagedArgs {
     long long kv_stride;
     float scale;
     float softcap;
-    float inv_softcap;
+    float cap_in, cap_out;  // softcap on x = s log2(e): cap_out tanh(x cap_in)
     int window;
     int neox;
     int n_runs;
@@ -81,7 +82,7 @@ struct PagedArgs {
     int n_full;             // step: layers without a window stand first
     int total;              // work units
     int total0;             // step: units of those layers
-    int pages0, pages1;     // step: pages of all runs, without and with the window
+    int units0, units1;     // step: units of a segment, over all runs, without and with the window
     int append;             // step: write the run's row, too
     int q_vec, kv_vec;      // 16-byte loads of q / of k and v are possible
     const float2* rope[kMaxRopeCfgs];  // [capacity][HD/2] (cos, sin)
@@ -95,7 +96,10 @@ struct PagedArgs {
 };
 static_assert(sizeof(PagedArgs) <= 4096, "kernel parameters");
 
-__host__ __device__ constexpr int record_bytes(int hd) { return 2 * kPageRows * hd + 16; }
+constexpr int kScaleBytes = 16;
+__host__ __device__ constexpr int record_bytes(int hd) { return kScaleBytes + 2 * kPageRows * hd; }
+// The K (0) or V (1) tile of a record.
+__host__ __device__ constexpr int tile_at(int hd, int which) { return kScaleBytes + which * kPageRows * hd; }
 
 // Byte of (row, dim) inside a K or V tile of a record.
 __host__ __device__ __forceinline__ uint32_t tile_byte(int hd, int row, int d) {
@@ -162,17 +166,16 @@ __device__ __forceinline__ float rope_plain(const float* x, int d, int half, con
                  : __fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
 }
 
-// 16 values to codes (x * inv) and back.
+// Four values to codes (x * inv) and back; 16 likewise.
+template <int DT>
+__device__ __forceinline__ uint32_t pack4(float x, float y, float z, float w, float inv) {
+    return to_code<DT>(x * inv) | to_code<DT>(y * inv) << 8 | to_code<DT>(z * inv) << 16 | to_code<DT>(w * inv) << 24;
+}
 template <int DT>
 __device__ __forceinline__ uint4 pack_codes(const float (&x)[16], float inv) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        w[i] = to_code<DT>(x[4 * i] * inv) | to_code<DT>(x[4 * i + 1] * inv) << 8 |
-               to_code<DT>(x[4 * i + 2] * inv) << 16 | to_code<DT>(x[4 * i + 3] * inv) << 24;
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint4(pack4<DT>(x[0], x[1], x[2], x[3], inv), pack4<DT>(x[4], x[5], x[6], x[7], inv),
+                      pack4<DT>(x[8], x[9], x[10], x[11], inv), pack4<DT>(x[12], x[13], x[14], x[15], inv));
 }
-
 template <int DT>
 __device__ __forceinline__ void unpack_codes(const uint4& c, float (&x)[16]) {
     const uint32_t w[4] = {c.x, c.y, c.z, c.w};

@@ -42,23 +42,26 @@ namespace jx {
 
 template <int HD, int GP>
 struct StepCfg {
-    static constexpr int R = record_bytes(HD);
-    static constexpr int W = 4;                        // warps
-    static constexpr int CTAS = HD == 256 ? 1 : 2;  // resident per SM
-    // ring stages per warp: as many records as the SM's shared memory holds
-    static constexpr int O_BYTES = W * GP * HD * 4;
-    static constexpr int ML_BYTES = W * GP * 2 * 4;
-    static constexpr int MISC = 64;
-    static constexpr int budget = (227 * 1024) / CTAS - 1024 - O_BYTES - ML_BYTES - MISC;
-    static constexpr int fit = budget / (W * (R + 8));
-    static constexpr int NS = fit > 8 ? 8 : fit;
-    static constexpr int OFF_O = W * NS * R;
-    static constexpr int OFF_ML = OFF_O + O_BYTES;
-    static constexpr int OFF_BAR = OFF_ML + ML_BYTES;
-    static constexpr int OFF_MISC = OFF_BAR + W * NS * 8;
-    static constexpr int SMEM = OFF_MISC + MISC;
-    static_assert(NS >= 2, "ring");
-    static_assert(OFF_BAR % 8 == 0 && OFF_O % 16 == 0, "alignment");
+    static constexpr int W = 4;  // warps per CTA
+    // Resident CTAs per SM, by the registers their accumulators need.
+    static constexpr int CTAS = HD == 256 ? 2 : (HD == 128 ? 3 : 4);
+    // A stage holds a record, or (wide heads) half of one: scales and K, or V.
+    static constexpr bool SPLIT = HD >= 128;
+    static constexpr int STAGE = SPLIT ? tile_at(HD, 1) : record_bytes(HD);
+    static constexpr int MISC = W * GP * 2 * 4 + 64;  // (m, l) of each warp and column; flags
+    static constexpr int budget = (227 * 1024) / CTAS - 1024 - MISC;
+    static constexpr int fit = budget / (W * (STAGE + 8));
+    static constexpr int NS = fit > 8 ? 8 : fit;  // stages per warp
+    // floats of a partial result: o [GP][HD], then (m, l) [GP]; 16-byte aligned
+    static constexpr int PART = (GP * (HD + 2) + 3) / 4 * 4;
+    static_assert(PART <= kStepCols * (HD + 2), "scratch");
+    static constexpr int OFF_MISC = W * NS * STAGE;
+    static constexpr int OFF_BAR = OFF_MISC + MISC;
+    static constexpr int SMEM = OFF_BAR + W * NS * 8;
+    static_assert(NS >= (SPLIT ? 3 : 2), "ring");
+    static_assert(OFF_BAR % 8 == 0 && OFF_MISC % 16 == 0, "alignment");
+    // a warp's part of a finished piece lies in the stage it read last
+    static_assert(GP * HD * 4 <= kPageRows * HD, "result in a V tile");
 };
 
 // Rows of an 8-row matrix in the order the lanes take them: two rows read by
@@ -68,56 +71,75 @@ __device__ __forceinline__ int row_perm(int g) {
     return HD >= 128 ? (g & 1) * 4 + (g >> 1) : g;
 }
 
-// One piece: units [x0, x0 + n) of the flattened space, pages page0 .. of a segment.
+// One piece: pages page0 .. page0+n-1 of a sequence for one layer and kv head.
 struct Piece {
     int run, layer, h;
     int page0, n;
-    int x0;
-    int seg_x0, seg_n;  // the whole segment
+    int in_seg;         // pages of the segment before it
+    int seg_x0, seg_n;  // the segment's first unit, and its pages
+    int rot;            // its first page goes to warp rot
+    bool coop;          // read by all warps of the CTA, page by page in turn; else by warp rot alone
 };
 
-// Walks the pieces of units [x, end).
+// Walks the pieces of units [x, end).  A segment takes kPieceCost units before
+// its pages' own: what it costs to start and finish one is counted into a CTA's
+// share, which matters where sequences are short.
+// A piece that is a whole segment of at most 1/16 of the share is one warp's
+// (the next in turn): it starts and ends without a barrier, and without all
+// four warps preparing the same q.  The others are read by all warps together.
 struct PieceWalk {
-    int x, end, r, cls;
+    int x, end, r, cls, small, owned;
 
     __device__ __forceinline__ void init(int x_, int end_) {
         x = x_;
         end = end_;
         r = 0;
         cls = 0;
+        small = (end_ - x_) / 16;
+        owned = 0;
     }
     // Layers [0, n_full) attend everything, [n_full, n_layers) a window; the
     // windowed ones' units stand behind the others'.
     __device__ __forceinline__ bool next(const PagedArgs& a, Piece& p) {
-        if (x >= end) return false;
-        if (cls == 0 && x >= a.total0) {
-            cls = 1;
-            r = 0;
+        while (x < end) {
+            if (cls == 0 && x >= a.total0) {
+                cls = 1;
+                r = 0;
+            }
+            const int per = (cls ? a.n_layers - a.n_full : a.n_full) * a.n_kv;  // segments of a run
+            const int y = x - (cls ? a.total0 : 0);
+            auto off = [&](int i) {
+                return i < a.n_runs ? (cls ? a.runs[i].off1 : a.runs[i].off) : (cls ? a.units1 : a.units0);
+            };
+            if (y >= off(r + 1) * per) {  // the run that holds y
+                int lo = r + 1, hi = a.n_runs - 1;
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (y >= off(mid + 1) * per) lo = mid + 1;
+                    else hi = mid;
+                }
+                r = lo;
+            }
+            const int first = off(r), len = off(r + 1) - first;
+            const int rem = y - first * per;
+            const int seg = rem / len, u = rem - seg * len;
+            const int n = min(len - u, end - x);
+            const int pg = max(0, u - kPieceCost);
+            p.n = u + n - kPieceCost - pg;
+            p.seg_x0 = x - u;
+            x += n;
+            if (p.n <= 0) continue;
+            p.run = r;
+            p.layer = (cls ? a.n_full : 0) + seg / a.n_kv;
+            p.h = seg % a.n_kv;
+            p.in_seg = pg;
+            p.seg_n = len - kPieceCost;
+            p.page0 = (cls ? max(0, a.runs[r].pos0 - a.window + 1) / kPageRows : 0) + pg;
+            p.coop = p.n < p.seg_n || p.n > small;
+            p.rot = (p.coop ? x : owned++) & 3;
+            return true;
         }
-        const int base = cls ? a.total0 : 0;
-        const int per = (cls ? a.n_layers - a.n_full : a.n_full) * a.n_kv;  // segments of a run
-        const int y = x - base;
-        int first = cls ? a.runs[r].off1 : a.runs[r].off;
-        int next_off = r + 1 < a.n_runs ? (cls ? a.runs[r + 1].off1 : a.runs[r + 1].off) : (cls ? a.pages1 : a.pages0);
-        while (y >= next_off * per) {
-            ++r;
-            first = next_off;
-            next_off = r + 1 < a.n_runs ? (cls ? a.runs[r + 1].off1 : a.runs[r + 1].off) : (cls ? a.pages1 : a.pages0);
-        }
-        const int np = next_off - first;
-        const int rem = y - first * per;
-        const int seg = rem / np, pg = rem - seg * np;
-        p.run = r;
-        p.layer = (cls ? a.n_full : 0) + seg / a.n_kv;
-        p.h = seg % a.n_kv;
-        const int pos0 = a.runs[r].pos0;
-        p.page0 = (cls ? max(0, pos0 - a.window + 1) / kPageRows : 0) + pg;
-        p.x0 = x;
-        p.seg_x0 = x - pg;
-        p.seg_n = np;
-        p.n = min(np - pg, end - x);
-        x += p.n;
-        return true;
+        return false;
     }
 };
 
@@ -185,7 +207,7 @@ struct StepWarp {
     uint32_t qf[KS][NBC][2];
     float o[KS][NBC][4];
     float m[2], l[2];
-    float unscale[2];
+    float unscale;     // a.scale log2(e), and what q was scaled by taken back
     int lo[2], hi[2];  // attended rows of this lane's two columns
 
     __device__ __forceinline__ static float col_sum(const float (&x)[NBC][4], int r) {
@@ -203,52 +225,55 @@ struct StepWarp {
         else return t == 0 ? ((h & 0xFFFFu) | (w << 16)) : 0u;
     }
 
-    __device__ __forceinline__ void begin(const PagedArgs& a, const Piece& p, int lane) {
+    // Prepares q of a piece: rotated into `tmp` (GP * HD floats of shared memory,
+    // this warp's own) by a compact loop, then read back as operands.
+    __device__ __forceinline__ void begin(const PagedArgs& a, const Piece& p, float* tmp, int lane) {
         const int g = lane >> 2, t = lane & 3;
         const PagedRun& run = a.runs[p.run];
         const PagedLayer L = a.layers[p.layer];
         const int ncol = run.n * a.G;
+        const bool vec = a.q_vec && L.half % 4 == 0;
         float mx = 0.0f;
-        float4 x[KS];
-        {
-            const int col = g % GP, part = g / GP;
-            const int tok = col / a.G;
-            const bool use = col < ncol && (NBC == 2 || part < 2);
-            const long long io = static_cast<long long>(run.io0 + tok) * a.n_io_layers + L.io;
-            const float* src = a.q + io * a.q_stride + (p.h * a.G + col % a.G) * HD;
-            const float2* cs = a.rope[L.cfg] + static_cast<long long>(run.pos0 + tok) * (HD / 2);
-            const bool vec = a.q_vec && L.half % 4 == 0;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const int d = HD >= 64 ? (t + 4 * (ks / 4)) * 16 + (ks % 4) * 4 : t * 8 + ks * 4;
-                x[ks] = use ? rope4(src, d, L.half, cs, a.neox != 0, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
-                mx = fmaxf(fmaxf(mx, fmaxf(fabsf(x[ks].x), fabsf(x[ks].y))), fmaxf(fabsf(x[ks].z), fabsf(x[ks].w)));
+#pragma unroll 2
+        for (int i = lane; i < GP * HD / 4; i += 32) {
+            const int col = i / (HD / 4), d = i % (HD / 4) * 4;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (col < ncol) {
+                const int tok = run.n > 1 ? col / a.G : 0;
+                const long long io = static_cast<long long>(run.io0 + tok) * a.n_io_layers + L.io;
+                x = rope4(a.q + io * a.q_stride + (p.h * a.G + col - tok * a.G) * HD, d, L.half,
+                          a.rope[L.cfg] + static_cast<long long>(run.pos0 + tok) * (HD / 2), a.neox != 0, vec);
             }
-            // each head's largest |q| is brought into [2^14, 2^15): no bits of the
-            // second part are lost to fp16's range
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const int e = static_cast<int>((__float_as_uint(mx) >> 23) & 0xFFu) - 127;
-            const int sh = min(60, max(-60, 14 - e));
-            const float up = exp2_int(sh), down = exp2_int(-sh);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                uint32_t h01, l01, h23, l23;
-                split_pair<DT_F16T>(x[ks].x * up, x[ks].y * up, h01, l01);
-                split_pair<DT_F16T>(x[ks].z * up, x[ks].w * up, h23, l23);
-                if constexpr (NBC == 2) {
-                    qf[ks][0][0] = h01;
-                    qf[ks][0][1] = h23;
-                    qf[ks][1][0] = l01;
-                    qf[ks][1][1] = l23;
-                } else {
-                    qf[ks][0][0] = part == 0 ? h01 : (part == 1 ? l01 : 0u);
-                    qf[ks][0][1] = part == 0 ? h23 : (part == 1 ? l23 : 0u);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) unscale[j] = __shfl_sync(0xffffffffu, down, ((2 * t + j) % GP) * 4);
+            *reinterpret_cast<float4*>(tmp + 4 * i) = x;
+            mx = fmaxf(fmaxf(mx, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
         }
+        // the largest |q| is brought into [2^14, 2^15): no bits of the second part
+        // are lost to fp16's range
+        mx = warp_max(mx);
+        const int e = static_cast<int>((__float_as_uint(mx) >> 23) & 0xFFu) - 127;
+        const int sh = min(60, max(-60, 14 - e));
+        const float up = exp2_int(sh);
+        unscale = exp2_int(-sh) * (a.scale * 1.4426950408889634f);
+        __syncwarp();
+        const int part = g / GP;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d = HD >= 64 ? (t + 4 * (ks / 4)) * 16 + (ks % 4) * 4 : t * 8 + ks * 4;
+            const float4 x = *reinterpret_cast<const float4*>(tmp + (g % GP) * HD + d);
+            uint32_t h01, l01, h23, l23;
+            split_pair<DT_F16T>(x.x * up, x.y * up, h01, l01);
+            split_pair<DT_F16T>(x.z * up, x.w * up, h23, l23);
+            if constexpr (NBC == 2) {
+                qf[ks][0][0] = h01;
+                qf[ks][0][1] = h23;
+                qf[ks][1][0] = l01;
+                qf[ks][1][1] = l23;
+            } else {
+                qf[ks][0][0] = part == 0 ? h01 : (part == 1 ? l01 : 0u);
+                qf[ks][0][1] = part == 0 ? h23 : (part == 1 ? l23 : 0u);
+            }
+        }
+        __syncwarp();  // tmp is read before it is used for something else
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int col = (2 * t + j) % GP;
@@ -266,10 +291,12 @@ struct StepWarp {
                 for (int r = 0; r < 4; ++r) o[mh][nb][r] = 0.0f;
     }
 
-    // One record in shared memory at `rec`, rows row0 .. row0+31.
-    __device__ __forceinline__ void page(const PagedArgs& a, const unsigned char* rec, int row0, bool edge, int lane) {
+    uint32_t bp[2][NBC][2];  // weights of a page as operands
+
+    // Weights of rows row0 .. row0+31 from their K tile and scales.
+    __device__ __forceinline__ void scores(const PagedArgs& a, const unsigned char* rec, const float4 sc, int row0,
+                                           bool edge, int lane) {
         const int g = lane >> 2, t = lane & 3;
-        const float4 sc = *reinterpret_cast<const float4*>(rec + 2 * kPageRows * HD);
         float acc[2][NBC][4];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -317,6 +344,7 @@ struct StepWarp {
         // exponents: x = s log2e + kV; rows b*16 + (r>>1)*8 + perm(g), column slot r&1
         float x[2][4];
         float vinv[2];
+        const bool capped = a.softcap > 0.0f;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const float ks = b ? sc.y : sc.x;
@@ -325,10 +353,9 @@ struct StepWarp {
             vinv[b] = __uint_as_float((254u - ve) << 23);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float s = col_sum(acc[b], r) * (unscale[r & 1] * ks);
-                s *= a.scale;
-                if (a.softcap > 0.0f) s = a.softcap * tanhf(s * a.inv_softcap);
-                s = fmaf(s, 1.4426950408889634f, kv);
+                float s = col_sum(acc[b], r) * (unscale * ks);
+                if (capped) s = a.cap_out * tanhf(s * a.cap_in);
+                s += kv;
                 if (edge) {
                     const int row = row0 + b * 16 + (r >> 1) * 8 + rp;
                     if (row < lo[r & 1] || row > hi[r & 1]) s = -INFINITY;
@@ -362,14 +389,15 @@ struct StepWarp {
                     }
             }
         }
-        uint32_t bp[2][NBC][2];
+        float mb[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) mb[j] = m[j] == -INFINITY ? 0.0f : static_cast<float>(kBase) - m[j];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             float pr[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float mr = m[r & 1] == -INFINITY ? 0.0f : m[r & 1];
-                pr[r] = ex2_approx(x[b][r] - mr + static_cast<float>(kBase));
+                pr[r] = ex2_approx(x[b][r] + mb[r & 1]);
             }
             l[0] = fmaf(pr[0] + pr[2], vinv[b], l[0]);
             l[1] = fmaf(pr[1] + pr[3], vinv[b], l[1]);
@@ -381,8 +409,11 @@ struct StepWarp {
                 for (int nb = 0; nb < NBC; ++nb) bp[b][nb][hf] = movmatrix_trans(pick(h, w, nb, t));
             }
         }
+    }
+
+    // O += P V for the page whose weights `scores` left.
+    __device__ __forceinline__ void values(uint32_t vbase, int lane) {
         const int i8 = lane >> 3, vr = (i8 & 1) * 8 + row_perm<HD>(lane & 7);
-        const uint32_t vbase = smem_u32(rec) + kPageRows * HD;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
 #pragma unroll
@@ -403,8 +434,7 @@ struct StepWarp {
         }
     }
 
-    // This warp's (o, m, l) of the piece to shared memory: o_s [warp][col][HD],
-    // ml_s [warp][col][2].
+    // This warp's part of a piece to shared memory: o_s [col][HD], ml_s [col][2].
     __device__ __forceinline__ void finish(float* o_s, float* ml_s, int lane) {
         const int g = lane >> 2, t = lane & 3;
         const bool w0 = GP == 8 || (GP == 4 && t < 2) || (GP <= 2 && t == 0);
@@ -430,64 +460,96 @@ struct StepWarp {
     }
 };
 
-// The step's new row, by the warp whose record (in shared memory at `rec`, in
-// the pool at `home`) receives it: the same arithmetic and thread layout as
-// append_kernel, one lane per 16 values.
+// The step's new row, by the warp whose record (in shared memory: scales, K and
+// V tile; in the pool at `home`) receives it: append_kernel's arithmetic, four
+// values per lane and turn.  At head_dim up to 64 the warp's halves take K and V
+// at once, else one after the other.
 template <int HD, int DT>
-__device__ __forceinline__ void step_append(const PagedArgs& a, const Piece& p, unsigned char* rec,
-                                            unsigned char* home, int lane) {
-    constexpr int CPR = HD / 16;
+__device__ __forceinline__ void step_append(const PagedArgs& a, const Piece& p, unsigned char* scales,
+                                            unsigned char* kt, unsigned char* vt, unsigned char* home, int lane) {
+    constexpr int TURNS = HD <= 64 ? 1 : 2;              // tensors one after the other
+    constexpr int SPAN = HD / 4 < 32 ? HD / 4 : 32;      // lanes of a tensor
+    constexpr int NG = HD / 4 / SPAN;                    // groups of four per lane
     const PagedRun& run = a.runs[p.run];
     const PagedLayer L = a.layers[p.layer];
-    const int which = lane / CPR, d0 = lane % CPR * 16;
     const int row = run.pos0 % kPageRows, blk = row / kBlockRows;
-    const uint32_t tile = static_cast<uint32_t>(which * kPageRows * HD);
-    const uint32_t at_scale = 2 * kPageRows * HD + (which * 2 + blk) * 4;
-    const bool on = which < 2;
-    float x[16];
-    float m = 0.0f;
-    if (on) {
-        const long long io = static_cast<long long>(run.io0) * a.n_io_layers + L.io;
-        const float* src = (which ? a.v_in : a.k_in) + io * a.kv_stride + p.h * HD;
-        const float2* cs = a.rope[L.cfg] + static_cast<long long>(run.pos0) * (HD / 2);
-        const bool vec = a.kv_vec && L.half % 4 == 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 v = rope4(src, d0 + 4 * i, which ? 0 : L.half, cs, a.neox != 0, vec);
-            x[4 * i] = cache_value(v.x);
-            x[4 * i + 1] = cache_value(v.y);
-            x[4 * i + 2] = cache_value(v.z);
-            x[4 * i + 3] = cache_value(v.w);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(x[i]));
-    }
-#pragma unroll
-    for (int s = 1; s < CPR; s <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
     const bool joins = row % kBlockRows != 0;
-    const int k_old = on && joins ? max(kMinExp, scale_exp(*reinterpret_cast<float*>(rec + at_scale))) : kMinExp;
-    __syncwarp();  // the old scale is read by all before one lane replaces it
-    if (on) {
+    const long long io = static_cast<long long>(run.io0) * a.n_io_layers + L.io;
+    const float2* cs = a.rope[L.cfg] + static_cast<long long>(run.pos0) * (HD / 2);
+    const bool vec = a.kv_vec && L.half % 4 == 0;
+#pragma unroll 1
+    for (int turn = 0; turn < TURNS; ++turn) {
+        const int which = TURNS == 2 ? turn : lane / SPAN;
+        const bool on = which < 2;
+        const float* src = (which == 0 ? a.k_in : a.v_in) + io * a.kv_stride + p.h * HD;
+        unsigned char* rec = which == 0 ? kt : vt;
+        unsigned char* tile = home + tile_at(HD, which & 1);
+        float* scale = reinterpret_cast<float*>(scales) + (which & 1) * 2 + blk;
+        float4 x[NG];
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int d = (lane % SPAN + i * SPAN) * 4;
+            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (on) x[i] = rope4(src, d, which == 0 ? L.half : 0, cs, a.neox != 0, vec);
+            x[i] = make_float4(cache_value(x[i].x), cache_value(x[i].y), cache_value(x[i].z), cache_value(x[i].w));
+            m = fmaxf(fmaxf(m, fmaxf(fabsf(x[i].x), fabsf(x[i].y))), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+        }
+#pragma unroll
+        for (int s = 1; s < SPAN; s <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+        const int k_old = joins ? max(kMinExp, scale_exp(*scale)) : kMinExp;
         const int k = max(k_old, block_exp<DT>(m));
-        const uint4 c = pack_codes<DT>(x, exp2_int(-k));
-        *reinterpret_cast<uint4*>(rec + tile + tile_byte(HD, row, d0)) = c;
-        *reinterpret_cast<uint4*>(home + tile + tile_byte(HD, row, d0)) = c;
-        if (joins && k > k_old)
-            for (int r = blk * kBlockRows; r < row; ++r) {
-                const uint32_t at = tile + tile_byte(HD, r, d0);
-                unpack_codes<DT>(*reinterpret_cast<const uint4*>(rec + at), x);
-                const uint4 cr = pack_codes<DT>(x, exp2_int(k_old - k));
-                *reinterpret_cast<uint4*>(rec + at) = cr;
-                *reinterpret_cast<uint4*>(home + at) = cr;
+        __syncwarp();  // the old scale is read by all before one lane replaces it
+        if (on) {
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const int d = (lane % SPAN + i * SPAN) * 4;
+                const uint32_t c = pack4<DT>(x[i].x, x[i].y, x[i].z, x[i].w, exp2_int(-k));
+                *reinterpret_cast<uint32_t*>(rec + tile_byte(HD, row, d)) = c;
+                *reinterpret_cast<uint32_t*>(tile + tile_byte(HD, row, d)) = c;
+                if (joins && k > k_old) {
+                    const float f = exp2_int(k_old - k);
+#pragma unroll 1
+                    for (int r = blk * kBlockRows; r < row; ++r) {
+                        const uint32_t at = tile_byte(HD, r, d);
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + at);
+                        const uint32_t n = pack4<DT>(from_code<DT>(w & 0xFFu), from_code<DT>(w >> 8 & 0xFFu),
+                                                     from_code<DT>(w >> 16 & 0xFFu), from_code<DT>(w >> 24), f);
+                        *reinterpret_cast<uint32_t*>(rec + at) = n;
+                        *reinterpret_cast<uint32_t*>(tile + at) = n;
+                    }
+                }
             }
-        if (d0 == 0) {
-            *reinterpret_cast<float*>(rec + at_scale) = exp2_int(k);
-            *reinterpret_cast<float*>(home + at_scale) = exp2_int(k);
+            if (lane % SPAN == 0) {
+                *scale = exp2_int(k);
+                reinterpret_cast<float*>(home)[which * 2 + blk] = exp2_int(k);
+            }
         }
     }
     __syncwarp();
-    fence_proxy_async_shared();  // these writes before the stage's next bulk copy
+    fence_proxy_async_shared();  // these writes before the stages' next bulk copies
     __syncwarp();
+}
+
+// The inputs a piece begins with (q, the position's cosines and sines, the new
+// k and v) into L2 while the pieces before it are still being read.
+template <int HD>
+__device__ __forceinline__ void warm_inputs(const PagedArgs& a, const Piece& p, int lane) {
+    const PagedRun& run = a.runs[p.run];
+    const PagedLayer L = a.layers[p.layer];
+    auto warm = [&](const void* at, int bytes) {
+        for (int b = lane * 128; b < bytes; b += 32 * 128)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(at) + b));
+    };
+    for (int j = 0; j < run.n; ++j) {
+        const long long io = static_cast<long long>(run.io0 + j) * a.n_io_layers + L.io;
+        warm(a.q + io * a.q_stride + p.h * a.G * HD, a.G * HD * 4);
+        warm(a.rope[L.cfg] + static_cast<long long>(run.pos0 + j) * (HD / 2), HD * 4);
+        if (a.append && (L.flags & kLayerAppend)) {
+            warm(a.k_in + io * a.kv_stride + p.h * HD, HD * 4);
+            warm(a.v_in + io * a.kv_stride + p.h * HD, HD * 4);
+        }
+    }
 }
 
 template <int HD, int GP, int DT>
@@ -495,13 +557,14 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
     paged_step_kernel(const __grid_constant__ PagedArgs a) {
     using C = StepCfg<HD, GP>;
     constexpr int W = C::W, NS = C::NS;
+    static_assert(W == 4, "PieceWalk's rotation");
     extern __shared__ __align__(16) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float* o_s = reinterpret_cast<float*>(smem + C::OFF_O);
-    float* ml_s = reinterpret_cast<float*>(smem + C::OFF_ML);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC);
-    int* flag = reinterpret_cast<int*>(smem + C::OFF_MISC) + 1;
-    unsigned char* ring = smem + warp * NS * C::R;
+    float* ml_s = reinterpret_cast<float*>(smem + C::OFF_MISC);                 // [warp][col](m, l)
+    int* o_at = reinterpret_cast<int*>(smem + C::OFF_MISC + W * GP * 2 * 4);    // [warp]: its o in smem
+    volatile int* abort_flag = o_at + W;
+    int* flag = o_at + W + 1;
+    unsigned char* ring = smem + warp * NS * C::STAGE;
     const uint32_t ring_u32 = smem_u32(ring);
     const uint32_t bars = smem_u32(smem + C::OFF_BAR) + warp * NS * 8;
     if (threadIdx.x == 0) *abort_flag = 0;
@@ -515,101 +578,193 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
     const int b0 = static_cast<int>(static_cast<long long>(a.total) * c / P);
     const int b1 = static_cast<int>(static_cast<long long>(a.total) * (c + 1) / P);
 
-    // ---- the prefetch cursor: this warp's records, in the order it reads them
-    PieceWalk pw;
-    pw.init(b0, b1);
-    Piece pp;
-    pp.n = 0;
-    int p_i = 0, p_cnt = 0, p_first = 0, ids = 0;
-    const unsigned char* p_base = nullptr;
-    int issued = 0, used = 0;
-    auto prefetch = [&]() {
-        while (p_i >= p_cnt) {
-            if (!pw.next(a, pp)) return;
-            p_first = (warp - pp.x0 % W + W) % W;  // first own page of the piece
-            p_cnt = (pp.n - p_first + W - 1) / W;
-            p_i = 0;
-            p_base = a.pool + a.layers[pp.layer].cache_layer * a.layer_bytes + static_cast<long long>(pp.h) * C::R;
-        }
-        if (p_i % 32 == 0) {
-            const int own = p_i + lane;
-            ids = own < p_cnt ? a.table[static_cast<long long>(a.runs[pp.run].seq) * a.max_pages + pp.page0 + p_first + own * W] : 0;
-        }
-        const int id = __shfl_sync(0xffffffffu, ids, p_i % 32);
-        ++p_i;
-        if (__shfl_sync(0xffffffffu, *abort_flag, 0)) return;
-        const int st = issued % NS;
-        ++issued;
-        if (lane == 0) {
-            mbar_arrive_expect_tx(bars + 8 * st, C::R);
-            bulk_load(ring_u32 + st * C::R, p_base + id * a.page_bytes, C::R, bars + 8 * st);
-        }
-    };
-#pragma unroll 1
-    for (int s = 0; s < NS; ++s) prefetch();
-
+    // ---- the prefetch cursor: this warp's records (halves), in the order it reads them
     PieceWalk cw;
     cw.init(b0, b1);
     Piece p;
+    bool more = cw.next(a, p);
+    PieceWalk pw = cw;
+    Piece pp = p;
+    bool p_more = more;
+    int p_i = 0, p_cnt = 0, p_first = 0, p_step = 1, ids = 0;
+    const unsigned char* p_base = nullptr;
+    const unsigned char* p_src = nullptr;
+    bool p_half = false;  // V of the record at p_src is next
+    int issued = 0, p_st = 0;
+    bool dead = false;    // a wait ran out: nothing more is issued
+    auto enter = [&]() {  // the cursor takes up piece pp
+        p_i = 0;
+        p_step = pp.coop ? W : 1;
+        p_first = pp.coop ? (warp - pp.rot) & (W - 1) : 0;  // first own page of the piece
+        p_cnt = pp.coop ? (pp.n - p_first + W - 1) / W : (warp == pp.rot ? pp.n : 0);
+        p_base = a.pool + a.layers[pp.layer].cache_layer * a.layer_bytes +
+                 static_cast<long long>(pp.h) * record_bytes(HD);
+    };
+    if (more) enter();
+    auto prefetch = [&]() {
+        if (dead || !p_more) return;
+        if (!p_half) {
+            while (p_i >= p_cnt) {
+                p_more = pw.next(a, pp);
+                if (!p_more) return;
+                enter();
+                if (warp == pp.rot) warm_inputs<HD>(a, pp, lane);
+            }
+            if (p_i % 32 == 0) {
+                const int own = p_i + lane;
+                ids = own < p_cnt
+                          ? a.table[static_cast<long long>(a.runs[pp.run].seq) * a.max_pages + pp.page0 + p_first + own * p_step]
+                          : 0;
+            }
+            p_src = p_base + __shfl_sync(0xffffffffu, ids, p_i % 32) * a.page_bytes;
+            ++p_i;
+        }
+        if (lane == 0) {
+            const uint32_t bytes = C::SPLIT && p_half ? kPageRows * HD : C::STAGE;
+            mbar_arrive_expect_tx(bars + 8 * p_st, bytes);
+            bulk_load(ring_u32 + p_st * C::STAGE, p_half ? p_src + tile_at(HD, 1) : p_src, bytes, bars + 8 * p_st);
+        }
+        if constexpr (C::SPLIT) p_half = !p_half;
+        ++issued;
+        p_st = p_st + 1 == NS ? 0 : p_st + 1;
+    };
+    // Stages that may be refilled; one of them is kept back at the start and end of
+    // a piece, for its q and its result.
+    int free_stages = NS;
+    auto refill = [&](int keep) {
+#pragma unroll 1
+        for (; free_stages > keep; --free_stages) prefetch();
+    };
+    refill(1);
+
+    int c_st = 0;
+    uint32_t c_par = 0;  // the stage read next, and its phase
+    auto wait = [&](int at, uint32_t par) {
+        const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * at, par, abort_flag, a.err, a.dbg, 40,
+                                                                  issued, true, a.wait_limit));
+        dead = dead || !ok;
+    };
+    auto advance = [&]() {
+        ++free_stages;
+        if (++c_st == NS) {
+            c_st = 0;
+            c_par ^= 1u;
+        }
+    };
     StepWarp<HD, GP, DT> sw;
-    while (cw.next(a, p)) {
-        sw.begin(a, p, lane);
+    for (; more; more = cw.next(a, p)) {
+        if (!p.coop && warp != p.rot) continue;
+        // the stage kept back: the one read last (at the start, the last one)
+        const int l_st = c_st == 0 ? NS - 1 : c_st - 1;
+        unsigned char* o_mine = ring + l_st * C::STAGE + (C::SPLIT ? 0 : tile_at(HD, 1));
+        const int step = p.coop ? W : 1;
+        const int first = p.coop ? (warp - p.rot) & (W - 1) : 0;
+        const bool any = first < p.n;
+        if (any) {
+            sw.begin(a, p, reinterpret_cast<float*>(o_mine), lane);
+            fence_proxy_async_shared();  // what the stage held, before its next bulk copy
+            __syncwarp();
+        }
         const PagedRun& run = a.runs[p.run];
         const PagedLayer L = a.layers[p.layer];
         const int last_row = run.pos0 + run.n - 1;
         // pages every column attends in full need no test of their rows
         const int lo_all = (L.flags & kLayerWindow) ? max(0, last_row - a.window + 1) : 0;
-        for (int i = (warp - p.x0 % W + W) % W; i < p.n; i += W) {
-            const int st = used % NS;
-            const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * st, (used / NS) & 1, abort_flag, a.err,
-                                                                      a.dbg, 40, used, true, a.wait_limit));
-            ++used;
-            unsigned char* rec = ring + st * C::R;
-            const int row0 = (p.page0 + i) * kPageRows;
-            if (ok) {
-                if (a.append && (L.flags & kLayerAppend) && run.pos0 / kPageRows == p.page0 + i) {
-                    const int id = a.table[static_cast<long long>(run.seq) * a.max_pages + p.page0 + i];
-                    step_append<HD, DT>(a, p, rec, a.pool + id * a.page_bytes + L.cache_layer * a.layer_bytes +
-                                                       static_cast<long long>(p.h) * C::R, lane);
-                }
-                sw.page(a, rec, row0, row0 < lo_all || row0 + kPageRows - 1 > run.pos0, lane);
+        const int append_page = a.append && (L.flags & kLayerAppend) ? run.pos0 / kPageRows - p.page0 : -1;
+        for (int i = first; i < p.n; i += step) {
+            refill(0);
+            wait(c_st, c_par);
+            unsigned char* rec = ring + c_st * C::STAGE;
+            unsigned char* vt = rec + tile_at(HD, 1);
+            if constexpr (C::SPLIT) {
+                const int v_st = c_st + 1 == NS ? 0 : c_st + 1;
+                vt = ring + v_st * C::STAGE;
+                if (i == append_page) wait(v_st, v_st == 0 ? c_par ^ 1u : c_par);
             }
-            __syncwarp();  // every lane has read the record before it is overwritten
-            prefetch();
+            const int row0 = (p.page0 + i) * kPageRows;
+            if (!dead) {
+                if (i == append_page) {
+                    const int id = a.table[static_cast<long long>(run.seq) * a.max_pages + p.page0 + i];
+                    step_append<HD, DT>(a, p, rec, rec + tile_at(HD, 0), vt,
+                                        a.pool + id * a.page_bytes + L.cache_layer * a.layer_bytes +
+                                            static_cast<long long>(p.h) * record_bytes(HD), lane);
+                }
+                sw.scores(a, rec + tile_at(HD, 0), *reinterpret_cast<const float4*>(rec), row0,
+                          row0 < lo_all || row0 + kPageRows - 1 > run.pos0, lane);
+            }
+            if constexpr (C::SPLIT) {
+                advance();
+                wait(c_st, c_par);
+            }
+            if (!dead) sw.values(smem_u32(vt), lane);
+            advance();
+            __syncwarp();  // every lane has read the stages before they are refilled
         }
-        sw.finish(o_s + warp * GP * HD, ml_s + warp * GP * 2, lane);
+        // the last stage read carries the result; the others are refilled meanwhile
+        const int r_st = c_st == 0 ? NS - 1 : c_st - 1;
+        o_mine = ring + r_st * C::STAGE + (C::SPLIT ? 0 : tile_at(HD, 1));
+        refill(1);
+        const int ncol = run.n * a.G;
+        auto out_at = [&](int col, int d) {  // of a column: a head, or a token's head
+            const int tok = run.n > 1 ? col / a.G : 0;
+            const long long io = static_cast<long long>(run.io0 + tok) * a.n_io_layers + L.io;
+            return a.out + io * a.q_stride + (p.h * a.G + col - tok * a.G) * HD + d;
+        };
+        if (!p.coop) {
+            // a whole segment, read by this warp alone
+            float* ml = ml_s + warp * GP * 2;
+            sw.finish(reinterpret_cast<float*>(o_mine), ml, lane);
+            __syncwarp();
+            for (int e = lane; e < ncol * HD; e += 32) {
+                *out_at(e / HD, e % HD) = __fdividef(reinterpret_cast<const float*>(o_mine)[e], ml[e / HD * 2 + 1]);
+            }
+            __syncwarp();
+            continue;
+        }
+        if (any) {
+            sw.finish(reinterpret_cast<float*>(o_mine), ml_s + warp * GP * 2, lane);
+        } else if (lane < GP) {
+            ml_s[(warp * GP + lane) * 2] = -INFINITY;
+            ml_s[(warp * GP + lane) * 2 + 1] = 0.0f;
+        }
+        if (lane == 0) o_at[warp] = any ? static_cast<int>(o_mine - smem) : -1;
         __syncthreads();
         // ---- the warps' parts joined: the segment's output, or a partial of it
         const bool whole = p.n == p.seg_n;
-        const int ncol = run.n * a.G;
-        float* part = a.scratch + static_cast<long long>(p.x0 == b0 ? 2 * c : 2 * c + 1) * (GP * (HD + 2));
-        for (int e = threadIdx.x; e < ncol * HD; e += W * 32) {
+        float* part = a.scratch + static_cast<long long>(p.in_seg == 0 ? 2 * c + 1 : 2 * c) * C::PART;
+#pragma unroll 1
+        for (int e = threadIdx.x * 2; e < ncol * HD; e += W * 32 * 2) {
             const int col = e / HD, d = e % HD;
+            float2 ml[W];
             float M = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < W; ++w) M = fmaxf(M, ml_s[(w * GP + col) * 2]);
-            float Ls = 0.0f, O = 0.0f;
+            for (int w = 0; w < W; ++w) {
+                ml[w] = *reinterpret_cast<const float2*>(ml_s + (w * GP + col) * 2);
+                M = fmaxf(M, ml[w].x);
+            }
+            float Ls = 0.0f;
+            float2 O = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const float mw = ml_s[(w * GP + col) * 2];
-                const float f = mw == -INFINITY ? 0.0f : ex2_approx(mw - M);
-                Ls = fmaf(ml_s[(w * GP + col) * 2 + 1], f, Ls);
-                O = fmaf(o_s[(w * GP + col) * HD + d], f, O);
+                if (ml[w].x == -INFINITY) continue;
+                const float f = ex2_approx(ml[w].x - M);
+                const float2 o = *reinterpret_cast<const float2*>(smem + o_at[w] + e * 4);
+                Ls = fmaf(ml[w].y, f, Ls);
+                O = make_float2(fmaf(o.x, f, O.x), fmaf(o.y, f, O.y));
             }
             if (whole) {
-                const long long io = static_cast<long long>(run.io0 + col / a.G) * a.n_io_layers + L.io;
-                a.out[io * a.q_stride + (p.h * a.G + col % a.G) * HD + d] = O / Ls;
+                float* dst = out_at(col, d);
+                const float inv = __fdividef(1.0f, Ls);
+                dst[0] = O.x * inv;
+                dst[1] = O.y * inv;
             } else {
-                part[col * (HD + 2) + d] = O;
-                if (d == 0) {
-                    part[col * (HD + 2) + HD] = M;
-                    part[col * (HD + 2) + HD + 1] = Ls;
-                }
+                *reinterpret_cast<float2*>(part + e) = O;
+                if (d == 0) *reinterpret_cast<float2*>(part + GP * HD + 2 * col) = make_float2(M, Ls);
             }
         }
         if (!whole) {
-            const int c0 = static_cast<int>(owner_of(p.seg_x0, a.total, P));
-            const int c1 = static_cast<int>(owner_of(p.seg_x0 + p.seg_n - 1, a.total, P));
+            const int c0 = static_cast<int>(owner_of(p.seg_x0 + kPieceCost, a.total, P));
+            const int c1 = static_cast<int>(owner_of(p.seg_x0 + kPieceCost + p.seg_n - 1, a.total, P));
             __syncthreads();
             if (threadIdx.x == 0) *flag = atomic_add_acq_rel_gpu(a.counters + c0, 1) == c1 - c0;
             __syncthreads();
@@ -617,42 +772,49 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
                 // the last of the segment's CTAs
                 if (threadIdx.x == 0) a.counters[c0] = 0;
                 fence_acq_rel_gpu();
-                const int s0 = p.seg_x0 == static_cast<int>(static_cast<long long>(a.total) * c0 / P) ? 2 * c0 : 2 * c0 + 1;
-                constexpr int Q = 8;
-                for (int e = threadIdx.x; e < ncol * HD; e += W * 32) {
+                constexpr int Q = 8;  // parts whose loads are in flight together
+                for (int e = threadIdx.x * 4; e < ncol * HD; e += W * 32 * 4) {
                     const int col = e / HD, d = e % HD;
-                    float M = -INFINITY, Ls = 0.0f, O = 0.0f;
+                    float M = -INFINITY, Ls = 0.0f;
+                    float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     for (int q0 = c0; q0 <= c1; q0 += Q) {
-                        float mv[Q], lv[Q], ov[Q];
+                        float2 ml[Q];
+                        float4 ov[Q];
 #pragma unroll
                         for (int q = 0; q < Q; ++q) {
-                            const bool on = q0 + q <= c1;
-                            const float* src = a.scratch + static_cast<long long>(q0 + q == c0 ? s0 : 2 * (q0 + q)) * (GP * (HD + 2)) + col * (HD + 2);
-                            mv[q] = on ? __ldcg(src + HD) : -INFINITY;
-                            lv[q] = on ? __ldcg(src + HD + 1) : 0.0f;
-                            ov[q] = on ? __ldcg(src + d) : 0.0f;
+                            // beyond the last part: the last one again, with no weight
+                            const int cq = min(q0 + q, c1);
+                            const float* src = a.scratch + static_cast<long long>(cq == c0 ? 2 * c0 + 1 : 2 * cq) * C::PART;
+                            ml[q] = __ldcg(reinterpret_cast<const float2*>(src + GP * HD + 2 * col));
+                            ov[q] = __ldcg(reinterpret_cast<const float4*>(src + e));
+                            if (q0 + q > c1) ml[q].x = -INFINITY;
                         }
                         float Mn = M;
 #pragma unroll
-                        for (int q = 0; q < Q; ++q) Mn = fmaxf(Mn, mv[q]);
+                        for (int q = 0; q < Q; ++q) Mn = fmaxf(Mn, ml[q].x);
                         if (Mn == -INFINITY) continue;
                         const float f0 = M == -INFINITY ? 0.0f : ex2_approx(M - Mn);
                         Ls *= f0;
-                        O *= f0;
+                        O = make_float4(O.x * f0, O.y * f0, O.z * f0, O.w * f0);
 #pragma unroll
                         for (int q = 0; q < Q; ++q) {
-                            const float f = mv[q] == -INFINITY ? 0.0f : ex2_approx(mv[q] - Mn);
-                            Ls = fmaf(lv[q], f, Ls);
-                            O = fmaf(ov[q], f, O);
+                            const float f = ml[q].x == -INFINITY ? 0.0f : ex2_approx(ml[q].x - Mn);
+                            Ls = fmaf(ml[q].y, f, Ls);
+                            O = make_float4(fmaf(ov[q].x, f, O.x), fmaf(ov[q].y, f, O.y), fmaf(ov[q].z, f, O.z),
+                                            fmaf(ov[q].w, f, O.w));
                         }
                         M = Mn;
                     }
-                    const long long io = static_cast<long long>(run.io0 + col / a.G) * a.n_io_layers + L.io;
-                    a.out[io * a.q_stride + (p.h * a.G + col % a.G) * HD + d] = O / Ls;
+                    float* dst = out_at(col, d);
+                    const float inv = __fdividef(1.0f, Ls);
+                    dst[0] = O.x * inv;
+                    dst[1] = O.y * inv;
+                    dst[2] = O.z * inv;
+                    dst[3] = O.w * inv;
                 }
             }
         }
-        __syncthreads();  // o_s, ml_s and flag before the next piece writes them
+        __syncthreads();  // o, ml_s and flag are read before they are written again
     }
     // every copy has landed before the CTA exits, after a wait that ran out too
     for (int k = max(0, issued - NS); k < issued; ++k)
@@ -672,7 +834,9 @@ cudaError_t step_launch_one(const PagedArgs& a, int num_sms, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         if (dev < 64) set[dev] = true;
     }
-    const int grid = std::max(1, std::min(num_sms * C::CTAS, (a.total + C::W - 1) / C::W));
+    // no more CTAs than give each warp a page
+    const int per = C::W + kPieceCost;
+    const int grid = std::max(1, std::min(num_sms * C::CTAS, (a.total + per - 1) / per));
     paged_step_kernel<HD, GP, DT><<<grid, C::W * 32, C::SMEM, st>>>(a);
     return cudaGetLastError();
 }

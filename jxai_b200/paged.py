@@ -103,19 +103,19 @@ class PagedKVCache:
     def fork(self, src: int, dst: int, n_rows: int | None = None, stream=None) -> None:
         """dst becomes the first n_rows rows of src (default: all), on the same pages."""
         n = self.seq_pos(src) if n_rows is None else n_rows
-        check(self.lib.jx_pkv_fork(self.handle, src, dst, n, _stream_ptr(stream)))
+        check(self.lib.jx_pkv_fork(self.handle, src, dst, n, _stream_ptr(stream, self.device)))
 
     def copy(self, src: int, dst: int, stream=None) -> None:
         """dst becomes a copy of src on pages of its own."""
-        check(self.lib.jx_pkv_copy(self.handle, src, dst, _stream_ptr(stream)))
+        check(self.lib.jx_pkv_copy(self.handle, src, dst, _stream_ptr(stream, self.device)))
 
     def keep(self, seq: int, rows: Sequence[int], stream=None) -> None:
         """Cuts the sequence down to the given rows (ascending), in every layer."""
         arr = _i32_array(rows)
-        check(self.lib.jx_pkv_keep(self.handle, seq, arr, len(arr), _stream_ptr(stream)))
+        check(self.lib.jx_pkv_keep(self.handle, seq, arr, len(arr), _stream_ptr(stream, self.device)))
 
     def compact(self, seq: int, keep_recent: int = 128, stream=None) -> None:
-        check(self.lib.jx_pkv_compact(self.handle, seq, keep_recent, _stream_ptr(stream)))
+        check(self.lib.jx_pkv_compact(self.handle, seq, keep_recent, _stream_ptr(stream, self.device)))
 
     # contents ---------------------------------------------------------------
     def _tensor(self, t, name: str, shape, dtypes):
@@ -141,7 +141,7 @@ class PagedKVCache:
                 self._tensor(v_codes, "v_codes", codes, kinds),
                 self._tensor(v_scales, "v_scales", scales, (torch.float32,))]
         check(self.lib.jx_pkv_load_rows(self.handle, seq, row0, n, *(t.data_ptr() for t in keep),
-                                        _stream_ptr(stream)))
+                                        _stream_ptr(stream, self.device)))
 
     def read(self, seqs: Sequence[int], row0: Sequence[int], n_rows: int, dtype=None, out=None,
              stream=None):
@@ -153,14 +153,17 @@ class PagedKVCache:
         if len(ids) != len(first):
             raise JxError(-1, "read: one first row per sequence")
         shape = (len(ids), self.n_layers, 2, n_rows, self.n_kv_heads, self.head_dim)
+        if dtype not in (None, torch.bfloat16, torch.float32):
+            raise JxError(-1, "rows are read as bfloat16 or float32")
         if out is None:
-            out = torch.empty(shape, dtype=dtype or torch.bfloat16, device=f"cuda:{self.device}")
-        if (not out.is_cuda or tuple(out.shape) != shape or not out.is_contiguous()
-                or out.dtype not in (torch.bfloat16, torch.float32)):
+            out = torch.empty(shape, dtype=dtype or torch.bfloat16,
+                              device=torch.device("cuda", self.device))
+        elif (not out.is_cuda or tuple(out.shape) != shape or not out.is_contiguous()
+                or out.dtype not in ((torch.bfloat16, torch.float32) if dtype is None else (dtype,))):
             raise JxError(-1, f"out must be a contiguous CUDA tensor {shape} of bfloat16 or float32")
         kind = JX_F32 if out.dtype == torch.float32 else JX_BF16
         check(self.lib.jx_pkv_read_rows(self.handle, ids, first, len(ids), n_rows, kind,
-                                        out.data_ptr(), _stream_ptr(stream)))
+                                        out.data_ptr(), _stream_ptr(stream, self.device)))
         return out
 
     # plumbing -----------------------------------------------------------------
@@ -169,7 +172,7 @@ class PagedKVCache:
 
     def check_device_error(self, stream=None) -> int:
         code = C.c_int()
-        rc = self.lib.jx_pkv_check_device_error(self.handle, C.byref(code), _stream_ptr(stream))
+        rc = self.lib.jx_pkv_check_device_error(self.handle, C.byref(code), _stream_ptr(stream, self.device))
         if rc not in (0, -6):
             check(rc)
         return code.value
