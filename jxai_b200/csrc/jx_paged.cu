@@ -8,6 +8,8 @@
 // has to outlive the call.
 #include "jx_paged.h"
 
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 #include <cmath>
 #include <cstdarg>
@@ -43,6 +45,20 @@ int pfail(int code, const char* fmt, ...) {
         if (e_ != cudaSuccess)                                                            \
             return pfail(JX_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(e_));    \
     } while (0)
+
+using TensorMapEncode = PFN_cuTensorMapEncodeTiled_v12000;
+TensorMapEncode tensor_map_encode() {
+    static TensorMapEncode fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<TensorMapEncode>(p);
+    });
+    return fn;
+}
 
 struct OnDevice {  // the handle's device for the duration of a call
     int prev = -1;
@@ -341,6 +357,92 @@ __global__ void read_kernel(const __grid_constant__ ReadArgs a) {
     }
 }
 
+// Rows of a prompt's sequences from codes to fp16, for the tensor-core prompt
+// kernel: out [slot][layer][rows][n_kv * HD], K and V.
+struct WidenArgs {
+    const unsigned char* pool;
+    const int* table;
+    uint16_t* out[2];
+    float2* head_scale;   // [slot][layer][kv head]
+    long long page_bytes;
+    long long layer_bytes;
+    long long slot_elems; // elements of a slot (all layers) and of a layer in `out`
+    long long layer_elems;
+    int max_pages, n_kv, n_layers, n_runs, window;
+    PagedLayer layers[kMaxCallLayers];
+    PagedRun runs[kMaxRuns];  // off: first row chunk
+};
+static_assert(sizeof(WidenArgs) <= 4096, "kernel parameters");
+
+constexpr int kWidenRows = 64;
+
+// A code times 2^(k - K), K so that the head's largest block exponent becomes 8:
+// exact in fp16 for blocks down to 2^-32 of the largest scale (below that a
+// value is off by 2^-33 of the largest), and never beyond 448 * 2^7.  The factor
+// 2^K of each head goes to the prompt kernel, which multiplies scores and
+// outputs by it.  One CTA per (64 rows, layer, kv head); the exponents of the
+// sequence's blocks (16 bytes per page) are read by every one of them.
+template <int HD, int DT>
+__global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ WidenArgs a) {
+    constexpr int kTop = DT == DT_I8 ? 8 : 7;
+    __shared__ int red[2][8];
+    int s = 0;
+    while (s + 1 < a.n_runs && a.runs[s + 1].off <= static_cast<int>(blockIdx.x)) ++s;
+    const PagedRun run = a.runs[s];
+    const int l = blockIdx.y / a.n_kv, h = blockIdx.y % a.n_kv;
+    const PagedLayer L = a.layers[l];
+    const int end = run.pos0 + run.n;
+    const int lo = (L.flags & kLayerWindow) ? max(0, run.pos0 - a.window + 1) : 0;
+    const int first = lo / kPageRows, last = (end - 1) / kPageRows;
+    const int row0 = lo / kWidenRows * kWidenRows + (static_cast<int>(blockIdx.x) - run.off) * kWidenRows;
+    if (row0 >= end) return;
+    const int* table = a.table + static_cast<long long>(run.seq) * a.max_pages;
+    const unsigned char* base = a.pool + L.cache_layer * a.layer_bytes + static_cast<long long>(h) * record_bytes(HD);
+    int ek = kMinExp, ev = kMinExp;
+    for (int p = first + threadIdx.x; p <= last; p += 256) {
+        const float4 sc = *reinterpret_cast<const float4*>(base + table[p] * a.page_bytes);
+        // a page's second block may begin behind the sequence's end
+        const bool two = p * kPageRows + kBlockRows < end;
+        ek = max(ek, max(scale_exp(sc.x), two ? scale_exp(sc.y) : kMinExp));
+        ev = max(ev, max(scale_exp(sc.z), two ? scale_exp(sc.w) : kMinExp));
+    }
+    ek = __reduce_max_sync(0xffffffffu, ek);
+    ev = __reduce_max_sync(0xffffffffu, ev);
+    if (threadIdx.x % 32 == 0) {
+        red[0][threadIdx.x / 32] = ek;
+        red[1][threadIdx.x / 32] = ev;
+    }
+    __syncthreads();
+    for (int w = 0; w < 8; ++w) {
+        ek = max(ek, red[0][w]);
+        ev = max(ev, red[1][w]);
+    }
+    ek -= kTop;
+    ev -= kTop;
+    if (blockIdx.x == static_cast<unsigned>(run.off) && threadIdx.x == 0)
+        a.head_scale[(static_cast<long long>(s) * a.n_layers + l) * a.n_kv + h] = make_float2(exp2_int(ek), exp2_int(ev));
+    constexpr int CPR = HD / 16;
+    for (int i = threadIdx.x; i < kWidenRows * CPR * 2; i += 256) {
+        const int which = i / (kWidenRows * CPR), c = i % CPR, t = row0 + i / CPR % kWidenRows;
+        if (t < lo || t >= end) continue;
+        const unsigned char* rec = base + table[t / kPageRows] * a.page_bytes;
+        const int k = scale_exp(reinterpret_cast<const float*>(rec)[which * 2 + (t / kBlockRows & 1)]) - (which ? ev : ek);
+        const float f = exp2_int(max(k, -60));
+        float x[16];
+        unpack_codes<DT>(*reinterpret_cast<const uint4*>(rec + tile_at(HD, which) + tile_byte(HD, t % kPageRows, c * 16)), x);
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const __half2 v = __floats2half2_rn(x[2 * j] * f, x[2 * j + 1] * f);
+            w[j] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        uint4* dst = reinterpret_cast<uint4*>(a.out[which] + s * a.slot_elems + l * a.layer_elems +
+                                              (static_cast<long long>(t) * a.n_kv + h) * HD + c * 16);
+        dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+
 // Calls f(integral_constant<HD>, integral_constant<DT>) for a cache's format.
 template <int V>
 using Int = std::integral_constant<int, V>;
@@ -381,11 +483,18 @@ struct jx_pkv {
     int* d_counters = nullptr;
     int* d_err = nullptr;
     int* d_dbg = nullptr;
-    int* d_rows = nullptr;                // keep: row list and source page table
-    size_t d_rows_n = 0;
-    int* h_rows = nullptr;                // pinned
-    size_t h_rows_n = 0;
-    cudaEvent_t ev_rows = nullptr;        // the copy out of h_rows
+    struct Upload {                       // a list for a kernel: pinned, and its device copy
+        void* h = nullptr;
+        void* d = nullptr;
+        size_t bytes = 0;
+        cudaEvent_t done = nullptr;       // the kernels that read the device copy
+        bool pending = false;
+    } up[2];
+    int up_next = 0;
+    uint16_t* d_wide = nullptr;           // prompts: fp16 rows of a group of layers
+    size_t wide_bytes = 0;
+    float2* d_head_scale = nullptr;
+    size_t head_scales = 0;
     int num_sms = 0;
     int opt_wait_limit_ms = 0;
     int last_launches = 0;
@@ -562,6 +671,55 @@ int check_device_ptr(const void* p, const char* name, int device) {
     return pfail(JX_ERR_INVALID, "%s must be memory of device %d", name, device);
 }
 
+// A pinned buffer of `bytes` and its device copy, free to be written: used in
+// turn, so that a call prepares its list while the previous one's is in use.
+int take_upload(jx_pkv* kv, size_t bytes, jx_pkv::Upload** out) {
+    jx_pkv::Upload& u = kv->up[kv->up_next];
+    kv->up_next ^= 1;
+    if (!u.done) PKV_CUDA(cudaEventCreateWithFlags(&u.done, cudaEventDisableTiming));
+    if (u.pending) PKV_CUDA(cudaEventSynchronize(u.done));
+    u.pending = false;
+    if (u.bytes < bytes) {
+        if (u.h) PKV_CUDA(cudaFreeHost(u.h));
+        u.h = nullptr;
+        if (u.d) PKV_CUDA(cudaFree(u.d));
+        u.d = nullptr;
+        u.bytes = 0;
+        if (cudaHostAlloc(&u.h, 2 * bytes, cudaHostAllocDefault) != cudaSuccess ||
+            cudaMalloc(&u.d, 2 * bytes) != cudaSuccess) {
+            cudaGetLastError();
+            return pfail(JX_ERR_NOMEM, "list of %zu bytes failed", 2 * bytes);
+        }
+        u.bytes = 2 * bytes;
+    }
+    *out = &u;
+    return JX_OK;
+}
+
+// Queues the copy, and after the kernels that read it, the buffer's release.
+int send_upload(jx_pkv::Upload* u, size_t bytes, cudaStream_t st) {
+    PKV_CUDA(cudaMemcpyAsync(u->d, u->h, bytes, cudaMemcpyHostToDevice, st));
+    return JX_OK;
+}
+int release_upload(jx_pkv::Upload* u, cudaStream_t st) {
+    PKV_CUDA(cudaEventRecord(u->done, st));
+    u->pending = true;
+    return JX_OK;
+}
+
+int grow_device(void** p, size_t* have, size_t need, const char* what) {
+    if (*have >= need) return JX_OK;
+    if (*p) PKV_CUDA(cudaFree(*p));  // (waits for the device)
+    *p = nullptr;
+    *have = 0;
+    if (cudaMalloc(p, need) != cudaSuccess) {
+        cudaGetLastError();
+        return pfail(JX_ERR_NOMEM, "%s of %zu bytes failed", what, need);
+    }
+    *have = need;
+    return JX_OK;
+}
+
 // The rows of a call written to the given layers.
 int append_rows(jx_pkv* kv, PagedArgs& A, const std::vector<PagedLayer>& part, const std::vector<PagedRun>& runs,
                 cudaStream_t st, int* launches) {
@@ -634,6 +792,180 @@ int step_rows(jx_pkv* kv, PagedArgs& A, const std::vector<PagedLayer>& part, con
         }
     }
     return JX_OK;
+}
+
+// Tokens of a sequence from which on a prompt goes to the tensor-core kernel.
+constexpr int kPromptTokens = 48;
+// fp16 rows held at one time: a group of layers whose rows stay in L2 between
+// the kernel that writes them and the one that reads them.
+constexpr size_t kWideBudget = size_t{48} << 20;
+
+// Prompt attention on the tensor cores: the rows of a group of layers are
+// brought to fp16 (exact, see widen_kernel), then prefill_tc_kernel runs over
+// them as over an fp16 cache.  Its work items are laid out for its persistent
+// CTAs here: longest first, dealt in turn and back.
+int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all, const std::vector<PagedRun>& runs,
+              cudaStream_t st, int* launches) {
+    const jx_pkv_desc& D = kv->d;
+    const int hd = static_cast<int>(D.head_dim), G = A.G, TQ = 128 / G, BN = prefill_tc_rows(hd);
+    const TensorMapEncode enc = tensor_map_encode();
+    if (!enc) return pfail(JX_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    struct Group {
+        size_t r0, nr;
+        std::vector<PagedLayer> layers;
+        long long rows;          // per slot
+        size_t items, at_items, at_first;
+        int grid;
+    };
+    std::vector<Group> groups;
+    const size_t row_bytes = static_cast<size_t>(D.n_kv_heads) * hd * 2;
+    for (size_t r0 = 0; r0 < runs.size();) {
+        // sequences whose rows of one layer fit the budget go together (one at least)
+        long long rows = 0;
+        size_t nr = 0;
+        while (r0 + nr < runs.size() && nr < kMaxRuns) {
+            const long long t = (static_cast<long long>(runs[r0 + nr].pos0) + runs[r0 + nr].n + 127) / 128 * 128;
+            const long long m = std::max<long long>(rows, t);
+            if (nr > 0 && 2 * row_bytes * m * (nr + 1) > kWideBudget) break;
+            rows = m;
+            ++nr;
+        }
+        const size_t layer_bytes = 2 * row_bytes * rows * nr;
+        const size_t per = std::min<size_t>(kMaxCallLayers, std::max<size_t>(1, kWideBudget / layer_bytes));
+        // layers of one RoPE setting share a launch
+        std::vector<PagedLayer> order = all;
+        std::stable_sort(order.begin(), order.end(), [](const PagedLayer& x, const PagedLayer& y) { return x.cfg < y.cfg; });
+        for (size_t l0 = 0; l0 < order.size();) {
+            Group g{r0, nr, {}, rows, 0, 0, 0, 0};
+            while (l0 < order.size() && g.layers.size() < per && (g.layers.empty() || order[l0].cfg == g.layers[0].cfg))
+                g.layers.push_back(order[l0++]);
+            groups.push_back(std::move(g));
+        }
+        r0 += nr;
+    }
+    // the work items of every group, in one list
+    std::vector<PrefillTile> items;
+    std::vector<int> firsts;
+    std::vector<PrefillTile> tiles, sorted;
+    for (Group& g : groups) {
+        tiles.clear();
+        for (size_t i = 0; i < g.nr; ++i) {
+            const PagedRun& r = runs[g.r0 + i];
+            for (int j = 0; j < r.n; j += TQ)
+                for (size_t l = 0; l < g.layers.size(); ++l) {
+                    const PagedLayer& L = g.layers[l];
+                    PrefillTile t{};
+                    t.seq = static_cast<int>(i);
+                    t.cache_layer = static_cast<int>(l);
+                    t.io0 = (r.io0 + j) * A.n_io_layers + L.io;
+                    t.io_step = A.n_io_layers;
+                    t.tok_row0 = r.pos0 + j;
+                    t.ntok = std::min(TQ, r.n - j);
+                    t.window = (L.flags & kLayerWindow) ? A.window : 0;
+                    t.rope_row0 = t.tok_row0;
+                    t.rope_half = L.half;
+                    t.kv_lo = t.window > 0 ? std::max(0, t.tok_row0 - t.window + 1) : 0;
+                    t.n_tiles = (t.tok_row0 + t.ntok - t.kv_lo + BN - 1) / BN;
+                    tiles.push_back(t);
+                }
+        }
+        std::stable_sort(tiles.begin(), tiles.end(), [](const PrefillTile& x, const PrefillTile& y) { return x.n_tiles > y.n_tiles; });
+        const size_t n = tiles.size() * D.n_kv_heads;
+        g.items = n;
+        g.grid = static_cast<int>(std::min<size_t>(std::max(kv->num_sms, 1), n));
+        g.at_items = items.size();
+        g.at_first = firsts.size();
+        const size_t P = static_cast<size_t>(g.grid);
+        items.resize(items.size() + n);
+        // CTA c runs the items at its place in each round of P, every other round reversed
+        size_t at = g.at_items;
+        for (size_t c = 0; c < P; ++c) {
+            firsts.push_back(static_cast<int>(at - g.at_items));
+            for (size_t round = 0;; ++round) {
+                const size_t i = round * P + (round % 2 ? P - 1 - c : c);
+                if (round * P >= n) break;
+                if (i >= n) continue;
+                items[at] = tiles[i / D.n_kv_heads];
+                items[at++].kvh = static_cast<int>(i % D.n_kv_heads);
+            }
+        }
+        firsts.push_back(static_cast<int>(at - g.at_items));
+    }
+    const size_t first_at = items.size() * sizeof(PrefillTile);
+    const size_t bytes = first_at + firsts.size() * sizeof(int);
+    size_t wide = 0, heads = 0;
+    for (const Group& g : groups) {
+        wide = std::max<size_t>(wide, 2 * row_bytes * g.rows * g.nr * g.layers.size());
+        heads = std::max<size_t>(heads, g.nr * g.layers.size() * D.n_kv_heads);
+    }
+    if (int rc = grow_device(reinterpret_cast<void**>(&kv->d_wide), &kv->wide_bytes, wide, "fp16 rows")) return rc;
+    if (int rc = grow_device(reinterpret_cast<void**>(&kv->d_head_scale), &kv->head_scales, heads * sizeof(float2), "head scales")) return rc;
+    jx_pkv::Upload* u = nullptr;
+    if (int rc = take_upload(kv, bytes, &u)) return rc;
+    std::memcpy(u->h, items.data(), first_at);
+    std::memcpy(static_cast<char*>(u->h) + first_at, firsts.data(), firsts.size() * sizeof(int));
+    if (int rc = send_upload(u, bytes, st)) return rc;
+    for (const Group& g : groups) {
+        const size_t nl = g.layers.size();
+        WidenArgs w{};
+        w.pool = kv->pool;
+        w.table = kv->d_table;
+        w.page_bytes = kv->page_bytes;
+        w.layer_bytes = kv->layer_bytes;
+        w.layer_elems = static_cast<long long>(g.rows) * D.n_kv_heads * hd;
+        w.slot_elems = w.layer_elems * static_cast<long long>(nl);
+        w.out[0] = kv->d_wide;
+        w.out[1] = kv->d_wide + w.slot_elems * static_cast<long long>(g.nr);
+        w.head_scale = kv->d_head_scale;
+        w.max_pages = A.max_pages;
+        w.n_kv = A.n_kv;
+        w.n_layers = static_cast<int>(nl);
+        w.n_runs = static_cast<int>(g.nr);
+        w.window = A.window;
+        std::copy(g.layers.begin(), g.layers.end(), w.layers);
+        int chunks = 0;
+        for (size_t i = 0; i < g.nr; ++i) {
+            w.runs[i] = runs[g.r0 + i];
+            w.runs[i].off = chunks;
+            chunks += (w.runs[i].pos0 + w.runs[i].n + kWidenRows - 1) / kWidenRows;
+        }
+        const dim3 grid(chunks, static_cast<unsigned>(nl * A.n_kv));
+        dispatch(D, [&](auto h, auto dt) { widen_kernel<h.value, dt.value><<<grid, 256, 0, st>>>(w); });
+        if (int rc = launched("widen")) return rc;
+        CUtensorMap maps[2];
+        const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D.n_kv_heads) * hd, static_cast<cuuint64_t>(g.rows), nl, g.nr};
+        const cuuint64_t strides[3] = {row_bytes, row_bytes * g.rows, row_bytes * g.rows * nl};
+        const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(BN), 1, 1};
+        const cuuint32_t one[4] = {1, 1, 1, 1};
+        for (int k = 0; k < 2; ++k)
+            if (enc(&maps[k], CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, w.out[k], dims, strides, box, one,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+                return pfail(JX_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+        PrefillArgs p{};
+        p.tiles = reinterpret_cast<const PrefillTile*>(u->d) + g.at_items;
+        p.cta_first = reinterpret_cast<const int*>(static_cast<const char*>(u->d) + first_at) + g.at_first;
+        p.n_items = static_cast<int>(g.items);
+        p.neox = A.neox;
+        p.q_vec = A.q_vec;
+        p.q = A.q;
+        p.out = A.out;
+        p.q_stride = A.q_stride;
+        p.rope = A.rope[g.layers[0].cfg];
+        p.scale = A.scale;
+        p.softcap = A.softcap;
+        p.inv_softcap = A.softcap > 0.0f ? 1.0f / A.softcap : 0.0f;
+        p.err = A.err;
+        p.dbg = A.dbg;
+        p.wait_limit = A.wait_limit;
+        p.head_scale = kv->d_head_scale;
+        p.scale_layers = static_cast<int>(nl);
+        p.scale_heads = A.n_kv;
+        const cudaError_t e = prefill_tc_launch(p, &maps[0], &maps[1], hd, DT_F16T, G, g.grid, st);
+        if (e != cudaSuccess) return pfail(JX_ERR_CUDA, "prompt launch failed: %s", cudaGetErrorString(e));
+        *launches += 2;
+    }
+    return release_upload(u, st);
 }
 
 int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const jx_step_args* a,
@@ -760,6 +1092,8 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
     A.q_vec = reinterpret_cast<uintptr_t>(a->q) % 16 == 0 && a->q_stride % 4 == 0;
     A.kv_vec = reinterpret_cast<uintptr_t>(a->k) % 16 == 0 && reinterpret_cast<uintptr_t>(a->v) % 16 == 0 &&
                a->kv_stride % 4 == 0;
+    // the prompt kernel writes its rows 16 bytes at a time
+    const bool out_vec = reinterpret_cast<uintptr_t>(a->out) % 16 == 0 && a->q_stride % 4 == 0;
     A.scratch = kv->d_scratch;
     A.counters = kv->d_counters;
     int launches = 0;
@@ -769,7 +1103,14 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
         for (const PagedLayer& L : all)
             if (L.flags & kLayerAppend) part.push_back(L);
         if (int rc = append_rows(kv, A, part, runs, st, &launches)) return rc;
-        // then attention, for blocks of as many tokens as fill the kernel's columns
+        // then attention: on the tensor cores, or (few tokens, or a shape that kernel
+        // does not take) for blocks of as many tokens as fill the step kernel's columns
+        if (prefill_tc_supported(static_cast<int>(D.head_dim), DT_F16T, static_cast<int>(G)) && out_vec &&
+            a->n_seqs >= kPromptTokens * runs.size()) {
+            if (int rc = prompt_tc(kv, A, all, runs, st, &launches)) return rc;
+            kv->last_launches = launches;
+            return JX_OK;
+        }
         const int nq = std::max(1, kStepCols / static_cast<int>(G));
         std::vector<PagedRun> blocks;
         for (const PagedRun& r : runs)
@@ -789,33 +1130,6 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
         }
     }
     kv->last_launches = launches;
-    return JX_OK;
-}
-
-// Device and pinned buffers of at least n ints for keep's row list.
-int ensure_rows(jx_pkv* kv, size_t n) {
-    if (!kv->ev_rows) PKV_CUDA(cudaEventCreateWithFlags(&kv->ev_rows, cudaEventDisableTiming));
-    else PKV_CUDA(cudaEventSynchronize(kv->ev_rows));  // the last list has left the pinned buffer
-    if (kv->h_rows_n < n) {
-        if (kv->h_rows) PKV_CUDA(cudaFreeHost(kv->h_rows));
-        kv->h_rows = nullptr;
-        kv->h_rows_n = 0;
-        if (cudaHostAlloc(reinterpret_cast<void**>(&kv->h_rows), 2 * n * sizeof(int), cudaHostAllocDefault) != cudaSuccess) {
-            cudaGetLastError();
-            return pfail(JX_ERR_NOMEM, "pinned buffer of %zu bytes failed", 2 * n * sizeof(int));
-        }
-        kv->h_rows_n = 2 * n;
-    }
-    if (kv->d_rows_n < n) {
-        if (kv->d_rows) PKV_CUDA(cudaFree(kv->d_rows));  // (waits for the device)
-        kv->d_rows = nullptr;
-        kv->d_rows_n = 0;
-        if (cudaMalloc(&kv->d_rows, 2 * n * sizeof(int)) != cudaSuccess) {
-            cudaGetLastError();
-            return pfail(JX_ERR_NOMEM, "row list of %zu bytes failed", 2 * n * sizeof(int));
-        }
-        kv->d_rows_n = 2 * n;
-    }
     return JX_OK;
 }
 
@@ -841,20 +1155,22 @@ int keep_impl(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, cu
                      fresh, kv->free_pages.size(), D.n_pages);
     // [rows][source pages][result pages]
     const size_t n_src = pg.size(), n_list = n_rows + n_src + n_pages;
-    if (int rc = ensure_rows(kv, n_list)) return rc;
-    std::memcpy(kv->h_rows, rows, n_rows * sizeof(int));
-    std::memcpy(kv->h_rows + n_rows, pg.data(), n_src * sizeof(int));
+    jx_pkv::Upload* u = nullptr;
+    if (int rc = take_upload(kv, n_list * sizeof(int), &u)) return rc;
+    int* list = static_cast<int*>(u->h);
+    std::memcpy(list, rows, n_rows * sizeof(int));
+    std::memcpy(list + n_rows, pg.data(), n_src * sizeof(int));
     std::vector<int> result(pg.begin(), pg.begin() + n_pages);
     if (!in_place)
         for (uint32_t i = keep_pages; i < n_pages; ++i) result[i] = take_page(kv);
-    std::memcpy(kv->h_rows + n_rows + n_src, result.data(), n_pages * sizeof(int));
-    PKV_CUDA(cudaMemcpyAsync(kv->d_rows, kv->h_rows, n_list * sizeof(int), cudaMemcpyHostToDevice, st));
-    PKV_CUDA(cudaEventRecord(kv->ev_rows, st));
+    std::memcpy(list + n_rows + n_src, result.data(), n_pages * sizeof(int));
+    if (int rc = send_upload(u, n_list * sizeof(int), st)) return rc;
+    const int* d_list = static_cast<const int*>(u->d);
     KeepArgs k{};
     k.pool = kv->pool;
-    k.rows = kv->d_rows;
-    k.src_table = kv->d_rows + n_rows;
-    k.dst_table = kv->d_rows + n_rows + n_src;
+    k.rows = d_list;
+    k.src_table = d_list + n_rows;
+    k.dst_table = d_list + n_rows + n_src;
     k.page_bytes = kv->page_bytes;
     k.n_rec = static_cast<int>(D.n_layers * D.n_kv_heads);
     k.n_rows = static_cast<int>(n_rows);
@@ -866,6 +1182,7 @@ int keep_impl(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, cu
         keep_kernel<hd.value, dt.value><<<grid, 2 * hd.value, 0, st>>>(k);
     });
     if (int rc = launched("keep")) return rc;
+    if (int rc = release_upload(u, st)) return rc;
     if (in_place) {
         drop_rows(kv, seq, n_rows);
         return JX_OK;
@@ -977,9 +1294,13 @@ int jx_pkv_destroy(jx_pkv* kv) {
     cudaFree(kv->d_counters);
     cudaFree(kv->d_err);
     cudaFree(kv->d_dbg);
-    cudaFree(kv->d_rows);
-    if (kv->h_rows) cudaFreeHost(kv->h_rows);
-    if (kv->ev_rows) cudaEventDestroy(kv->ev_rows);
+    cudaFree(kv->d_wide);
+    cudaFree(kv->d_head_scale);
+    for (auto& u : kv->up) {
+        cudaFree(u.d);
+        if (u.h) cudaFreeHost(u.h);
+        if (u.done) cudaEventDestroy(u.done);
+    }
     for (RopeCfg& r : kv->ropes) cudaFree(r.d_tab);
     delete kv;
     return JX_OK;

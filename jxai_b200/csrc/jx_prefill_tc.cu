@@ -580,7 +580,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
             const int n = tl.n_tiles;
             // unscale is a power of two: (S * unscale) * scale rounds once, as
             // the reference's dot * scale does
-            const float sc_mul = a.scale * unscale;
+            // (a cache held in 8 bits gives K and V of a head times powers of two)
+            const float2 hs = a.head_scale
+                                  ? __ldg(a.head_scale + (static_cast<long long>(tl.seq) * a.scale_layers +
+                                                          tl.cache_layer) * a.scale_heads + tl.kvh)
+                                  : make_float2(1.0f, 1.0f);
+            const float sc_mul = a.scale * unscale * hs.x;
             const bool capped = a.softcap > 0.0f;
             // columns every live row of the item attends: [lo_all, hi_all]
             const int hi_all = tl.tok_row0;  // the first token's row
@@ -721,7 +726,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
                 tc_fence_after();
                 float* dst = a.out + io * a.q_stride + static_cast<long long>(tl.kvh * G + h) * HD +
                              hf * HW;
-                const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
+                const float inv = lt > 0.0f ? hs.y / lt : 0.0f;
 #pragma unroll
                 for (int c = 0; c < HW; c += 32) {
                     uint32_t t32[32];

@@ -126,7 +126,9 @@ class Model:
                 # roundings (3 * 2^-24), one fp32 addition per 16 products and a few more
                 # operations ((HD/16 + 5) * 2^-23 of the sum of magnitudes).  A weight: twice
                 # the score's error (its own and the maximum's) and exp2's 2^-22; as parts of
-                # 16 bits 2^-22.  The sums over rows: one rounding (2^-23) per 16 rows.
+                # 16 bits 2^-22, or 2^-25 of the largest where it is small.  The sums over rows:
+                # one rounding (2^-23) per 16 rows.
                 ds = size * ((HD / 16 + 5) * 2.0 ** -23 + 2.0 ** -22 + 3 * 2.0 ** -24) + 2.0 ** -22
-                tol[i, h] = np.abs(Vr).max() * (4 * ds + 2.0 ** -21 + (len(p) / 16 + 4) * 2.0 ** -23)
+                tol[i, h] = np.abs(Vr).max() * (4 * ds + 2.0 ** -21 + (len(p) / 16 + 4) * 2.0 ** -23
+                                              + len(p) * 2.0 ** -25)
         return out.reshape(n, H * HD), np.broadcast_to(tol, (n, H, HD)).reshape(n, H * HD)

@@ -26,6 +26,7 @@ class Pair:
         self.model = Model(n_seqs, L, cap, HK, HD, dtype)
         self.rng = np.random.default_rng(seed)
         self.kw = dict(rope_dim=kw.get("rope_dim", HD), base=kw.get("base", 1e4), neox=kw.get("neox", True))
+        self.kw_layer = {}  # layer -> RoPE settings of its own
         self.swa = kw.get("swa", [False] * L)
         self.window, self.softcap = kw.get("window", 0), kw.get("softcap", 0.0)
         self.shares = kw.get("shares", {})  # layer -> layer whose rows it reads
@@ -65,7 +66,7 @@ class Pair:
                 ref, tol = self.model.step(
                     s, l, p, q[at:at + m, l], k[at:at + m, l], v[at:at + m, l], self.H, self.scale,
                     self.softcap, self.window if self.swa[l] else 0, append=l not in self.shares,
-                    src=self.shares.get(l, l), **self.kw)
+                    src=self.shares.get(l, l), **self.kw_layer.get(l, self.kw))
                 err = np.abs(got[at:at + m, l] - ref)
                 assert np.isfinite(got[at:at + m, l]).all()
                 assert (err <= tol).all(), (s, l, float((err / tol).max()), float(err.max()))
@@ -166,6 +167,36 @@ def test_padded_strides(dtype):
     p = Pair(4, 2, 64, dtype, L=2, cap=100, seed=5)
     p.run([(0, 0, 40)], True, pad=3)
     p.run([(0, 40, 1)], False, pad=3)
+
+
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+def test_long_prompts_after_rows(dtype):
+    """Prompts on the tensor cores: every group, both head widths, windows, soft caps, two RoPE
+    settings, rows cached before, several sequences of unlike lengths in one call."""
+    for H, HK, HD in [(2, 2, 64), (4, 2, 128), (4, 1, 64), (8, 1, 128), (8, 2, 128)]:
+        p = Pair(H, HK, HD, dtype, n_seqs=3, L=3, cap=420, swa=[False, True, True], window=70,
+                 softcap=15.0 if HD == 64 else 0.0, neox=HD == 64, rope_dim=HD // 2 if H == 4 else HD,
+                 seed=H + HD)
+        p.layers[2].rope_base = 1e6
+        x = p.inputs(130)
+        p.kw_layer = {2: dict(p.kw, base=1e6)}
+        p.run([(1, 0, 130)], True, inputs=x)
+        p.run([(0, 0, 49), (1, 130, 150), (2, 0, 131)], True, spread=2.0)
+        p.run([(1, 280, 1), (0, 49, 1)], False)
+
+
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+def test_scales_far_apart(dtype):
+    """Blocks whose scales differ by powers of two up to 2^24, and one head far larger than the
+    other: what each row is worth stays what it is."""
+    p = Pair(4, 2, 64, dtype, cap=300, seed=31)
+    q, k, v = p.inputs(200)
+    f = 2.0 ** (-8 * (np.arange(200) // 50))
+    k, v = k * f[:, None, None], v * f[:, None, None]
+    k[..., 64:] *= 1e-3
+    v[..., 64:] *= 1e3
+    p.run([(0, 0, 200)], True, inputs=[q, k.astype(np.float32), v.astype(np.float32)])
+    p.run([(0, 200, 1)], False)
 
 
 @pytest.mark.parametrize("dtype", ["int8", "e4m3"])
