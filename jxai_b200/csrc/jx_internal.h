@@ -132,9 +132,6 @@ struct PrefillArgs {
     int* err;
     int* dbg;
     long long wait_limit;
-    // (K, V) factors of each [seq][layer][kv head] of the cache, or null: 1
-    const float2* head_scale;
-    int scale_layers, scale_heads;
 };
 
 // Tensor-core prefill for (head_dim, cache dtype, query group) -- 16-bit

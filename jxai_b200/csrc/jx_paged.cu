@@ -368,7 +368,7 @@ struct WidenArgs {
     long long layer_bytes;
     long long slot_elems; // elements of a slot (all layers) and of a layer in `out`
     long long layer_elems;
-    int max_pages, n_kv, n_layers, n_runs, window;
+    int max_pages, n_kv, n_layers, n_runs, window, rows;
     PagedLayer layers[kMaxCallLayers];
     PagedRun runs[kMaxRuns];  // off: first row chunk
 };
@@ -395,7 +395,10 @@ __global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ Wide
     const int lo = (L.flags & kLayerWindow) ? max(0, run.pos0 - a.window + 1) : 0;
     const int first = lo / kPageRows, last = (end - 1) / kPageRows;
     const int row0 = lo / kWidenRows * kWidenRows + (static_cast<int>(blockIdx.x) - run.off) * kWidenRows;
-    if (row0 >= end) return;
+    // rows behind the last one that share its tile are zeros: their weights are 0,
+    // but 0 times what the buffer held before might not be
+    const int zeros = min(a.rows, end + kPromptRows);
+    if (row0 >= zeros) return;
     const int* table = a.table + static_cast<long long>(run.seq) * a.max_pages;
     const unsigned char* base = a.pool + L.cache_layer * a.layer_bytes + static_cast<long long>(h) * record_bytes(HD);
     int ek = kMinExp, ev = kMinExp;
@@ -424,7 +427,13 @@ __global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ Wide
     constexpr int CPR = HD / 16;
     for (int i = threadIdx.x; i < kWidenRows * CPR * 2; i += 256) {
         const int which = i / (kWidenRows * CPR), c = i % CPR, t = row0 + i / CPR % kWidenRows;
-        if (t < lo || t >= end) continue;
+        if (t < lo || t >= zeros) continue;
+        uint4* dst = reinterpret_cast<uint4*>(a.out[which] + s * a.slot_elems + l * a.layer_elems +
+                                              (static_cast<long long>(t) * a.n_kv + h) * HD + c * 16);
+        if (t >= end) {
+            dst[0] = dst[1] = make_uint4(0u, 0u, 0u, 0u);
+            continue;
+        }
         const unsigned char* rec = base + table[t / kPageRows] * a.page_bytes;
         const int k = scale_exp(reinterpret_cast<const float*>(rec)[which * 2 + (t / kBlockRows & 1)]) - (which ? ev : ek);
         const float f = exp2_int(max(k, -60));
@@ -436,8 +445,6 @@ __global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ Wide
             const __half2 v = __floats2half2_rn(x[2 * j] * f, x[2 * j + 1] * f);
             w[j] = *reinterpret_cast<const uint32_t*>(&v);
         }
-        uint4* dst = reinterpret_cast<uint4*>(a.out[which] + s * a.slot_elems + l * a.layer_elems +
-                                              (static_cast<long long>(t) * a.n_kv + h) * HD + c * 16);
         dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
         dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
@@ -796,18 +803,22 @@ int step_rows(jx_pkv* kv, PagedArgs& A, const std::vector<PagedLayer>& part, con
 
 // Tokens of a sequence from which on a prompt goes to the tensor-core kernel.
 constexpr int kPromptTokens = 48;
-// fp16 rows held at one time: a group of layers whose rows stay in L2 between
-// the kernel that writes them and the one that reads them.
-constexpr size_t kWideBudget = size_t{48} << 20;
+// fp16 rows held at one time.  A group of layers grows until its rows would
+// leave L2 (126 MB) before they are read, but not before its work items give
+// every CTA several; never beyond the second figure.
+constexpr size_t kWideL2 = size_t{64} << 20, kWideMost = size_t{1} << 30;
+constexpr size_t kItemsPerCta = 8;
+// K/V streams (one kv head of a layer and sequence) that CTAs read at one time
+// where a group's rows exceed L2: as many as fit this.
+constexpr size_t kStreamL2 = size_t{32} << 20;
 
 // Prompt attention on the tensor cores: the rows of a group of layers are
-// brought to fp16 (exact, see widen_kernel), then prefill_tc_kernel runs over
-// them as over an fp16 cache.  Its work items are laid out for its persistent
+// brought to fp16 (see widen_kernel), then paged_prompt_kernel runs over them.  Its work items are laid out for its persistent
 // CTAs here: longest first, dealt in turn and back.
 int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all, const std::vector<PagedRun>& runs,
               cudaStream_t st, int* launches) {
     const jx_pkv_desc& D = kv->d;
-    const int hd = static_cast<int>(D.head_dim), G = A.G, TQ = 128 / G, BN = prefill_tc_rows(hd);
+    const int hd = static_cast<int>(D.head_dim), G = A.G, TQ = 2 * kPromptRows / G, BN = kPromptRows;
     const TensorMapEncode enc = tensor_map_encode();
     if (!enc) return pfail(JX_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
     struct Group {
@@ -826,12 +837,17 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
         while (r0 + nr < runs.size() && nr < kMaxRuns) {
             const long long t = (static_cast<long long>(runs[r0 + nr].pos0) + runs[r0 + nr].n + 127) / 128 * 128;
             const long long m = std::max<long long>(rows, t);
-            if (nr > 0 && 2 * row_bytes * m * (nr + 1) > kWideBudget) break;
+            if (nr > 0 && 2 * row_bytes * m * (nr + 1) > kWideMost) break;
             rows = m;
             ++nr;
         }
         const size_t layer_bytes = 2 * row_bytes * rows * nr;
-        const size_t per = std::min<size_t>(kMaxCallLayers, std::max<size_t>(1, kWideBudget / layer_bytes));
+        size_t layer_items = 0;
+        for (size_t i = 0; i < nr; ++i) layer_items += (runs[r0 + i].n + TQ - 1) / TQ * D.n_kv_heads;
+        const size_t enough = kItemsPerCta * std::max(kv->num_sms, 1);
+        const size_t per = std::min<size_t>(
+            std::min<size_t>(kMaxCallLayers, std::max<size_t>(1, kWideMost / layer_bytes)),
+            std::max<size_t>(std::max<size_t>(1, kWideL2 / layer_bytes), (enough + layer_items - 1) / layer_items));
         // layers of one RoPE setting share a launch
         std::vector<PagedLayer> order = all;
         std::stable_sort(order.begin(), order.end(), [](const PagedLayer& x, const PagedLayer& y) { return x.cfg < y.cfg; });
@@ -846,9 +862,11 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
     // the work items of every group, in one list
     std::vector<PrefillTile> items;
     std::vector<int> firsts;
-    std::vector<PrefillTile> tiles, sorted;
+    std::vector<PrefillTile> tiles;
+    std::vector<std::pair<uint32_t, uint32_t>> order;  // (tile, kv head) of each item
     for (Group& g : groups) {
         tiles.clear();
+        order.clear();
         for (size_t i = 0; i < g.nr; ++i) {
             const PagedRun& r = runs[g.r0 + i];
             for (int j = 0; j < r.n; j += TQ)
@@ -875,6 +893,20 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
         g.grid = static_cast<int>(std::min<size_t>(std::max(kv->num_sms, 1), n));
         g.at_items = items.size();
         g.at_first = firsts.size();
+        for (uint32_t i = 0; i < tiles.size(); ++i)
+            for (uint32_t h = 0; h < D.n_kv_heads; ++h) order.emplace_back(i, h);
+        if (2 * row_bytes * g.rows * g.nr * g.layers.size() > 2 * kWideL2) {
+            // more than L2 holds: stream by stream, a batch of streams at a time; the
+            // last rounds longest first again, so that the CTAs end together
+            const size_t batch = std::max<size_t>(1, kStreamL2 / (4 * static_cast<size_t>(g.rows) * hd));
+            auto of = [&](const std::pair<uint32_t, uint32_t>& x) {
+                const PrefillTile& t = tiles[x.first];
+                return ((static_cast<size_t>(t.seq) * g.layers.size() + t.cache_layer) * D.n_kv_heads + x.second) / batch;
+            };
+            std::stable_sort(order.begin(), order.end(), [&](const auto& x, const auto& y) { return of(x) < of(y); });
+            std::stable_sort(order.end() - static_cast<std::ptrdiff_t>(std::min<size_t>(n, 3 * g.grid)), order.end(),
+                             [](const auto& x, const auto& y) { return x.first < y.first; });
+        }
         const size_t P = static_cast<size_t>(g.grid);
         items.resize(items.size() + n);
         // CTA c runs the items at its place in each round of P, every other round reversed
@@ -885,8 +917,8 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
                 const size_t i = round * P + (round % 2 ? P - 1 - c : c);
                 if (round * P >= n) break;
                 if (i >= n) continue;
-                items[at] = tiles[i / D.n_kv_heads];
-                items[at++].kvh = static_cast<int>(i % D.n_kv_heads);
+                items[at] = tiles[order[i].first];
+                items[at++].kvh = static_cast<int>(order[i].second);
             }
         }
         firsts.push_back(static_cast<int>(at - g.at_items));
@@ -922,12 +954,13 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
         w.n_layers = static_cast<int>(nl);
         w.n_runs = static_cast<int>(g.nr);
         w.window = A.window;
+        w.rows = static_cast<int>(g.rows);
         std::copy(g.layers.begin(), g.layers.end(), w.layers);
         int chunks = 0;
         for (size_t i = 0; i < g.nr; ++i) {
             w.runs[i] = runs[g.r0 + i];
             w.runs[i].off = chunks;
-            chunks += (w.runs[i].pos0 + w.runs[i].n + kWidenRows - 1) / kWidenRows;
+            chunks += (w.runs[i].pos0 + w.runs[i].n + kPromptRows + kWidenRows - 1) / kWidenRows;
         }
         const dim3 grid(chunks, static_cast<unsigned>(nl * A.n_kv));
         dispatch(D, [&](auto h, auto dt) { widen_kernel<h.value, dt.value><<<grid, 256, 0, st>>>(w); });
@@ -942,26 +975,26 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
                 return pfail(JX_ERR_CUDA, "cuTensorMapEncodeTiled failed");
-        PrefillArgs p{};
+        PromptArgs p{};
         p.tiles = reinterpret_cast<const PrefillTile*>(u->d) + g.at_items;
         p.cta_first = reinterpret_cast<const int*>(static_cast<const char*>(u->d) + first_at) + g.at_first;
-        p.n_items = static_cast<int>(g.items);
-        p.neox = A.neox;
-        p.q_vec = A.q_vec;
         p.q = A.q;
         p.out = A.out;
         p.q_stride = A.q_stride;
         p.rope = A.rope[g.layers[0].cfg];
-        p.scale = A.scale;
-        p.softcap = A.softcap;
-        p.inv_softcap = A.softcap > 0.0f ? 1.0f / A.softcap : 0.0f;
-        p.err = A.err;
-        p.dbg = A.dbg;
-        p.wait_limit = A.wait_limit;
         p.head_scale = kv->d_head_scale;
         p.scale_layers = static_cast<int>(nl);
         p.scale_heads = A.n_kv;
-        const cudaError_t e = prefill_tc_launch(p, &maps[0], &maps[1], hd, DT_F16T, G, g.grid, st);
+        p.neox = A.neox;
+        p.q_vec = A.q_vec;
+        p.scale = A.scale;
+        p.softcap = A.softcap;
+        p.cap_in = A.cap_in;
+        p.cap_out = A.cap_out;
+        p.err = A.err;
+        p.dbg = A.dbg;
+        p.wait_limit = A.wait_limit;
+        const cudaError_t e = paged_prompt_launch(p, &maps[0], &maps[1], hd, G, g.grid, st);
         if (e != cudaSuccess) return pfail(JX_ERR_CUDA, "prompt launch failed: %s", cudaGetErrorString(e));
         *launches += 2;
     }
@@ -1105,7 +1138,7 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
         if (int rc = append_rows(kv, A, part, runs, st, &launches)) return rc;
         // then attention: on the tensor cores, or (few tokens, or a shape that kernel
         // does not take) for blocks of as many tokens as fill the step kernel's columns
-        if (prefill_tc_supported(static_cast<int>(D.head_dim), DT_F16T, static_cast<int>(G)) && out_vec &&
+        if (paged_prompt_supported(static_cast<int>(D.head_dim), static_cast<int>(G)) && out_vec && a->scale > 0.0f &&
             a->n_seqs >= kPromptTokens * runs.size()) {
             if (int rc = prompt_tc(kv, A, all, runs, st, &launches)) return rc;
             kv->last_launches = launches;

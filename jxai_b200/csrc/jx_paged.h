@@ -15,6 +15,7 @@
 // number 1024 + u); e4m3 codes as they are.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -166,6 +167,34 @@ __device__ __forceinline__ float rope_plain(const float* x, int d, int half, con
                  : __fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
 }
 
+// Four consecutive dims of a rotated head.  vec: 16-byte loads are possible and
+// a group of four does not cross the end of the rotated part.
+__device__ __forceinline__ float4 rope4(const float* x, int d, int half, const float2* cs, bool neox, bool vec) {
+    if (!vec)
+        return make_float4(rope_plain(x, d, half, cs, neox), rope_plain(x, d + 1, half, cs, neox),
+                           rope_plain(x, d + 2, half, cs, neox), rope_plain(x, d + 3, half, cs, neox));
+    const float4 v = *reinterpret_cast<const float4*>(x + d);
+    if (d >= 2 * half) return v;
+    if (neox) {
+        const bool first = d < half;
+        const int j = first ? d : d - half;
+        const float4 w = *reinterpret_cast<const float4*>(x + (first ? d + half : d - half));
+        const float4 c0 = *reinterpret_cast<const float4*>(cs + j);
+        const float4 c1 = *reinterpret_cast<const float4*>(cs + j + 2);
+        auto rot = [&](float mine, float other, float c, float s) {
+            return first ? __fsub_rn(__fmul_rn(mine, c), __fmul_rn(other, s))
+                         : __fadd_rn(__fmul_rn(other, s), __fmul_rn(mine, c));
+        };
+        return make_float4(rot(v.x, w.x, c0.x, c0.y), rot(v.y, w.y, c0.z, c0.w), rot(v.z, w.z, c1.x, c1.y),
+                           rot(v.w, w.w, c1.z, c1.w));
+    }
+    const float4 c = *reinterpret_cast<const float4*>(cs + d / 2);
+    return make_float4(__fsub_rn(__fmul_rn(v.x, c.x), __fmul_rn(v.y, c.y)),
+                       __fadd_rn(__fmul_rn(v.x, c.y), __fmul_rn(v.y, c.x)),
+                       __fsub_rn(__fmul_rn(v.z, c.z), __fmul_rn(v.w, c.w)),
+                       __fadd_rn(__fmul_rn(v.z, c.w), __fmul_rn(v.w, c.z)));
+}
+
 // Four values to codes (x * inv) and back; 16 likewise.
 template <int DT>
 __device__ __forceinline__ uint32_t pack4(float x, float y, float z, float w, float inv) {
@@ -189,6 +218,30 @@ __device__ __forceinline__ long long owner_of(long long x, long long total, long
 }
 
 #endif  // __CUDACC__
+
+// The prompt kernel (jx_paged_prompt.cu): items of up to 2 * 128/G tokens over
+// fp16 rows (tensor maps of 128-row boxes), whose K and V of a head are to be
+// multiplied by head_scale [seq][layer][kv head] (K, V).
+struct PrefillTile;
+struct PromptArgs {
+    const PrefillTile* tiles;
+    const int* cta_first;   // CTA b runs tiles [cta_first[b], cta_first[b + 1])
+    const float* q;
+    float* out;
+    long long q_stride;
+    const float2* rope;     // rows of HD/2 (cos, sin) pairs, by position
+    const float2* head_scale;
+    int scale_layers, scale_heads;
+    int neox, q_vec;
+    float scale, softcap, cap_in, cap_out;
+    int* err;
+    int* dbg;
+    long long wait_limit;
+};
+constexpr int kPromptRows = 128;  // rows of a K or V tile, and of a query tile
+bool paged_prompt_supported(int hd, int G);
+cudaError_t paged_prompt_launch(const PromptArgs& a, const CUtensorMap* tmK, const CUtensorMap* tmV, int hd, int G,
+                                int grid, cudaStream_t st);
 
 // The step kernel (jx_paged_step.cuh) for `cols` columns: query heads of a kv
 // head, times the tokens of a block.

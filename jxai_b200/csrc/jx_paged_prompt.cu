@@ -1,0 +1,440 @@
+// jx_paged_prompt.cu -- causal prompt attention on the tensor cores (tcgen05) for
+// the paged 8-bit cache, whose rows were brought to fp16 (widen_kernel).
+//
+//  * Work item: 2 * 128/G consecutive tokens of a sequence, one layer, one kv
+//    head: two tiles X = 0, 1 of 128 query rows (row r = token r/G, head r%G)
+//    that read the same K and V tiles.
+//  * What bounds it: per 128 x 128 scores, 2 * 128*128*HD*2 multiply-adds for each
+//    of S and P.V (q and p in two fp16 parts; 512 cycles each at head_dim 128)
+//    against 16384 exponentials at 16 per cycle (1024 cycles) and about 6
+//    instructions per score on four schedulers.  The three overlap only if there
+//    is always a tile for each, so two tiles take turns: while one's softmax runs,
+//    the tensor cores work on the other.
+//  * Warp 0 streams K and V tiles (128 rows, TMA, 128-byte swizzle) through a
+//    ring.  Warp 1 issues the MMAs of both tiles from one thread.  Warps 2-5 and
+//    6-9 are the softmax of tile 0 and 1: one thread per row, no exchange between
+//    threads.
+//  * TMEM (512 columns): S of both tiles, 128 each, and O of both.  The weights
+//    replace the scores they came from -- as fp16, both parts take exactly S's
+//    columns -- and are the A operand of P.V from there; no weight passes through
+//    shared memory, which Q (two parts, both tiles) and the ring fill.
+//  * A tile's next S overwrites its P: it is issued once that P.V has completed,
+//    while the other tile's work is in the queue.
+//  * The running maximum moves only when a tile exceeds it by 2^8 (O is then
+//    rescaled in TMEM, its P.V known complete from the S that follows it); a
+//    weight of 1 is 2^7 in fp16, so weights reach 2^15 and the fp16 floor lies
+//    2^-32 below 1.
+//  * Every mbarrier wait is bounded; one that runs out raises the abort flag and
+//    the device error word, and every role finishes its control flow.
+#include "jx_internal.h"
+#include "jx_paged.h"
+#include "jx_tcgen05.cuh"
+
+namespace jx {
+namespace {
+
+constexpr int kThreads = 32 * 10;
+constexpr float kLog2 = 1.4426950408889634f;
+
+template <int HD>
+struct PromptCfg {
+    static constexpr int BN = 128;
+    static constexpr int NSLAB = HD / 64;        // 128-byte slabs of a head row
+    static constexpr int SLAB = 128 * 128;       // 128 rows of one slab
+    static constexpr int TILE = SLAB * NSLAB;    // a K or V tile, or one part of a Q tile
+    static constexpr int NS = HD == 64 ? 8 : 3;  // ring stages (K0, V0, K1, ...)
+    static constexpr int OFF_Q = 0;              // [tile][part]
+    static constexpr int OFF_KV = 4 * TILE;
+    static constexpr int OFF_BAR = OFF_KV + NS * TILE;
+    static constexpr int B_KVF = 0, B_KVE = NS, B_QF = 2 * NS, B_SF = B_QF + 2, B_PF = B_SF + 2, B_PV = B_PF + 2,
+                         B_OE = B_PV + 2, B_DONE = B_OE + 2, NBARS = B_DONE + 1;
+    static constexpr int OFF_MISC = OFF_BAR + NBARS * 8;
+    static constexpr int SMEM = OFF_MISC + 16 + 1024;  // + alignment slack
+    static constexpr int COL_S = 0, COL_O = 256;       // tile X: + 128 X
+    static_assert(SMEM <= 227 * 1024, "shared memory budget");
+};
+
+template <int HD, int G>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                        const PromptArgs a) {
+    using C = PromptCfg<HD>;
+    constexpr int BN = C::BN, TQ = 128 / G;
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t sbase = (raw + 1023u) & ~1023u;  // 128-byte-swizzled tiles: 1024-byte aligned
+    unsigned char* base = smem_raw + (sbase - raw);
+    const uint32_t bars = sbase + C::OFF_BAR;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + C::OFF_MISC);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(base + C::OFF_MISC + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int it_begin = a.cta_first[blockIdx.x], it_end = a.cta_first[blockIdx.x + 1];
+#define BAR(i) (bars + 8u * static_cast<uint32_t>(i))
+#define WAIT(i, par, site, idx) \
+    mbar_wait_bounded(BAR(i), (par), abort_flag, a.err, a.dbg, (site), (idx), true, a.wait_limit)
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::NS; ++s) {
+            mbar_init(BAR(C::B_KVF + s), 1);
+            mbar_init(BAR(C::B_KVE + s), 1);
+        }
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(BAR(C::B_QF + x), 4);
+            mbar_init(BAR(C::B_SF + x), 1);
+            mbar_init(BAR(C::B_PF + x), 4);
+            mbar_init(BAR(C::B_PV + x), 1);
+            mbar_init(BAR(C::B_OE + x), 4);
+        }
+        mbar_init(BAR(C::B_DONE), 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_slot), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    // K/V tiles that tile x of an item reads (it has no later rows to attend)
+    auto tiles_of = [](const PrefillTile& t, int x) {
+        const int tok = x == 0 ? min(t.ntok, TQ) : t.ntok - TQ;
+        return tok <= 0 ? 0 : (t.tok_row0 + x * TQ + tok - t.kv_lo + BN - 1) / BN;
+    };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        if (lane == 0) {
+            prefetch_tensormap(&tmK);
+            prefetch_tensormap(&tmV);
+        }
+        int n = 0, issued = 0;  // tiles of the ring so far
+        for (int it = it_begin; it < it_end; ++it) {
+            const PrefillTile tl = a.tiles[it];
+            const int nt = max(tiles_of(tl, 0), tiles_of(tl, 1));
+            for (int t = 0; t < 2 * nt; ++t, ++n) {
+                const int st = n % C::NS;
+                if (n >= C::NS) WAIT(C::B_KVE + st, ((n / C::NS) & 1) ^ 1u, 50, n);
+                if (__shfl_sync(0xffffffffu, *abort_flag, 0)) continue;
+                issued = n + 1;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(BAR(C::B_KVF + st), C::TILE);
+#pragma unroll
+                    for (int b = 0; b < C::NSLAB; ++b)
+                        tma_load_4d(sbase + C::OFF_KV + st * C::TILE + b * C::SLAB, (t & 1) ? &tmV : &tmK,
+                                    BAR(C::B_KVF + st), tl.kvh * HD + b * 64, tl.kv_lo + t / 2 * BN, tl.cache_layer, tl.seq);
+                }
+                __syncwarp();
+            }
+        }
+        // every issued tile lands before the CTA exits
+        for (int k = max(0, issued - C::NS); k < issued; ++k)
+            mbar_wait_bounded(BAR(C::B_KVF + k % C::NS), (k / C::NS) & 1, abort_flag, a.err, a.dbg, 51, k, false,
+                              kDrainLimitCycles);
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        constexpr uint32_t ID_S = idesc_f16(DT_F16T, 128, BN, false);
+        constexpr uint32_t ID_PV = idesc_f16(DT_F16T, 128, HD, true);
+        int n0 = 0, itc = 0;          // first ring tile of the item, items so far
+        int pf[2] = {0, 0};           // weights taken, and P.V issued, of each tile
+        for (int it = it_begin; it < it_end; ++it, ++itc) {
+            const PrefillTile tl = a.tiles[it];
+            const int cnt[2] = {tiles_of(tl, 0), tiles_of(tl, 1)};
+            const int nt = max(cnt[0], cnt[1]);
+            auto kv_at = [&](int n) { return sbase + C::OFF_KV + (n % C::NS) * C::TILE; };
+            auto issue_s = [&](int x, int t) {  // S = Q_hi.K^T + Q_lo.K^T
+                const int n = n0 + 2 * t;
+                WAIT(C::B_KVF + n % C::NS, (n / C::NS) & 1, 52, n);
+                tc_fence_after();
+                if (lane == 0) {
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int ks = 0; ks < HD / 16; ++ks) {
+                            const uint32_t off = (ks / 4) * C::SLAB + (ks % 4) * 32;
+                            tc_mma(tmem + C::COL_S + x * 128,
+                                   sw128_desc(sbase + C::OFF_Q + (2 * x + part) * C::TILE + off, 16, 1024),
+                                   sw128_desc(kv_at(n) + off, 16, 1024), ID_S, (part | ks) != 0 ? 1u : 0u);
+                        }
+                    tc_commit(BAR(C::B_SF + x));
+                }
+                __syncwarp();
+            };
+            auto release = [&](int n) {  // a ring tile, once all MMAs issued so far are done
+                if (lane == 0) tc_commit(BAR(C::B_KVE + n % C::NS));
+                __syncwarp();
+            };
+            for (int x = 0; x < 2; ++x) {
+                WAIT(C::B_QF + x, itc & 1, 53, itc);
+                if (cnt[x] == 0) continue;
+                // S takes the place of the item before's last P
+                if (pf[x] > 0) WAIT(C::B_PV + x, (pf[x] - 1) & 1, 61, itc);
+                issue_s(x, 0);
+            }
+            if (nt > 0) release(n0);
+            for (int t = 0; t < nt; ++t) {
+                for (int x = 0; x < 2; ++x) {
+                    if (t < cnt[x]) {
+                        WAIT(C::B_PF + x, pf[x] & 1, 54, t);
+                        // the first P.V overwrites O: the item before has read it
+                        if (t == 0 && itc > 0) WAIT(C::B_OE + x, (itc - 1) & 1, 55, itc);
+                        const int n = n0 + 2 * t + 1;
+                        WAIT(C::B_KVF + n % C::NS, (n / C::NS) & 1, 56, n);
+                        tc_fence_after();
+                        if (lane == 0) {
+#pragma unroll
+                            for (int part = 0; part < 2; ++part)
+#pragma unroll
+                                for (int kb = 0; kb < BN / 16; ++kb)
+                                    tc_mma_ts(tmem + C::COL_O + x * 128, tmem + C::COL_S + x * 128 + part * 64 + kb * 8,
+                                              sw128_desc(kv_at(n) + kb * 16 * 128, C::SLAB, 1024), ID_PV,
+                                              (t | part | kb) != 0 ? 1u : 0u);
+                            tc_commit(BAR(C::B_PV + x));
+                        }
+                        __syncwarp();
+                        if (t + 1 < cnt[x]) {
+                            WAIT(C::B_PV + x, pf[x] & 1, 57, t);  // S takes the place of P
+                            issue_s(x, t + 1);
+                        }
+                        ++pf[x];
+                    }
+                }
+                release(n0 + 2 * t + 1);
+                if (t + 1 < nt) release(n0 + 2 * t + 2);
+            }
+            n0 += 2 * nt;
+        }
+        // every MMA completes before TMEM is freed
+        if (lane == 0) tc_commit(BAR(C::B_DONE));
+        __syncwarp();
+        mbar_wait_bounded(BAR(C::B_DONE), 0u, abort_flag, a.err, a.dbg, 58, 0, false, kDrainLimitCycles);
+    } else {
+        // ------------------------------------------------------------ softmax, one thread per row
+        const int x = (warp - 2) >> 2;
+        const int q4 = warp & 3;
+        const int r = q4 * 32 + lane;  // row of the tile = TMEM lane
+        const int j = r / G, h = r % G;
+        const uint32_t lane_addr = static_cast<uint32_t>(q4 * 32) << 16;
+        const uint32_t ts = tmem + lane_addr + C::COL_S + x * 128;
+        const uint32_t to = tmem + lane_addr + C::COL_O + x * 128;
+        const bool capped = a.softcap > 0.0f;
+        // This row of item tl's Q tile: rotated, brought into [2^14, 2^15), split into
+        // two fp16 parts.  Returns the power of two that undoes it.
+        auto stage_q = [&](const PrefillTile& tl) -> float {
+            const int tok = x * TQ + j;
+            float qr[HD];
+            if (tok < tl.ntok) {
+                const long long io = static_cast<long long>(tl.io0) + static_cast<long long>(tok) * tl.io_step;
+                const float* src = a.q + io * a.q_stride + static_cast<long long>(tl.kvh * G + h) * HD;
+                const float2* cs = a.rope + static_cast<long long>(tl.rope_row0 + tok) * (HD / 2);
+                const bool vec = a.q_vec && tl.rope_half % 4 == 0;
+#pragma unroll
+                for (int d = 0; d < HD; d += 4) {
+                    const float4 v = rope4(src, d, tl.rope_half, cs, a.neox != 0, vec);
+                    qr[d] = v.x;
+                    qr[d + 1] = v.y;
+                    qr[d + 2] = v.z;
+                    qr[d + 3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int d = 0; d < HD; ++d) qr[d] = 0.0f;
+            }
+            float mx = 0.0f;
+#pragma unroll
+            for (int d = 0; d < HD; ++d) mx = fmaxf(mx, fabsf(qr[d]));
+            const int e = static_cast<int>((__float_as_uint(mx) >> 23) & 0xFFu) - 127;
+            const int sh = min(60, max(-60, 14 - e));
+            const float up = exp2_int(sh);
+            unsigned char* q = base + C::OFF_Q + 2 * x * C::TILE;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    split_pair<DT_F16T>(qr[8 * c + 2 * i] * up, qr[8 * c + 2 * i + 1] * up, hi[i], lo[i]);
+                const int off = (c / 8) * C::SLAB + r * 128 + (((c % 8) ^ (r & 7)) * 16);
+                *reinterpret_cast<uint4*>(q + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(q + C::TILE + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(C::B_QF + x));
+            return exp2_int(-sh);
+        };
+        int g = 0;  // tiles of S so far
+        float unscale = it_begin < it_end ? stage_q(a.tiles[it_begin]) : 1.0f;
+        for (int it = it_begin; it < it_end; ++it) {
+            const PrefillTile tl = a.tiles[it];
+            const int nt = tiles_of(tl, x);
+            const int tok = x * TQ + j;
+            const bool live = tok < tl.ntok;
+            const int row0 = tl.tok_row0 + x * TQ, row_n = row0 + min(TQ, tl.ntok - x * TQ) - 1;  // of the tile's tokens
+            const int hi_r = live ? row0 + j : -1;
+            const int lo_r = live && tl.window > 0 ? max(0, hi_r - tl.window + 1) : 0;
+            const int lo_all = tl.window > 0 ? max(0, row_n - tl.window + 1) : 0;
+            const float2 hs = __ldg(a.head_scale + (static_cast<long long>(tl.seq) * a.scale_layers + tl.cache_layer) *
+                                                       a.scale_heads + tl.kvh);
+            const float mul = a.scale * unscale * hs.x;  // raw S -> score
+            const float mul2 = mul * kLog2;
+            float m = -INFINITY, l = 0.0f;  // the maximum in units of log2
+            for (int t = 0; t < nt; ++t, ++g) {
+                WAIT(C::B_SF + x, g & 1, 59, g);
+                __syncwarp();
+                tc_fence_after();
+                const int c0 = tl.kv_lo + t * BN;
+                const bool masked = c0 + BN - 1 > row0 || c0 < lo_all;
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < BN; c += 32) {
+                    uint32_t s[32];
+                    tmem_ld32(ts + c, s);
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int col = c0 + c + i;
+                            mx[i & 3] = fmaxf(mx[i & 3], col >= lo_r && col <= hi_r ? __uint_as_float(s[i]) : -INFINITY);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2)
+                            mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                    }
+                }
+                float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                // the score's soft cap is monotone: the capped maximum is the maximum's cap
+                mt = capped ? (mt == -INFINITY ? mt : a.cap_out * tanhf(mt * mul2 * a.cap_in)) : mt * mul2;
+                const bool move = mt > m + 8.0f || (m == -INFINITY && mt > -INFINITY);
+                if (__any_sync(0xffffffffu, move)) {
+                    const float f = !move ? 1.0f : (m == -INFINITY ? 0.0f : ex2_approx(m - mt));
+                    if (move) {
+                        l *= f;
+                        m = mt;
+                    }
+                    // this S was issued after the P.V before it had completed
+                    if (t > 0) {
+#pragma unroll
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(to + c, o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st32(to + c, o);
+                        }
+                    }
+                }
+                const float add = m == -INFINITY ? 0.0f : 7.0f - m;
+                float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t lw[64];  // second parts: their columns hold scores until all are read
+#pragma unroll
+                for (int c = 0; c < BN; c += 32) {
+                    uint32_t s[32], hw[16];
+                    tmem_ld32(ts + c, s);
+                    if (masked || capped) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            float v = __uint_as_float(s[i]) * mul2;
+                            if (capped) v = a.cap_out * tanhf(v * a.cap_in);
+                            const int col = c0 + c + i;
+                            s[i] = __float_as_uint(col >= lo_r && col <= hi_r ? v : -INFINITY);
+                        }
+                    }
+                    const float k = masked || capped ? 1.0f : mul2;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        float x0 = add, x1 = add;
+                        fma_x2(x0, x1, __uint_as_float(s[i]), __uint_as_float(s[i + 1]), k, k);
+                        const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                        add_x2(ls[i & 2], ls[(i & 2) + 1], p0, p1);
+                        split_pair<DT_F16T>(p0, p1, hw[i / 2], lw[c / 2 + i / 2]);
+                    }
+                    tmem_st16(ts + c / 2, hw);  // over columns that have been read
+                }
+#pragma unroll
+                for (int c = 0; c < 64; c += 16) tmem_st16(ts + 64 + c, reinterpret_cast<const uint32_t(&)[16]>(lw[c]));
+                l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(BAR(C::B_PF + x));
+            }
+            // the next item's Q while the last P.V runs: every S of this one is done
+            const float next = it + 1 < it_end ? stage_q(a.tiles[it + 1]) : 1.0f;
+            if (nt > 0) {
+                WAIT(C::B_PV + x, (g - 1) & 1, 60, g);
+                __syncwarp();
+                tc_fence_after();
+                const long long io = static_cast<long long>(tl.io0) + static_cast<long long>(tok) * tl.io_step;
+                float* dst = a.out + io * a.q_stride + static_cast<long long>(tl.kvh * G + h) * HD;
+                const float inv = l > 0.0f ? hs.y / l : 0.0f;
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(to + c, o);
+                    if (live) {
+#pragma unroll
+                        for (int d = 0; d < 32; d += 4)
+                            *reinterpret_cast<float4*>(dst + c + d) =
+                                make_float4(__uint_as_float(o[d]) * inv, __uint_as_float(o[d + 1]) * inv,
+                                            __uint_as_float(o[d + 2]) * inv, __uint_as_float(o[d + 3]) * inv);
+                    }
+                    __syncwarp();  // converged for the next .sync.aligned load
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(BAR(C::B_OE + x));  // O may be overwritten
+            unscale = next;
+        }
+    }
+#undef WAIT
+#undef BAR
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int HD, int G>
+cudaError_t launch_one(const PromptArgs& a, const CUtensorMap* tk, const CUtensorMap* tv, int grid, cudaStream_t st) {
+    constexpr int smem = PromptCfg<HD>::SMEM;
+    static bool set[64] = {false};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !set[dev]) {
+        e = cudaFuncSetAttribute(paged_prompt_kernel<HD, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) set[dev] = true;
+    }
+    paged_prompt_kernel<HD, G><<<grid, kThreads, smem, st>>>(*tk, *tv, a);
+    return cudaGetLastError();
+}
+
+template <int HD>
+cudaError_t launch_g(const PromptArgs& a, const CUtensorMap* tk, const CUtensorMap* tv, int G, int grid, cudaStream_t st) {
+    switch (G) {
+        case 1: return launch_one<HD, 1>(a, tk, tv, grid, st);
+        case 2: return launch_one<HD, 2>(a, tk, tv, grid, st);
+        case 4: return launch_one<HD, 4>(a, tk, tv, grid, st);
+        case 8: return launch_one<HD, 8>(a, tk, tv, grid, st);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace
+
+bool paged_prompt_supported(int hd, int G) {
+    return (hd == 64 || hd == 128) && (G == 1 || G == 2 || G == 4 || G == 8);
+}
+
+cudaError_t paged_prompt_launch(const PromptArgs& a, const CUtensorMap* tmK, const CUtensorMap* tmV, int hd, int G,
+                                int grid, cudaStream_t st) {
+    if (!paged_prompt_supported(hd, G)) return cudaErrorInvalidValue;
+    return hd == 64 ? launch_g<64>(a, tmK, tmV, G, grid, st) : launch_g<128>(a, tmK, tmV, G, grid, st);
+}
+
+}  // namespace jx

@@ -169,34 +169,6 @@ __device__ __forceinline__ void codes_split(uint32_t w, uint32_t& ev, uint32_t& 
     }
 }
 
-// Four consecutive dims of a rotated head.  vec: 16-byte loads are possible and
-// a group of four does not cross the end of the rotated part.
-__device__ __forceinline__ float4 rope4(const float* x, int d, int half, const float2* cs, bool neox, bool vec) {
-    if (!vec)
-        return make_float4(rope_plain(x, d, half, cs, neox), rope_plain(x, d + 1, half, cs, neox),
-                           rope_plain(x, d + 2, half, cs, neox), rope_plain(x, d + 3, half, cs, neox));
-    const float4 v = *reinterpret_cast<const float4*>(x + d);
-    if (d >= 2 * half) return v;
-    if (neox) {
-        const bool first = d < half;
-        const int j = first ? d : d - half;
-        const float4 w = *reinterpret_cast<const float4*>(x + (first ? d + half : d - half));
-        const float4 c0 = *reinterpret_cast<const float4*>(cs + j);
-        const float4 c1 = *reinterpret_cast<const float4*>(cs + j + 2);
-        auto rot = [&](float mine, float other, float c, float s) {
-            return first ? __fsub_rn(__fmul_rn(mine, c), __fmul_rn(other, s))
-                         : __fadd_rn(__fmul_rn(other, s), __fmul_rn(mine, c));
-        };
-        return make_float4(rot(v.x, w.x, c0.x, c0.y), rot(v.y, w.y, c0.z, c0.w), rot(v.z, w.z, c1.x, c1.y),
-                           rot(v.w, w.w, c1.z, c1.w));
-    }
-    const float4 c = *reinterpret_cast<const float4*>(cs + d / 2);
-    return make_float4(__fsub_rn(__fmul_rn(v.x, c.x), __fmul_rn(v.y, c.y)),
-                       __fadd_rn(__fmul_rn(v.x, c.y), __fmul_rn(v.y, c.x)),
-                       __fsub_rn(__fmul_rn(v.z, c.z), __fmul_rn(v.w, c.w)),
-                       __fadd_rn(__fmul_rn(v.z, c.w), __fmul_rn(v.w, c.z)));
-}
-
 template <int HD, int GP, int DT>
 struct StepWarp {
     static constexpr int NBC = (2 * GP + 7) / 8;  // column blocks: (part, head) pairs

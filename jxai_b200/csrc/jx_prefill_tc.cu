@@ -36,6 +36,7 @@
 //    control flow, waits for its copies / MMAs in flight and frees TMEM.
 #include "jx_device.cuh"
 #include "jx_internal.h"
+#include "jx_tcgen05.cuh"
 
 namespace jx {
 namespace {
@@ -45,123 +46,6 @@ constexpr int kSoftmaxWarps = 8;                       // warps 2-9
 // + TMA warp, MMA warp.  Ten warps put three on two of the SM's four
 // sub-partitions (16K registers each): at most 170 registers per thread.
 constexpr int kPfThreads = 32 * (2 + kSoftmaxWarps);
-
-// Loads 32 consecutive 32-bit TMEM columns of this thread's lane and waits
-// for them (one asm statement: the registers are valid when it ends).
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-
-// Loads 64 consecutive 32-bit TMEM columns of this thread's lane and waits
-// for them (one asm statement: the registers are valid when it ends).
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-        : "r"(taddr)
-        : "memory");
-}
-
-// Stores 32 consecutive 32-bit TMEM columns of this thread's lane and waits
-// until the stores are done (before a thread synchronisation hands the
-// columns to the tensor cores).
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n\t"
-        "tcgen05.wait::st.sync.aligned;"
-        :
-        : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-
-// As tmem_st32, 16 columns.
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n\t"
-        "tcgen05.wait::st.sync.aligned;"
-        :
-        : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-
-__device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem),
-                 "r"(ncols)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish() {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
-                 : "memory");
-}
-// Orders tcgen05 operations before / after a thread synchronisation (an
-// mbarrier arrive / wait or a CTA barrier).
-__device__ __forceinline__ void tc_fence_before() {
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-// The mbarrier completes once every tcgen05 operation this thread issued
-// before has completed.
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     bar)
-                 : "memory");
-}
-// D[tmem] (+)= A[smem] . B[smem]^T, one CTA, 16-bit operands, fp32 accumulator.
-__device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                       uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u),
-        "r"(0u), "r"(0u)
-        : "memory");
-}
-
-// D[tmem] (+)= A[tmem] . B[smem]^T: A read from tensor memory (lane = row,
-// each 32-bit column two consecutive 16-bit elements, the even one in the
-// low half), one CTA, fp32 accumulator.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                          uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u),
-        "r"(0u), "r"(0u)
-        : "memory");
-}
-
-// Shared-memory matrix descriptor of a 128-byte-swizzled operand tile (the
-// layout TMA's SWIZZLE_128B writes: 128-byte rows, 16-byte chunk c of row r at
-// chunk c ^ (r % 8), tile base 1024-byte aligned).  lbo / sbo in bytes:
-// K-major operands: lbo unused (16), sbo = 1024 (8 rows of 128 bytes);
-// MN-major operands: lbo = distance between 64-element column blocks, sbo =
-// 1024 (8 K-rows).  Bits 46-47 = 1 (tcgen05 descriptor), 61-63 = 2 (128B).
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-    return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) |
-           (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
-           (static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
-}
-
-// Instruction descriptor of kind::f16 with fp32 accumulation: A and B both
-// bf16 (DT_BF16) or both fp16, A K-major, B K-major or MN-major, M x N.
-__host__ __device__ constexpr uint32_t idesc_f16(int dt, int M, int N, bool b_mn) {
-    return (1u << 4) | ((dt == DT_BF16 ? 1u : 0u) << 7) | ((dt == DT_BF16 ? 1u : 0u) << 10) |
-           ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
-           (static_cast<uint32_t>(M >> 4) << 24);
-}
 
 __device__ __forceinline__ float f4_at(const float4& v, int i) {
     return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w));
@@ -580,12 +464,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
             const int n = tl.n_tiles;
             // unscale is a power of two: (S * unscale) * scale rounds once, as
             // the reference's dot * scale does
-            // (a cache held in 8 bits gives K and V of a head times powers of two)
-            const float2 hs = a.head_scale
-                                  ? __ldg(a.head_scale + (static_cast<long long>(tl.seq) * a.scale_layers +
-                                                          tl.cache_layer) * a.scale_heads + tl.kvh)
-                                  : make_float2(1.0f, 1.0f);
-            const float sc_mul = a.scale * unscale * hs.x;
+            const float sc_mul = a.scale * unscale;
             const bool capped = a.softcap > 0.0f;
             // columns every live row of the item attends: [lo_all, hi_all]
             const int hi_all = tl.tok_row0;  // the first token's row
@@ -726,7 +605,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
                 tc_fence_after();
                 float* dst = a.out + io * a.q_stride + static_cast<long long>(tl.kvh * G + h) * HD +
                              hf * HW;
-                const float inv = lt > 0.0f ? hs.y / lt : 0.0f;
+                const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
 #pragma unroll
                 for (int c = 0; c < HW; c += 32) {
                     uint32_t t32[32];
