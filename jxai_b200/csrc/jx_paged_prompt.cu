@@ -11,9 +11,9 @@
 //    is always a tile for each, so two tiles take turns: while one's softmax runs,
 //    the tensor cores work on the other.
 //  * Warp 0 streams K and V tiles (128 rows, TMA, 128-byte swizzle) through a
-//    ring.  Warp 1 issues the MMAs of both tiles from one thread.  Warps 2-5 and
-//    6-9 are the softmax of tile 0 and 1: one thread per row, no exchange between
-//    threads.
+//    ring.  Warp 1 issues the MMAs of both tiles from one thread.  Warps 2-9 and
+//    10-17 are the softmax of tile 0 and 1: two threads per row, each with half of
+//    its scores, weights and dims; they exchange the row's maximum per tile.
 //  * TMEM (512 columns): S of both tiles, 128 each, and O of both.  The weights
 //    replace the scores they came from -- as fp16, both parts take exactly S's
 //    columns -- and are the A operand of P.V from there; no weight passes through
@@ -33,7 +33,7 @@
 namespace jx {
 namespace {
 
-constexpr int kThreads = 32 * 10;
+constexpr int kThreads = 32 * 18;
 constexpr float kLog2 = 1.4426950408889634f;
 
 template <int HD>
@@ -49,7 +49,8 @@ struct PromptCfg {
     static constexpr int B_KVF = 0, B_KVE = NS, B_QF = 2 * NS, B_SF = B_QF + 2, B_PF = B_SF + 2, B_PV = B_PF + 2,
                          B_OE = B_PV + 2, B_DONE = B_OE + 2, NBARS = B_DONE + 1;
     static constexpr int OFF_MISC = OFF_BAR + NBARS * 8;
-    static constexpr int SMEM = OFF_MISC + 16 + 1024;  // + alignment slack
+    static constexpr int OFF_XCH = OFF_MISC + 16;      // [tile][half][128] floats: row exchanges
+    static constexpr int SMEM = OFF_XCH + 2 * 2 * 128 * 4;
     static constexpr int COL_S = 0, COL_O = 256;       // tile X: + 128 X
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
@@ -60,10 +61,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const PromptArgs a) {
     using C = PromptCfg<HD>;
     constexpr int BN = C::BN, TQ = 128 / G;
-    extern __shared__ unsigned char smem_raw[];
-    const uint32_t raw = smem_u32(smem_raw);
-    const uint32_t sbase = (raw + 1023u) & ~1023u;  // 128-byte-swizzled tiles: 1024-byte aligned
-    unsigned char* base = smem_raw + (sbase - raw);
+    // 128-byte-swizzled tiles: 1024-byte aligned (nothing else is in shared memory)
+    extern __shared__ __align__(1024) unsigned char base[];
+    const uint32_t sbase = smem_u32(base);
+    if (sbase & 1023u) {  // every thread takes this branch together
+        if (threadIdx.x == 0) atomicExch(a.err, kDevErrCheck);
+        return;
+    }
     const uint32_t bars = sbase + C::OFF_BAR;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + C::OFF_MISC);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(base + C::OFF_MISC + 4);
@@ -79,11 +83,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(BAR(C::B_KVE + s), 1);
         }
         for (int x = 0; x < 2; ++x) {
-            mbar_init(BAR(C::B_QF + x), 4);
+            mbar_init(BAR(C::B_QF + x), 8);
             mbar_init(BAR(C::B_SF + x), 1);
-            mbar_init(BAR(C::B_PF + x), 4);
+            mbar_init(BAR(C::B_PF + x), 8);
             mbar_init(BAR(C::B_PV + x), 1);
-            mbar_init(BAR(C::B_OE + x), 4);
+            mbar_init(BAR(C::B_OE + x), 8);
         }
         mbar_init(BAR(C::B_DONE), 1);
         *abort_flag = 0;
@@ -210,9 +214,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         mbar_wait_bounded(BAR(C::B_DONE), 0u, abort_flag, a.err, a.dbg, 58, 0, false, kDrainLimitCycles);
     } else {
-        // ------------------------------------------------------------ softmax, one thread per row
-        const int x = (warp - 2) >> 2;
+        // ------------------------------------------------------------ softmax, two threads per row
+        constexpr int SW = BN / 2, HW = HD / 2;  // scores and dims of a thread
+        const int x = (warp - 2) >> 3, hf = ((warp - 2) >> 2) & 1;
         const int q4 = warp & 3;
+        float* mine = reinterpret_cast<float*>(base + C::OFF_XCH) + (x * 2 + hf) * 128 + q4 * 32 + lane;
+        const float* other = reinterpret_cast<const float*>(base + C::OFF_XCH) + (x * 2 + (hf ^ 1)) * 128 + q4 * 32 + lane;
+        auto meet = [&]() { named_bar_sync(1 + x * 4 + q4, 64); };
+        // The other thread's value for this row.  A write must not meet the partner's
+        // read of the value before it: per tile the S in between sees to that, else
+        // the barriers do.
+        auto swap = [&](float v, bool before, bool after) {
+            if (before) meet();
+            *mine = v;
+            meet();
+            const float o = *other;
+            if (after) meet();
+            return o;
+        };
         const int r = q4 * 32 + lane;  // row of the tile = TMEM lane
         const int j = r / G, h = r % G;
         const uint32_t lane_addr = static_cast<uint32_t>(q4 * 32) << 16;
@@ -223,15 +242,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         // two fp16 parts.  Returns the power of two that undoes it.
         auto stage_q = [&](const PrefillTile& tl) -> float {
             const int tok = x * TQ + j;
-            float qr[HD];
+            float qr[HW];
             if (tok < tl.ntok) {
                 const long long io = static_cast<long long>(tl.io0) + static_cast<long long>(tok) * tl.io_step;
                 const float* src = a.q + io * a.q_stride + static_cast<long long>(tl.kvh * G + h) * HD;
                 const float2* cs = a.rope + static_cast<long long>(tl.rope_row0 + tok) * (HD / 2);
                 const bool vec = a.q_vec && tl.rope_half % 4 == 0;
 #pragma unroll
-                for (int d = 0; d < HD; d += 4) {
-                    const float4 v = rope4(src, d, tl.rope_half, cs, a.neox != 0, vec);
+                for (int d = 0; d < HW; d += 4) {
+                    const float4 v = rope4(src, hf * HW + d, tl.rope_half, cs, a.neox != 0, vec);
                     qr[d] = v.x;
                     qr[d + 1] = v.y;
                     qr[d + 2] = v.z;
@@ -239,21 +258,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             } else {
 #pragma unroll
-                for (int d = 0; d < HD; ++d) qr[d] = 0.0f;
+                for (int d = 0; d < HW; ++d) qr[d] = 0.0f;
             }
             float mx = 0.0f;
 #pragma unroll
-            for (int d = 0; d < HD; ++d) mx = fmaxf(mx, fabsf(qr[d]));
+            for (int d = 0; d < HW; ++d) mx = fmaxf(mx, fabsf(qr[d]));
+            mx = fmaxf(mx, swap(mx, true, false));
             const int e = static_cast<int>((__float_as_uint(mx) >> 23) & 0xFFu) - 127;
             const int sh = min(60, max(-60, 14 - e));
             const float up = exp2_int(sh);
             unsigned char* q = base + C::OFF_Q + 2 * x * C::TILE;
 #pragma unroll
-            for (int c = 0; c < HD / 8; ++c) {
+            for (int cc = 0; cc < HW / 8; ++cc) {
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    split_pair<DT_F16T>(qr[8 * c + 2 * i] * up, qr[8 * c + 2 * i + 1] * up, hi[i], lo[i]);
+                    split_pair<DT_F16T>(qr[8 * cc + 2 * i] * up, qr[8 * cc + 2 * i + 1] * up, hi[i], lo[i]);
+                const int c = hf * (HW / 8) + cc;
                 const int off = (c / 8) * C::SLAB + r * 128 + (((c % 8) ^ (r & 7)) * 16);
                 *reinterpret_cast<uint4*>(q + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                 *reinterpret_cast<uint4*>(q + C::TILE + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -283,26 +304,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                 WAIT(C::B_SF + x, g & 1, 59, g);
                 __syncwarp();
                 tc_fence_after();
-                const int c0 = tl.kv_lo + t * BN;
-                const bool masked = c0 + BN - 1 > row0 || c0 < lo_all;
+                const int c0 = tl.kv_lo + t * BN + hf * SW;
+                const bool masked = c0 + SW - 1 > row0 || c0 < lo_all;
+                uint32_t s[SW];
+                tmem_ld64(ts + hf * SW, s);
+                tc_fence_before();
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (masked) {
 #pragma unroll
-                for (int c = 0; c < BN; c += 32) {
-                    uint32_t s[32];
-                    tmem_ld32(ts + c, s);
-                    if (masked) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int col = c0 + c + i;
-                            mx[i & 3] = fmaxf(mx[i & 3], col >= lo_r && col <= hi_r ? __uint_as_float(s[i]) : -INFINITY);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2)
-                            mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                    for (int i = 0; i < SW; ++i) {
+                        if (c0 + i < lo_r || c0 + i > hi_r) s[i] = 0xFF800000u;  // -inf
+                        mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
                     }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < SW; i += 2)
+                        mx[(i >> 1) & 3] = fmax3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                 }
                 float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                mt = fmaxf(mt, swap(mt, false, false));  // both have read their scores, too
                 // the score's soft cap is monotone: the capped maximum is the maximum's cap
                 mt = capped ? (mt == -INFINITY ? mt : a.cap_out * tanhf(mt * mul2 * a.cap_in)) : mt * mul2;
                 const bool move = mt > m + 8.0f || (m == -INFINITY && mt > -INFINITY);
@@ -315,44 +335,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // this S was issued after the P.V before it had completed
                     if (t > 0) {
 #pragma unroll
-                        for (int c = 0; c < HD; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(to + c, o);
+                        for (int c = 0; c < HW; c += 16) {
+                            uint32_t o[16];  // (few: the scores are live)
+                            tmem_ld16(to + hf * HW + c, o);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st32(to + c, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st16(to + hf * HW + c, o);
                         }
                     }
                 }
                 const float add = m == -INFINITY ? 0.0f : 7.0f - m;
                 float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t lw[64];  // second parts: their columns hold scores until all are read
+                if (capped) {
+                    // (masked scores stay -inf: their weight is 0)
 #pragma unroll
-                for (int c = 0; c < BN; c += 32) {
-                    uint32_t s[32], hw[16];
-                    tmem_ld32(ts + c, s);
-                    if (masked || capped) {
+                    for (int i = 0; i < SW; ++i)
+                        if (s[i] != 0xFF800000u)
+                            s[i] = __float_as_uint(a.cap_out * tanhf(__uint_as_float(s[i]) * mul2 * a.cap_in));
+                }
+                const float k = capped ? 1.0f : mul2;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float v = __uint_as_float(s[i]) * mul2;
-                            if (capped) v = a.cap_out * tanhf(v * a.cap_in);
-                            const int col = c0 + c + i;
-                            s[i] = __float_as_uint(col >= lo_r && col <= hi_r ? v : -INFINITY);
-                        }
-                    }
-                    const float k = masked || capped ? 1.0f : mul2;
+                for (int c = 0; c < SW; c += 32) {
+                    uint32_t hw[16], lw[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
                         float x0 = add, x1 = add;
-                        fma_x2(x0, x1, __uint_as_float(s[i]), __uint_as_float(s[i + 1]), k, k);
+                        fma_x2(x0, x1, __uint_as_float(s[c + i]), __uint_as_float(s[c + i + 1]), k, k);
                         const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
                         add_x2(ls[i & 2], ls[(i & 2) + 1], p0, p1);
-                        split_pair<DT_F16T>(p0, p1, hw[i / 2], lw[c / 2 + i / 2]);
+                        split_pair<DT_F16T>(p0, p1, hw[i / 2], lw[i / 2]);
                     }
-                    tmem_st16(ts + c / 2, hw);  // over columns that have been read
+                    // over the scores, which are all in registers
+                    tmem_st16(ts + (hf * SW + c) / 2, hw);
+                    tmem_st16(ts + 64 + (hf * SW + c) / 2, lw);
                 }
-#pragma unroll
-                for (int c = 0; c < 64; c += 16) tmem_st16(ts + 64 + c, reinterpret_cast<const uint32_t(&)[16]>(lw[c]));
                 l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
                 tc_fence_before();
                 __syncwarp();
@@ -366,9 +382,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_after();
                 const long long io = static_cast<long long>(tl.io0) + static_cast<long long>(tok) * tl.io_step;
                 float* dst = a.out + io * a.q_stride + static_cast<long long>(tl.kvh * G + h) * HD;
-                const float inv = l > 0.0f ? hs.y / l : 0.0f;
+                const float lt = l + swap(l, true, true);
+                const float inv = lt > 0.0f ? hs.y / lt : 0.0f;
 #pragma unroll
-                for (int c = 0; c < HD; c += 32) {
+                for (int cc = 0; cc < HW; cc += 32) {
+                    const int c = hf * HW + cc;
                     uint32_t o[32];
                     tmem_ld32(to + c, o);
                     if (live) {
