@@ -177,16 +177,17 @@ __global__ void __launch_bounds__(2 * HD) append_kernel(const __grid_constant__ 
     float m = 0.0f;
     if (is_new) {
         const long long io = static_cast<long long>(run.io0 + t - run.pos0) * a.n_io_layers + L.io;
-        if (which == 0) {
-            const float* src = a.k_in + io * a.kv_stride + h * HD;
-            const float2* cs = a.rope[L.cfg] + static_cast<long long>(t) * (HD / 2);
+        const float* src = (which == 0 ? a.k_in : a.v_in) + io * a.kv_stride + h * HD;
+        const float2* cs = a.rope[L.cfg] + static_cast<long long>(t) * (HD / 2);
+        const int half = which == 0 ? L.half : 0;
+        const bool vec = a.kv_vec && half % 4 == 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                x[i] = cache_value(rope_plain(src, d0 + i, L.half, cs, a.neox != 0));
-        } else {
-            const float* src = a.v_in + io * a.kv_stride + h * HD + d0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = cache_value(src[i]);
+        for (int i = 0; i < 4; ++i) {
+            const float4 v = rope4(src, d0 + 4 * i, half, cs, a.neox != 0, vec);
+            x[4 * i] = cache_value(v.x);
+            x[4 * i + 1] = cache_value(v.y);
+            x[4 * i + 2] = cache_value(v.z);
+            x[4 * i + 3] = cache_value(v.w);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(x[i]));
