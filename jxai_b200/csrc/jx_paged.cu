@@ -503,6 +503,8 @@ struct jx_pkv {
     size_t wide_bytes = 0;
     float2* d_head_scale = nullptr;
     size_t head_scales = 0;
+    float* d_totals = nullptr;            // prompts: the CTAs' running sums
+    size_t totals_bytes = 0;
     int num_sms = 0;
     int opt_wait_limit_ms = 0;
     int last_launches = 0;
@@ -933,6 +935,9 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
     }
     if (int rc = grow_device(reinterpret_cast<void**>(&kv->d_wide), &kv->wide_bytes, wide, "fp16 rows")) return rc;
     if (int rc = grow_device(reinterpret_cast<void**>(&kv->d_head_scale), &kv->head_scales, heads * sizeof(float2), "head scales")) return rc;
+    if (int rc = grow_device(reinterpret_cast<void**>(&kv->d_totals), &kv->totals_bytes,
+                             static_cast<size_t>(std::max(kv->num_sms, 1)) * 2 * hd * kPromptRows * sizeof(float), "totals"))
+        return rc;
     jx_pkv::Upload* u = nullptr;
     if (int rc = take_upload(kv, bytes, &u)) return rc;
     std::memcpy(u->h, items.data(), first_at);
@@ -984,6 +989,7 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
         p.q_stride = A.q_stride;
         p.rope = A.rope[g.layers[0].cfg];
         p.head_scale = kv->d_head_scale;
+        p.totals = kv->d_totals;
         p.scale_layers = static_cast<int>(nl);
         p.scale_heads = A.n_kv;
         p.neox = A.neox;
@@ -1330,6 +1336,7 @@ int jx_pkv_destroy(jx_pkv* kv) {
     cudaFree(kv->d_dbg);
     cudaFree(kv->d_wide);
     cudaFree(kv->d_head_scale);
+    cudaFree(kv->d_totals);
     for (auto& u : kv->up) {
         cudaFree(u.d);
         if (u.h) cudaFreeHost(u.h);

@@ -231,6 +231,7 @@ struct PromptArgs {
     long long q_stride;
     const float2* rope;     // rows of HD/2 (cos, sin) pairs, by position
     const float2* head_scale;
+    float* totals;          // [grid][2][HD][128]
     int scale_layers, scale_heads;
     int neox, q_vec;
     float scale, softcap, cap_in, cap_out;

@@ -24,6 +24,11 @@
 //    rescaled in TMEM, its P.V known complete from the S that follows it); a
 //    weight of 1 is 2^7 in fp16, so weights reach 2^15 and the fp16 floor lies
 //    2^-32 below 1.
+//  * The tensor cores cut the sum they add to towards zero (about 1e-8 of it per
+//    MMA of 16 rows), which over thousands of rows adds up to 1e-5.  So O sums
+//    kDrain tiles, then the softmax threads add it to an fp32 total of their own
+//    in global memory (L2; [dim][row], so that a warp's accesses are whole lines),
+//    while the next S is being computed, and P.V begins anew.
 //  * Every mbarrier wait is bounded; one that runs out raises the abort flag and
 //    the device error word, and every role finishes its control flow.
 #include "jx_internal.h"
@@ -35,6 +40,7 @@ namespace {
 
 constexpr int kThreads = 32 * 18;
 constexpr float kLog2 = 1.4426950408889634f;
+constexpr int kDrain = 3;  // K/V tiles that O sums before it is added to the total
 
 template <int HD>
 struct PromptCfg {
@@ -193,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 for (int kb = 0; kb < BN / 16; ++kb)
                                     tc_mma_ts(tmem + C::COL_O + x * 128, tmem + C::COL_S + x * 128 + part * 64 + kb * 8,
                                               sw128_desc(kv_at(n) + kb * 16 * 128, C::SLAB, 1024), ID_PV,
-                                              (t | part | kb) != 0 ? 1u : 0u);
+                                              (t % kDrain != 0 || (part | kb) != 0) ? 1u : 0u);
                             tc_commit(BAR(C::B_PV + x));
                         }
                         __syncwarp();
@@ -233,6 +239,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             return o;
         };
         const int r = q4 * 32 + lane;  // row of the tile = TMEM lane
+        // this thread's running totals, dim c of its half at total[c * 128]
+        float* total = a.totals + ((static_cast<long long>(blockIdx.x) * 2 + x) * HD + hf * HW) * 128 + r;
         const int j = r / G, h = r % G;
         const uint32_t lane_addr = static_cast<uint32_t>(q4 * 32) << 16;
         const uint32_t ts = tmem + lane_addr + C::COL_S + x * 128;
@@ -300,7 +308,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float mul = a.scale * unscale * hs.x;  // raw S -> score
             const float mul2 = mul * kLog2;
             float m = -INFINITY, l = 0.0f;  // the maximum in units of log2
+            float behind = 1.0f;            // what the total is to be multiplied by since it was written
             for (int t = 0; t < nt; ++t, ++g) {
+                if (t > 0 && t % kDrain == 0) {
+                    // O of the tiles so far to the total, while S is being computed
+                    float sum[HW];
+#pragma unroll
+                    for (int c = 0; c < HW; ++c) sum[c] = t > kDrain ? __ldcg(total + c * 128) : 0.0f;
+                    WAIT(C::B_PV + x, (g - 1) & 1, 62, g);
+                    __syncwarp();
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < HW; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(to + hf * HW + c, o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            __stcg(total + (c + i) * 128, fmaf(sum[c + i], behind, __uint_as_float(o[i])));
+                    }
+                    behind = 1.0f;
+                    tc_fence_before();
+                }
                 WAIT(C::B_SF + x, g & 1, 59, g);
                 __syncwarp();
                 tc_fence_after();
@@ -330,10 +358,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float f = !move ? 1.0f : (m == -INFINITY ? 0.0f : ex2_approx(m - mt));
                     if (move) {
                         l *= f;
+                        behind *= f;
                         m = mt;
                     }
                     // this S was issued after the P.V before it had completed
-                    if (t > 0) {
+                    if (t % kDrain != 0) {
 #pragma unroll
                         for (int c = 0; c < HW; c += 16) {
                             uint32_t o[16];  // (few: the scores are live)
@@ -377,6 +406,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the next item's Q while the last P.V runs: every S of this one is done
             const float next = it + 1 < it_end ? stage_q(a.tiles[it + 1]) : 1.0f;
             if (nt > 0) {
+                const bool drained = nt > kDrain;
+                float sum[HW];
+#pragma unroll
+                for (int c = 0; c < HW; ++c) sum[c] = drained ? __ldcg(total + c * 128) : 0.0f;
                 WAIT(C::B_PV + x, (g - 1) & 1, 60, g);
                 __syncwarp();
                 tc_fence_after();
@@ -385,16 +418,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float lt = l + swap(l, true, true);
                 const float inv = lt > 0.0f ? hs.y / lt : 0.0f;
 #pragma unroll
-                for (int cc = 0; cc < HW; cc += 32) {
-                    const int c = hf * HW + cc;
-                    uint32_t o[32];
-                    tmem_ld32(to + c, o);
+                for (int c = 0; c < HW; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(to + hf * HW + c, o);
                     if (live) {
 #pragma unroll
-                        for (int d = 0; d < 32; d += 4)
-                            *reinterpret_cast<float4*>(dst + c + d) =
-                                make_float4(__uint_as_float(o[d]) * inv, __uint_as_float(o[d + 1]) * inv,
-                                            __uint_as_float(o[d + 2]) * inv, __uint_as_float(o[d + 3]) * inv);
+                        for (int d = 0; d < 16; d += 4)
+                            *reinterpret_cast<float4*>(dst + hf * HW + c + d) = make_float4(
+                                fmaf(sum[c + d], behind, __uint_as_float(o[d])) * inv,
+                                fmaf(sum[c + d + 1], behind, __uint_as_float(o[d + 1])) * inv,
+                                fmaf(sum[c + d + 2], behind, __uint_as_float(o[d + 2])) * inv,
+                                fmaf(sum[c + d + 3], behind, __uint_as_float(o[d + 3])) * inv);
                     }
                     __syncwarp();  // converged for the next .sync.aligned load
                 }

@@ -386,23 +386,39 @@ struct StepWarp {
     // O += P V for the page whose weights `scores` left.
     __device__ __forceinline__ void values(uint32_t vbase, int lane) {
         const int i8 = lane >> 3, vr = (i8 & 1) * 8 + row_perm<HD>(lane & 7);
+        // A page's 32 rows are summed from zero and then added: the tensor cores cut
+        // the sum they add to towards zero (about 1e-8 of it each time), which over
+        // the rows of a long cache would add up; an fp32 addition rounds.
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int c = 0; c < KS; c += 2) {  // chunks of 16 dims, two per load
+            float acc[2][NBC][4];
 #pragma unroll
-            for (int c = 0; c < KS; c += 2) {  // chunks of 16 dims, two per load
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int nb = 0; nb < NBC; ++nb)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][nb][r] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
                 uint32_t r0, r1, r2, r3;
                 ldsm_x4<true>(vbase + tile_byte(HD, b * 16 + vr, (c + (i8 >> 1)) * 16), r0, r1, r2, r3);
                 uint32_t e0, d0, e1, d1;
                 codes_split<DT>(r0, e0, d0);
                 codes_split<DT>(r1, e1, d1);
 #pragma unroll
-                for (int nb = 0; nb < NBC; ++nb) mma_16816<DT_F16T>(o[c][nb], e0, d0, e1, d1, bp[b][nb][0], bp[b][nb][1]);
+                for (int nb = 0; nb < NBC; ++nb) mma_16816<DT_F16T>(acc[0][nb], e0, d0, e1, d1, bp[b][nb][0], bp[b][nb][1]);
                 codes_split<DT>(r2, e0, d0);
                 codes_split<DT>(r3, e1, d1);
 #pragma unroll
-                for (int nb = 0; nb < NBC; ++nb)
-                    mma_16816<DT_F16T>(o[c + 1][nb], e0, d0, e1, d1, bp[b][nb][0], bp[b][nb][1]);
+                for (int nb = 0; nb < NBC; ++nb) mma_16816<DT_F16T>(acc[1][nb], e0, d0, e1, d1, bp[b][nb][0], bp[b][nb][1]);
             }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int nb = 0; nb < NBC; ++nb) {
+                    add_x2(o[c + i][nb][0], o[c + i][nb][1], acc[i][nb][0], acc[i][nb][1]);
+                    add_x2(o[c + i][nb][2], o[c + i][nb][3], acc[i][nb][2], acc[i][nb][3]);
+                }
         }
     }
 
