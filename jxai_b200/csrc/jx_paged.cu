@@ -219,44 +219,75 @@ struct KeepArgs {
     int serial;            // one CTA per record, block after block (in place)
 };
 
+constexpr int kKeepRecords = 4;  // records of a block that a CTA moves together
+
 // Kept rows gathered into dense blocks: each is scaled and rounded anew from
-// the values held.  Same thread layout as append_kernel.  Row i of the result
-// comes from a row >= i, and a CTA reads all of a block before it writes it: in
-// place (serial) no row is overwritten before it has been read.
+// the values held.  One CTA per (block of 16 rows, kKeepRecords records); its
+// first half takes K, its second V, one thread per 16 values of a row.  Where a
+// row lies is looked up once for all records, and their loads are in flight
+// together: a block alone is 8 KB behind three dependent loads.  Row i of the
+// result comes from a row >= i, and a CTA reads all of a block before it writes
+// it: in place (serial) no row is overwritten before it has been read.
 template <int HD, int DT>
 __global__ void __launch_bounds__(2 * HD) keep_kernel(const KeepArgs a) {
-    constexpr int CPR = HD / 16;
-    __shared__ float red[2 * HD / 32];
+    constexpr int CPR = HD / 16, R = kKeepRecords, WARPS = 2 * HD / 32;
+    __shared__ float red[R][WARPS];
     const int which = threadIdx.x / HD, tid = threadIdx.x % HD;
     const int row = tid / CPR, d0 = tid % CPR * 16;
-    const long long rec_off = static_cast<long long>(blockIdx.y) * record_bytes(HD);
+    const int rec0 = blockIdx.y * R, n_rec = min(R, a.n_rec - rec0);
     const int last = a.serial ? a.n_blk : static_cast<int>(blockIdx.x) + 1;
     for (int b = a.serial ? 0 : static_cast<int>(blockIdx.x); b < last; ++b) {
         const int blk = a.blk0 + b;
         const int i = blk * kBlockRows + row;
-        float x[16];
-        float m = 0.0f;
-        if (i < a.n_rows) {
+        const bool on = i < a.n_rows;
+        uint4 c[R];
+        float s[R];
+        if (on) {
             const int t = a.rows[i];
-            const unsigned char* rec = a.pool + a.src_table[t / kPageRows] * a.page_bytes + rec_off;
-            const float s = reinterpret_cast<const float*>(rec)[which * 2 + (t / kBlockRows & 1)];
-            unpack_codes<DT>(*reinterpret_cast<const uint4*>(rec + tile_at(HD, which) +
-                                                             tile_byte(HD, t % kPageRows, d0)), x);
+            const unsigned char* rec = a.pool + a.src_table[t / kPageRows] * a.page_bytes +
+                                       static_cast<long long>(rec0) * record_bytes(HD);
+            const uint32_t at = tile_at(HD, which) + tile_byte(HD, t % kPageRows, d0);
+            const int k = which * 2 + (t / kBlockRows & 1);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                x[j] *= s;
-                m = fmaxf(m, fabsf(x[j]));
-            }
+            for (int j = 0; j < R; ++j)
+                if (j < n_rec) {
+                    c[j] = *reinterpret_cast<const uint4*>(rec + j * record_bytes(HD) + at);
+                    s[j] = reinterpret_cast<const float*>(rec + j * record_bytes(HD))[k];
+                }
         }
-        m = half_max(m, red, HD);  // its barriers also order this block's reads before its writes
-        const int k = block_exp<DT>(m);
-        unsigned char* rec = a.pool + a.dst_table[blk / 2] * a.page_bytes + rec_off;
-        if (i < a.n_rows)
-            *reinterpret_cast<uint4*>(rec + tile_at(HD, which) +
-                                      tile_byte(HD, (blk & 1) * kBlockRows + row, d0)) =
-                pack_codes<DT>(x, exp2_int(-k));
-        if (tid == 0) reinterpret_cast<float*>(rec)[which * 2 + (blk & 1)] = exp2_int(k);
-        __syncthreads();  // this block's writes before the next one's reads
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            float m = 0.0f;
+            if (on && j < n_rec) {
+                float x[16];
+                unpack_codes<DT>(c[j], x);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(x[e]));
+                m *= s[j];
+            }
+            m = warp_max(m);
+            if (threadIdx.x % 32 == 0) red[j][threadIdx.x / 32] = m;
+        }
+        __syncthreads();  // this block's reads are done before its writes begin, too
+        unsigned char* rec = a.pool + a.dst_table[blk / 2] * a.page_bytes + static_cast<long long>(rec0) * record_bytes(HD);
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            if (j >= n_rec) break;
+            float m = 0.0f;
+            for (int w = 0; w < WARPS / 2; ++w) m = fmaxf(m, red[j][which * (WARPS / 2) + w]);
+            const int k = block_exp<DT>(m);
+            if (on) {
+                float x[16];
+                unpack_codes<DT>(c[j], x);
+                // the scale's change alone: code 2^ks to code 2^k
+                *reinterpret_cast<uint4*>(rec + j * record_bytes(HD) + tile_at(HD, which) +
+                                          tile_byte(HD, (blk & 1) * kBlockRows + row, d0)) =
+                    pack_codes<DT>(x, s[j] * exp2_int(-k));
+            }
+            if (tid == 0)
+                reinterpret_cast<float*>(rec + j * record_bytes(HD))[which * 2 + (blk & 1)] = exp2_int(k);
+        }
+        __syncthreads();  // this block's writes before the next one's reads; red is free
     }
 }
 
@@ -1217,7 +1248,7 @@ int keep_impl(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, cu
     k.blk0 = static_cast<int>(keep_pages * (kPageRows / kBlockRows));
     k.n_blk = static_cast<int>((n_rows + kBlockRows - 1) / kBlockRows) - k.blk0;
     k.serial = in_place ? 1 : 0;
-    const dim3 grid(in_place ? 1 : k.n_blk, k.n_rec);
+    const dim3 grid(in_place ? 1 : k.n_blk, (k.n_rec + kKeepRecords - 1) / kKeepRecords);
     dispatch(D, [&](auto hd, auto dt) {
         keep_kernel<hd.value, dt.value><<<grid, 2 * hd.value, 0, st>>>(k);
     });

@@ -26,7 +26,7 @@
 //    2^-32 below 1.
 //  * The tensor cores cut the sum they add to towards zero (about 1e-8 of it per
 //    MMA of 16 rows), which over thousands of rows adds up to 1e-5.  So O sums
-//    kDrain tiles, then the softmax threads add it to an fp32 total of their own
+//    a few tiles, then the softmax threads add it to an fp32 total of their own
 //    in global memory (L2; [dim][row], so that a warp's accesses are whole lines),
 //    while the next S is being computed, and P.V begins anew.
 //  * Every mbarrier wait is bounded; one that runs out raises the abort flag and
@@ -40,7 +40,7 @@ namespace {
 
 constexpr int kThreads = 32 * 18;
 constexpr float kLog2 = 1.4426950408889634f;
-constexpr int kDrain = 3;  // K/V tiles that O sums before it is added to the total
+
 
 template <int HD>
 struct PromptCfg {
@@ -58,6 +58,7 @@ struct PromptCfg {
     static constexpr int OFF_XCH = OFF_MISC + 16;      // [tile][half][128] floats: row exchanges
     static constexpr int SMEM = OFF_XCH + 2 * 2 * 128 * 4;
     static constexpr int COL_S = 0, COL_O = 256;       // tile X: + 128 X
+    static constexpr int DRAIN = HD == 64 ? 4 : 6;     // K/V tiles that O sums before it is added to the total
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
 
@@ -153,19 +154,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int cnt[2] = {tiles_of(tl, 0), tiles_of(tl, 1)};
             const int nt = max(cnt[0], cnt[1]);
             auto kv_at = [&](int n) { return sbase + C::OFF_KV + (n % C::NS) * C::TILE; };
-            auto issue_s = [&](int x, int t) {  // S = Q_hi.K^T + Q_lo.K^T
+            auto issue_s = [&](int x, int t) {  // S = Q_lo.K^T + Q_hi.K^T
                 const int n = n0 + 2 * t;
                 WAIT(C::B_KVF + n % C::NS, (n / C::NS) & 1, 52, n);
                 tc_fence_after();
                 if (lane == 0) {
+                    // the small parts first: what the sum loses is in proportion to its size
 #pragma unroll
-                    for (int part = 0; part < 2; ++part)
+                    for (int part = 1; part >= 0; --part)
 #pragma unroll
                         for (int ks = 0; ks < HD / 16; ++ks) {
                             const uint32_t off = (ks / 4) * C::SLAB + (ks % 4) * 32;
                             tc_mma(tmem + C::COL_S + x * 128,
                                    sw128_desc(sbase + C::OFF_Q + (2 * x + part) * C::TILE + off, 16, 1024),
-                                   sw128_desc(kv_at(n) + off, 16, 1024), ID_S, (part | ks) != 0 ? 1u : 0u);
+                                   sw128_desc(kv_at(n) + off, 16, 1024), ID_S, part == 0 || ks != 0 ? 1u : 0u);
                         }
                     tc_commit(BAR(C::B_SF + x));
                 }
@@ -194,12 +196,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc_fence_after();
                         if (lane == 0) {
 #pragma unroll
-                            for (int part = 0; part < 2; ++part)
+                            for (int part = 1; part >= 0; --part)
 #pragma unroll
                                 for (int kb = 0; kb < BN / 16; ++kb)
                                     tc_mma_ts(tmem + C::COL_O + x * 128, tmem + C::COL_S + x * 128 + part * 64 + kb * 8,
                                               sw128_desc(kv_at(n) + kb * 16 * 128, C::SLAB, 1024), ID_PV,
-                                              (t % kDrain != 0 || (part | kb) != 0) ? 1u : 0u);
+                                              t % C::DRAIN != 0 || part == 0 || kb != 0 ? 1u : 0u);
                             tc_commit(BAR(C::B_PV + x));
                         }
                         __syncwarp();
@@ -310,21 +312,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             float m = -INFINITY, l = 0.0f;  // the maximum in units of log2
             float behind = 1.0f;            // what the total is to be multiplied by since it was written
             for (int t = 0; t < nt; ++t, ++g) {
-                if (t > 0 && t % kDrain == 0) {
-                    // O of the tiles so far to the total, while S is being computed
-                    float sum[HW];
+                if (t > 0 && t % C::DRAIN == 0) {
+                    // O of the tiles so far to the total, while S is being computed; 32
+                    // dims at a time, the first ones' totals fetched during the wait
+                    float sum[32];
 #pragma unroll
-                    for (int c = 0; c < HW; ++c) sum[c] = t > kDrain ? __ldcg(total + c * 128) : 0.0f;
-                    WAIT(C::B_PV + x, (g - 1) & 1, 62, g);
-                    __syncwarp();
-                    tc_fence_after();
+                    for (int c = 0; c < HW; ++c) {
+                        if (c % 32 == 0) {
 #pragma unroll
-                    for (int c = 0; c < HW; c += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(to + hf * HW + c, o);
+                            for (int i = 0; i < 32; ++i) sum[i] = t > C::DRAIN ? __ldcg(total + (c + i) * 128) : 0.0f;
+                            if (c == 0) {
+                                WAIT(C::B_PV + x, (g - 1) & 1, 62, g);
+                                __syncwarp();
+                                tc_fence_after();
+                            }
+                        }
+                        if (c % 16 == 0) {
+                            uint32_t o[16];
+                            tmem_ld16(to + hf * HW + c, o);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            __stcg(total + (c + i) * 128, fmaf(sum[c + i], behind, __uint_as_float(o[i])));
+                            for (int i = 0; i < 16; ++i)
+                                __stcg(total + (c + i) * 128, fmaf(sum[c % 32 + i], behind, __uint_as_float(o[i])));
+                        }
                     }
                     behind = 1.0f;
                     tc_fence_before();
@@ -362,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         m = mt;
                     }
                     // this S was issued after the P.V before it had completed
-                    if (t % kDrain != 0) {
+                    if (t % C::DRAIN != 0) {
 #pragma unroll
                         for (int c = 0; c < HW; c += 16) {
                             uint32_t o[16];  // (few: the scores are live)
@@ -406,10 +415,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the next item's Q while the last P.V runs: every S of this one is done
             const float next = it + 1 < it_end ? stage_q(a.tiles[it + 1]) : 1.0f;
             if (nt > 0) {
-                const bool drained = nt > kDrain;
-                float sum[HW];
-#pragma unroll
-                for (int c = 0; c < HW; ++c) sum[c] = drained ? __ldcg(total + c * 128) : 0.0f;
                 WAIT(C::B_PV + x, (g - 1) & 1, 60, g);
                 __syncwarp();
                 tc_fence_after();
@@ -419,16 +424,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float inv = lt > 0.0f ? hs.y / lt : 0.0f;
 #pragma unroll
                 for (int c = 0; c < HW; c += 16) {
+                    float sum[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[i] = nt > C::DRAIN ? __ldcg(total + (c + i) * 128) : 0.0f;
                     uint32_t o[16];
                     tmem_ld16(to + hf * HW + c, o);
                     if (live) {
 #pragma unroll
                         for (int d = 0; d < 16; d += 4)
                             *reinterpret_cast<float4*>(dst + hf * HW + c + d) = make_float4(
-                                fmaf(sum[c + d], behind, __uint_as_float(o[d])) * inv,
-                                fmaf(sum[c + d + 1], behind, __uint_as_float(o[d + 1])) * inv,
-                                fmaf(sum[c + d + 2], behind, __uint_as_float(o[d + 2])) * inv,
-                                fmaf(sum[c + d + 3], behind, __uint_as_float(o[d + 3])) * inv);
+                                fmaf(sum[d], behind, __uint_as_float(o[d])) * inv,
+                                fmaf(sum[d + 1], behind, __uint_as_float(o[d + 1])) * inv,
+                                fmaf(sum[d + 2], behind, __uint_as_float(o[d + 2])) * inv,
+                                fmaf(sum[d + 3], behind, __uint_as_float(o[d + 3])) * inv);
                     }
                     __syncwarp();  // converged for the next .sync.aligned load
                 }
