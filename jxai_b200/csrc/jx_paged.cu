@@ -345,31 +345,30 @@ struct ReadArgs {
     void* out;
     long long page_bytes;
     int max_pages, n_kv, n_layers, n_rows, n;
+    int r0, rows;  // the rows of this launch, of n_rows
     int seq[kMaxRuns];
     int row0[kMaxRuns];
 };
+static_assert(sizeof(ReadArgs) <= 4096, "kernel parameters");
 
+// Values of rows; one (sequence, layer, K or V) per (z, y) of the grid, a thread
+// per 16 codes of a row, in the order of the output.
 template <int HD, int DT, bool F32>
 __global__ void read_kernel(const __grid_constant__ ReadArgs a) {
-    constexpr int CPR = HD / 16;
-    const long long per = static_cast<long long>(a.n_layers) * 2 * a.n_rows * a.n_kv * CPR;
-    const int s = blockIdx.y;
-    for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < per;
-         i += static_cast<long long>(gridDim.x) * blockDim.x) {
-        const int c = static_cast<int>(i % CPR);
-        const int h = static_cast<int>(i / CPR % a.n_kv);
-        long long q = i / CPR / a.n_kv;
-        const int t = a.row0[s] + static_cast<int>(q % a.n_rows);
-        q /= a.n_rows;
-        const int which = static_cast<int>(q & 1), l = static_cast<int>(q >> 1);
-        const unsigned char* rec =
-            a.pool + a.table[static_cast<long long>(a.seq[s]) * a.max_pages + t / kPageRows] * a.page_bytes +
-            (static_cast<long long>(l) * a.n_kv + h) * record_bytes(HD);
+    constexpr uint32_t CPR = HD / 16;
+    const int s = blockIdx.z, which = blockIdx.y & 1, l = blockIdx.y >> 1;
+    const int* table = a.table + static_cast<long long>(a.seq[s]) * a.max_pages;
+    const uint32_t per_row = a.n_kv * CPR, n = a.rows * per_row;
+    const long long out0 = (((static_cast<long long>(s) * a.n_layers + l) * 2 + which) * a.n_rows + a.r0) * per_row;
+    for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
+        const uint32_t r = i / per_row, c = i % CPR, h = (i - r * per_row) / CPR;
+        const int t = a.row0[s] + a.r0 + static_cast<int>(r);
+        const unsigned char* rec = a.pool + table[t / kPageRows] * a.page_bytes +
+                                   (static_cast<long long>(l) * a.n_kv + h) * record_bytes(HD);
         const float sc = reinterpret_cast<const float*>(rec)[which * 2 + (t / kBlockRows & 1)];
         float x[16];
-        unpack_codes<DT>(*reinterpret_cast<const uint4*>(rec + tile_at(HD, which) +
-                                                         tile_byte(HD, t % kPageRows, c * 16)), x);
-        const long long o = (s * per + i) * 16;
+        unpack_codes<DT>(*reinterpret_cast<const uint4*>(rec + tile_at(HD, which) + tile_byte(HD, t % kPageRows, c * 16)), x);
+        const long long o = (out0 + i) * 16;
         if constexpr (F32) {
             float4* dst = reinterpret_cast<float4*>(static_cast<float*>(a.out) + o);
 #pragma unroll
@@ -1297,9 +1296,9 @@ int jx_pkv_create(const jx_pkv_desc* desc, jx_pkv** out) {
             return pfail(JX_ERR_INVALID, "dtype %d: a paged cache holds JX_I8 or JX_E4M3", d.dtype);
         if (d.head_dim != 32 && d.head_dim != 64 && d.head_dim != 128 && d.head_dim != 256)
             return pfail(JX_ERR_UNSUPPORTED, "head_dim %u (compiled: 32, 64, 128, 256)", d.head_dim);
-        if (d.n_layers > 65535 || d.n_kv_heads > 512 ||
+        if (d.n_layers > 32767 || d.n_kv_heads > 512 ||
             static_cast<uint64_t>(d.n_layers) * d.n_kv_heads > 65535)
-            return pfail(JX_ERR_UNSUPPORTED, "n_kv_heads must be at most 512, n_layers * n_kv_heads at most 65535");
+            return pfail(JX_ERR_UNSUPPORTED, "n_layers must be at most 32767, n_kv_heads 512, their product 65535");
         if (d.capacity > (1u << 30) || d.n_pages > (1u << 30) ||
             static_cast<uint64_t>(d.n_seqs) * ((d.capacity + kPageRows - 1) / kPageRows) > (1ull << 30))
             return pfail(JX_ERR_INVALID, "capacity, n_pages and the page table must stay below 2^30 entries");
@@ -1567,17 +1566,24 @@ int jx_pkv_read_rows(jx_pkv* kv, const int32_t* seq_ids, const int32_t* row0, ui
         a.n_layers = static_cast<int>(D.n_layers);
         a.n_rows = static_cast<int>(n_rows);
         const long long per = static_cast<long long>(D.n_layers) * 2 * n_rows * D.n_kv_heads * (D.head_dim / 16);
+        const uint32_t per_row = D.n_kv_heads * (D.head_dim / 16);
+        const uint32_t most = (1u << 30) / per_row;  // rows of a launch: 32-bit indices
         for (uint32_t s0 = 0; s0 < n; s0 += kMaxRuns) {
             a.n = static_cast<int>(std::min<uint32_t>(kMaxRuns, n - s0));
             std::copy_n(seq_ids + s0, a.n, a.seq);
             std::copy_n(row0 + s0, a.n, a.row0);
             a.out = static_cast<char*>(out) + static_cast<size_t>(s0) * per * 16 * (dtype == JX_F32 ? 4 : 2);
-            const dim3 grid(static_cast<unsigned>(std::min<long long>((per + 255) / 256, 16ll * kv->num_sms)), a.n);
-            dispatch(D, [&](auto hd, auto dt) {
-                if (dtype == JX_F32) read_kernel<hd.value, dt.value, true><<<grid, 256, 0, st>>>(a);
-                else read_kernel<hd.value, dt.value, false><<<grid, 256, 0, st>>>(a);
-            });
-            if (int rc = launched("read")) return rc;
+            for (uint32_t r0 = 0; r0 < n_rows; r0 += most) {
+                a.r0 = static_cast<int>(r0);
+                a.rows = static_cast<int>(std::min(most, n_rows - r0));
+                const uint32_t work = static_cast<uint32_t>(a.rows) * per_row;
+                const dim3 grid(std::min<uint32_t>((work + 255) / 256, 4096), D.n_layers * 2, a.n);
+                dispatch(D, [&](auto hd, auto dt) {
+                    if (dtype == JX_F32) read_kernel<hd.value, dt.value, true><<<grid, 256, 0, st>>>(a);
+                    else read_kernel<hd.value, dt.value, false><<<grid, 256, 0, st>>>(a);
+                });
+                if (int rc = launched("read")) return rc;
+            }
         }
         return JX_OK;
     });

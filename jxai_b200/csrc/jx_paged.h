@@ -135,24 +135,6 @@ __device__ __forceinline__ int scale_exp(float s) {  // k of a stored scale 2^k
     return static_cast<int>(__float_as_uint(s) >> 23) - 127;
 }
 
-// Nearest code of y = x * 2^-k (ties to even), as the stored byte, and back.
-template <int DT>
-__device__ __forceinline__ uint32_t to_code(float y) {
-    if constexpr (DT == DT_I8) {
-        return static_cast<uint32_t>(min(127, max(-127, __float2int_rn(y))) + 128);
-    } else {
-        return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
-    }
-}
-template <int DT>
-__device__ __forceinline__ float from_code(uint32_t b) {
-    if constexpr (DT == DT_I8) {
-        return static_cast<float>(static_cast<int>(b) - 128);
-    } else {
-        return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(b), __NV_E4M3)));
-    }
-}
-
 // One element of a rotated head; each operation's result is an fp32 number
 // (no fused multiply-add), so that what the cache holds does not depend on
 // how the compiler contracts.  cs[j] = (cos, sin).
@@ -195,10 +177,35 @@ __device__ __forceinline__ float4 rope4(const float* x, int d, int half, const f
                        __fadd_rn(__fmul_rn(v.z, c.w), __fmul_rn(v.w, c.z)));
 }
 
-// Four values to codes (x * inv) and back; 16 likewise.
+// Four values to codes (nearest to x * inv, ties to even; inv a power of two and
+// |x * inv| within the codes' range) and back; 16 likewise.  int8: adding
+// 1.5 * 2^23 + 128 leaves the rounded code plus 128 in the sum's low byte, and a
+// byte under the exponent of 2^23 is that number plus its value: no conversion
+// instruction, of which an SM does 16 a cycle.
 template <int DT>
 __device__ __forceinline__ uint32_t pack4(float x, float y, float z, float w, float inv) {
-    return to_code<DT>(x * inv) | to_code<DT>(y * inv) << 8 | to_code<DT>(z * inv) << 16 | to_code<DT>(w * inv) << 24;
+    if constexpr (DT == DT_I8) {
+        constexpr float kMagic = 12582912.0f + 128.0f;
+        const uint32_t a = __float_as_uint(__fmaf_rn(x, inv, kMagic)), b = __float_as_uint(__fmaf_rn(y, inv, kMagic));
+        const uint32_t c = __float_as_uint(__fmaf_rn(z, inv, kMagic)), d = __float_as_uint(__fmaf_rn(w, inv, kMagic));
+        return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+    } else {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x * inv, y * inv), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(z * inv, w * inv), __NV_SATFINITE, __NV_E4M3);
+        return lo | hi << 16;
+    }
+}
+template <int DT>
+__device__ __forceinline__ float4 unpack4(uint32_t w) {
+    if constexpr (DT == DT_I8) {
+        auto at = [&](uint32_t sel) { return __uint_as_float(__byte_perm(w, 0x4B000000u, sel)) - (8388608.0f + 128.0f); };
+        return make_float4(at(0x7540), at(0x7541), at(0x7542), at(0x7543));
+    } else {
+        const __half2_raw l = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xFFFFu), __NV_E4M3);
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
+        const float2 a = __half22float2(__half2(l)), b = __half22float2(__half2(h));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
 }
 template <int DT>
 __device__ __forceinline__ uint4 pack_codes(const float (&x)[16], float inv) {
@@ -209,7 +216,13 @@ template <int DT>
 __device__ __forceinline__ void unpack_codes(const uint4& c, float (&x)[16]) {
     const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = from_code<DT>((w[i / 4] >> (8 * (i % 4))) & 0xFFu);
+    for (int i = 0; i < 4; ++i) {
+        const float4 v = unpack4<DT>(w[i]);
+        x[4 * i] = v.x;
+        x[4 * i + 1] = v.y;
+        x[4 * i + 2] = v.z;
+        x[4 * i + 3] = v.w;
+    }
 }
 
 // CTA that owns unit x when CTA c of P takes units [c*total/P, (c+1)*total/P).

@@ -501,8 +501,8 @@ __device__ __forceinline__ void step_append(const PagedArgs& a, const Piece& p, 
                     for (int r = blk * kBlockRows; r < row; ++r) {
                         const uint32_t at = tile_byte(HD, r, d);
                         const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + at);
-                        const uint32_t n = pack4<DT>(from_code<DT>(w & 0xFFu), from_code<DT>(w >> 8 & 0xFFu),
-                                                     from_code<DT>(w >> 16 & 0xFFu), from_code<DT>(w >> 24), f);
+                        const float4 v = unpack4<DT>(w);
+                        const uint32_t n = pack4<DT>(v.x, v.y, v.z, v.w, f);
                         *reinterpret_cast<uint32_t*>(rec + at) = n;
                         *reinterpret_cast<uint32_t*>(tile + at) = n;
                     }
