@@ -261,7 +261,8 @@ JX_API int jx_noalloc_set_option(const char* key, int value);
  *
  * A sequence holds the rows [0, seq_pos).  A call that writes rows may begin at
  * any position up to seq_pos; the sequence then ends at the row after the last
- * one written.  Calls on one jx_pkv are ordered on one stream, like those on a
+ * one written, in every layer (an engine that calls layer by layer passes the
+ * same positions for each; a layer that no call wrote holds undefined rows).  Calls on one jx_pkv are ordered on one stream, like those on a
  * jx_kv.  None of them can be captured into a CUDA graph (JX_ERR_UNSUPPORTED):
  * which page a row goes to is decided on the host, call by call. */
 typedef struct jx_pkv jx_pkv;

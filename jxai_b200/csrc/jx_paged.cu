@@ -15,6 +15,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <memory>
 #include <mutex>
 #include <new>
 #include <string>
@@ -749,9 +750,13 @@ int release_upload(jx_pkv::Upload* u, cudaStream_t st) {
 
 int grow_device(void** p, size_t* have, size_t need, const char* what) {
     if (*have >= need) return JX_OK;
-    if (*p) PKV_CUDA(cudaFree(*p));  // (waits for the device)
+    if (*p) {
+        PKV_CUDA(cudaDeviceSynchronize());  // earlier calls may still be reading it
+        PKV_CUDA(cudaFree(*p));
+    }
     *p = nullptr;
     *have = 0;
+    need = (need + (size_t{1} << 20) - 1) >> 20 << 20;
     if (cudaMalloc(p, need) != cudaSuccess) {
         cudaGetLastError();
         return pfail(JX_ERR_NOMEM, "%s of %zu bytes failed", what, need);
@@ -1314,11 +1319,11 @@ int jx_pkv_create(const jx_pkv_desc* desc, jx_pkv** out) {
         PKV_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, d.device));
         PKV_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d.device));
         if (major < 10) return pfail(JX_ERR_UNSUPPORTED, "device %d is older than this build's target, sm_100a", d.device);
-        jx_pkv* kv = new jx_pkv();
-        auto undo = [&](int code) {
-            jx_pkv_destroy(kv);
-            return code;
+        struct Destroy {
+            void operator()(jx_pkv* k) const { jx_pkv_destroy(k); }
         };
+        std::unique_ptr<jx_pkv, Destroy> owner(new jx_pkv());
+        jx_pkv* kv = owner.get();
         kv->d = d;
         kv->num_sms = sms;
         kv->layer_bytes = static_cast<long long>(d.n_kv_heads) * record_bytes(static_cast<int>(d.head_dim));
@@ -1333,23 +1338,23 @@ int jx_pkv_create(const jx_pkv_desc* desc, jx_pkv** out) {
         const size_t tb = static_cast<size_t>(d.n_seqs) * kv->max_pages * sizeof(int);
         if (cudaMalloc(&kv->pool, bytes) != cudaSuccess || cudaMalloc(&kv->d_table, tb) != cudaSuccess) {
             cudaGetLastError();
-            return undo(pfail(JX_ERR_NOMEM, "page pool of %zu bytes failed", bytes));
+            return pfail(JX_ERR_NOMEM, "page pool of %zu bytes failed", bytes);
         }
         const size_t ctas = static_cast<size_t>(sms) * kStepCtasPerSm;
         const size_t part = 2 * ctas * kStepCols * (d.head_dim + 2) * sizeof(float);
         if (cudaMalloc(&kv->d_scratch, part) != cudaSuccess || cudaMalloc(&kv->d_counters, ctas * sizeof(int)) != cudaSuccess ||
             cudaMemset(kv->d_counters, 0, ctas * sizeof(int)) != cudaSuccess) {
             cudaGetLastError();
-            return undo(pfail(JX_ERR_NOMEM, "scratch of %zu bytes failed", part));
+            return pfail(JX_ERR_NOMEM, "scratch of %zu bytes failed", part);
         }
         if (cudaMemset(kv->pool, 0, bytes) != cudaSuccess || cudaMemset(kv->d_table, 0, tb) != cudaSuccess ||
             cudaMalloc(&kv->d_err, sizeof(int)) != cudaSuccess || cudaMemset(kv->d_err, 0, sizeof(int)) != cudaSuccess ||
             cudaMalloc(&kv->d_dbg, 8 * sizeof(int)) != cudaSuccess ||
             cudaMemset(kv->d_dbg, 0, 8 * sizeof(int)) != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) {
             cudaGetLastError();
-            return undo(pfail(JX_ERR_CUDA, "cache initialisation failed"));
+            return pfail(JX_ERR_CUDA, "cache initialisation failed");
         }
-        *out = kv;
+        *out = owner.release();
         return JX_OK;
     });
 }

@@ -179,7 +179,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             for (int x = 0; x < 2; ++x) {
                 WAIT(C::B_QF + x, itc & 1, 53, itc);
-                if (cnt[x] == 0) continue;
+                if (cnt[x] == 0) {
+                    // no rows in this tile: its softmax is let on to the next item (it
+                    // would otherwise run ahead of the barriers' phases)
+                    if (lane == 0) tc_commit(BAR(C::B_SF + x));
+                    __syncwarp();
+                    continue;
+                }
                 // S takes the place of the item before's last P
                 if (pf[x] > 0) WAIT(C::B_PV + x, (pf[x] - 1) & 1, 61, itc);
                 issue_s(x, 0);
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(BAR(C::B_QF + x));
             return exp2_int(-sh);
         };
-        int g = 0;  // tiles of S so far
+        int g = 0, pv = 0;  // phases of S, and of P.V, so far
         float unscale = it_begin < it_end ? stage_q(a.tiles[it_begin]) : 1.0f;
         for (int it = it_begin; it < it_end; ++it) {
             const PrefillTile tl = a.tiles[it];
@@ -311,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float mul2 = mul * kLog2;
             float m = -INFINITY, l = 0.0f;  // the maximum in units of log2
             float behind = 1.0f;            // what the total is to be multiplied by since it was written
-            for (int t = 0; t < nt; ++t, ++g) {
+            for (int t = 0; t < nt; ++t, ++g, ++pv) {
                 if (t > 0 && t % C::DRAIN == 0) {
                     // O of the tiles so far to the total, while S is being computed; 32
                     // dims at a time, the first ones' totals fetched during the wait
@@ -322,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int i = 0; i < 32; ++i) sum[i] = t > C::DRAIN ? __ldcg(total + (c + i) * 128) : 0.0f;
                             if (c == 0) {
-                                WAIT(C::B_PV + x, (g - 1) & 1, 62, g);
+                                WAIT(C::B_PV + x, (pv - 1) & 1, 62, g);
                                 __syncwarp();
                                 tc_fence_after();
                             }
@@ -412,10 +418,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(BAR(C::B_PF + x));
             }
+            if (nt == 0) {
+                WAIT(C::B_SF + x, g & 1, 63, g);
+                ++g;
+            }
             // the next item's Q while the last P.V runs: every S of this one is done
             const float next = it + 1 < it_end ? stage_q(a.tiles[it + 1]) : 1.0f;
             if (nt > 0) {
-                WAIT(C::B_PV + x, (g - 1) & 1, 60, g);
+                WAIT(C::B_PV + x, (pv - 1) & 1, 60, g);
                 __syncwarp();
                 tc_fence_after();
                 const long long io = static_cast<long long>(tl.io0) + static_cast<long long>(tok) * tl.io_step;

@@ -430,6 +430,80 @@ def test_a_serving_run():
             p.check_rows(s)
 
 
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+def test_layer_by_layer(dtype):
+    """One call per layer at the same positions, as an engine runs a token."""
+    import torch
+    H, HK, HD, L = 4, 2, 64, 3
+    p = Pair(H, HK, HD, dtype, n_seqs=2, L=L, cap=128, seed=77)
+    for jobs, prompt in [([(1, 0, 60)], True), ([(1, 60, 1), (0, 0, 1)], False), ([(0, 1, 5)], True),
+                         ([(0, 6, 1), (1, 61, 1)], False)]:
+        n = sum(j[2] for j in jobs)
+        q, k, v = p.inputs(n)
+        seqs = [s for s, a, m in jobs for _ in range(m)]
+        pos = [a + i for s, a, m in jobs for i in range(m)]
+        for l in range(L):
+            wide = [cuda(x[:, l:l + 1]) for x in (q, k, v)]
+            out = torch.empty_like(wide[0])
+            (jx.attn_prefill if prompt else jx.attn_step)(
+                p.cache, [p.layers[l]], *wide, out, pos, H, HK, neox=True, seq_ids=seqs)
+            got, at = out.cpu().numpy()[:, 0], 0
+            for s, a, m in jobs:
+                ref, tol = p.model.step(s, l, a, q[at:at + m, l], k[at:at + m, l], v[at:at + m, l], H,
+                                        p.scale, **p.kw)
+                assert (np.abs(got[at:at + m] - ref) <= tol).all()
+                at += m
+        for s, a, m in jobs:
+            p.model.rows[s] = a + m
+            p.check_rows(s)
+
+
+@pytest.mark.parametrize("tokens", [3, 50])
+def test_more_sequences_than_a_launch_takes(tokens):
+    """Prompts and steps of 131 sequences of unlike lengths, with a window."""
+    p = Pair(2, 1, 64, "int8", n_seqs=131, L=2, cap=64, swa=[False, True], window=20, seed=5)
+    jobs = [(s, 0, tokens + s % 4) for s in range(131)]
+    p.run(jobs, True)
+    p.run([(s, n, 1) for s, _, n in reversed(jobs)], False)
+
+
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+def test_padded_rows_on_the_tensor_cores(dtype):
+    p = Pair(8, 2, 128, dtype, cap=200, seed=15)
+    p.run([(0, 0, 150)], True, pad=4)
+
+
+def test_calls_in_a_row_share_their_buffers():
+    """Prompts of several sizes, keeps and steps queued without a wait between them: lists, widened
+    rows and totals are used in turn."""
+    import torch
+    H, HK, HD = 8, 2, 64
+    caches = [jx.PagedKVCache(2, 2, 600, HK, HD, dtype="int8") for _ in range(2)]
+    layers = [jx.Layer(HD, HD, 1e4, l) for l in range(2)]
+    g = torch.Generator(device="cuda").manual_seed(0)
+    sizes = [300, 64, 500, 65, 600, 130]
+    data = [[torch.randn(n, 2, w, generator=g, device="cuda") for w in (H * HD, HK * HD, HK * HD)] for n in sizes]
+    torch.cuda.synchronize()
+
+    def go(cache, wait):
+        outs = []
+        for i, (n, (q, k, v)) in enumerate(zip(sizes, data)):
+            out = torch.empty_like(q)
+            jx.attn_prefill(cache, layers, q, k, v, out, np.arange(n), H, HK, seq_ids=np.zeros(n, int))
+            cache.fork(0, 1)
+            cache.keep(1, np.arange(i, n, 2))
+            m = cache.seq_pos(1)
+            one = torch.empty_like(q[:1])
+            jx.attn_step(cache, layers, q[:1], k[:1], v[:1], one, [m], H, HK, seq_ids=[1])
+            outs += [out, one, cache.read([1], [0], m + 1)]
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs
+    for a, b in zip(go(caches[0], False), go(caches[1], True)):
+        assert torch.equal(a, b)
+
+
 def refuses(code, fn, *args, **kw):
     with pytest.raises(jx.JxError) as e:
         fn(*args, **kw)

@@ -1,6 +1,7 @@
 """The paged cache's host side where no GPU is needed."""
 import ctypes as C
 import os
+import random
 import subprocess
 import tempfile
 
@@ -88,3 +89,110 @@ def test_integer_lists():
     for bad in (np.zeros(2), np.zeros((2, 2), int), np.array([1 << 31])):
         with pytest.raises(jx.JxError):
             _i32_array(bad)
+
+
+class Bar:
+    """An mbarrier: `count` arrivals complete a phase; a wait names a phase by its parity."""
+
+    def __init__(self):
+        self.phase = 0
+
+    def arrive(self):
+        self.phase += 1
+
+    def passes(self, parity):
+        return (self.phase & 1) != parity
+
+
+def prompt_barriers(items, stages, rng):
+    """The waits and arrivals of jx_paged_prompt.cu's roles for items of (tiles of query tile 0,
+    of tile 1), taken in a random order.  Every wait has to end, and on the phase it means."""
+    full, empty = [[Bar() for _ in range(stages)] for _ in range(2)]
+    q, s, p, pv, o = [[Bar(), Bar()] for _ in range(5)]
+    pipe, copies = [], []  # MMA commits and TMA copies, in order
+
+    def producer():
+        n = 0
+        for c in items:
+            for _ in range(2 * max(c)):
+                if n >= stages:
+                    yield empty[n % stages], ((n // stages) & 1) ^ 1, n // stages
+                copies.append(n % stages)
+                n += 1
+
+    def issuer():
+        n0, done = 0, [0, 0]
+
+        def tile(n):
+            return full[n % stages], (n // stages) & 1, n // stages + 1
+        for i, c in enumerate(items):
+            for x in range(2):
+                yield q[x], i & 1, i + 1
+                if c[x]:
+                    if done[x]:
+                        yield pv[x], (done[x] - 1) & 1, done[x]
+                    yield tile(n0)
+                pipe.append(s[x])
+            if max(c):
+                pipe.append(empty[n0 % stages])
+            for t in range(max(c)):
+                for x in range(2):
+                    if t >= c[x]:
+                        continue
+                    yield p[x], done[x] & 1, done[x] + 1
+                    if t == 0 and i:
+                        yield o[x], (i - 1) & 1, i
+                    yield tile(n0 + 2 * t + 1)
+                    pipe.append(pv[x])
+                    if t + 1 < c[x]:
+                        yield pv[x], done[x] & 1, done[x] + 1
+                        yield tile(n0 + 2 * t + 2)
+                        pipe.append(s[x])
+                    done[x] += 1
+                for k in (1, 2) if t + 1 < max(c) else (1,):
+                    pipe.append(empty[(n0 + 2 * t + k) % stages])
+            n0 += 2 * max(c)
+
+    def softmax(x):
+        g = n = 0
+        q[x].arrive()
+        for i, c in enumerate(items):
+            for t in range(c[x]):
+                if t and t % 4 == 0:
+                    yield pv[x], (n - 1) & 1, n
+                yield s[x], g & 1, g + 1
+                p[x].arrive()
+                g, n = g + 1, n + 1
+            if not c[x]:
+                yield s[x], g & 1, g + 1
+                g += 1
+            if i + 1 < len(items):
+                q[x].arrive()
+            if c[x]:
+                yield pv[x], (n - 1) & 1, n
+            o[x].arrive()
+
+    roles = [producer(), issuer(), softmax(0), softmax(1)]
+    waits = {i: next(r, None) for i, r in enumerate(roles)}
+    while any(waits.values()):
+        ready = [i for i, w in waits.items() if w and w[0].passes(w[1])]
+        acts = ready + ["pipe"] * bool(pipe) + ["copy"] * bool(copies)
+        assert acts, "a wait never ends"
+        act = rng.choice(acts)
+        if act == "pipe":
+            pipe.pop(0).arrive()
+        elif act == "copy":
+            full[copies.pop(0)].arrive()
+        else:
+            assert waits[act][0].phase == waits[act][2], "a wait ends on another phase"
+            waits[act] = next(roles[act], None)
+
+
+def test_prompt_kernel_barriers():
+    rng = random.Random(0)
+    for _ in range(1500):
+        items = []
+        for _ in range(rng.randint(1, 6)):
+            a = rng.randint(1, 9)
+            items.append((a, rng.choice([0, a, a + 1, max(1, a - 1)])))
+        prompt_barriers(items, rng.choice([3, 8]), rng)
