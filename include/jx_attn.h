@@ -338,7 +338,7 @@ JX_API int jx_pkv_attn_prefill(jx_pkv* kv, const jx_layer_desc* layers, uint32_t
 
 /* As jx_kv_check_device_error. */
 JX_API int jx_pkv_check_device_error(jx_pkv* kv, int* code, void* stream);
-/* "wait_limit_ms": as in jx_kv_set_option. */
+/* "wait_limit_ms" and "test_wait_cta" (of a step): as in jx_kv_set_option. */
 JX_API int jx_pkv_set_option(jx_pkv* kv, const char* key, int value);
 /* Kernels the last jx_pkv_attn_step / jx_pkv_attn_prefill launched. */
 JX_API int jx_pkv_last_launch_count(const jx_pkv* kv, int* count);

@@ -538,6 +538,7 @@ struct jx_pkv {
     size_t totals_bytes = 0;
     int num_sms = 0;
     int opt_wait_limit_ms = 0;
+    int opt_test_wait_cta = 0;
     int last_launches = 0;
 };
 
@@ -1164,6 +1165,7 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
     A.err = kv->d_err;
     A.dbg = kv->d_dbg;
     A.wait_limit = wait_limit_cycles(kv->opt_wait_limit_ms);
+    A.test_wait_cta = kv->opt_test_wait_cta;
     A.q_vec = reinterpret_cast<uintptr_t>(a->q) % 16 == 0 && a->q_stride % 4 == 0;
     A.kv_vec = reinterpret_cast<uintptr_t>(a->k) % 16 == 0 && reinterpret_cast<uintptr_t>(a->v) % 16 == 0 &&
                a->kv_stride % 4 == 0;
@@ -1628,9 +1630,13 @@ int jx_pkv_check_device_error(jx_pkv* kv, int* code, void* stream) {
 
 int jx_pkv_set_option(jx_pkv* kv, const char* key, int value) {
     if (!kv || !key) return pfail(JX_ERR_INVALID, "null argument");
+    if (value < 0) return pfail(JX_ERR_INVALID, "%s must not be negative", key);
     if (std::strcmp(key, "wait_limit_ms") == 0) {
-        if (value < 0) return pfail(JX_ERR_INVALID, "wait_limit_ms must not be negative");
         kv->opt_wait_limit_ms = value;
+        return JX_OK;
+    }
+    if (std::strcmp(key, "test_wait_cta") == 0) {
+        kv->opt_test_wait_cta = value;
         return JX_OK;
     }
     return pfail(JX_ERR_INVALID, "unknown option '%s'", key);

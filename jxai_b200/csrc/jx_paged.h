@@ -86,6 +86,7 @@ struct PagedArgs {
     int units0, units1;     // step: units of a segment, over all runs, without and with the window
     int append;             // step: write the run's row, too
     int q_vec, kv_vec;      // 16-byte loads of q / of k and v are possible
+    int test_wait_cta;      // step: CTA + 1 that waits on a barrier nothing arrives at (test hook)
     const float2* rope[kMaxRopeCfgs];  // [capacity][HD/2] (cos, sin)
     float* scratch;
     int* counters;

@@ -49,7 +49,7 @@ struct StepCfg {
     static constexpr bool SPLIT = HD >= 128;
     static constexpr int STAGE = SPLIT ? tile_at(HD, 1) : record_bytes(HD);
     static constexpr int MISC = W * GP * 2 * 4 + 64;  // (m, l) of each warp and column; flags
-    static constexpr int budget = (227 * 1024) / CTAS - 1024 - MISC;
+    static constexpr int budget = (227 * 1024) / CTAS - 1024 - MISC - 8;
     static constexpr int fit = budget / (W * (STAGE + 8));
     static constexpr int NS = fit > 8 ? 8 : fit;  // stages per warp
     // floats of a partial result: o [GP][HD], then (m, l) [GP]; 16-byte aligned
@@ -57,7 +57,7 @@ struct StepCfg {
     static_assert(PART <= kStepCols * (HD + 2), "scratch");
     static constexpr int OFF_MISC = W * NS * STAGE;
     static constexpr int OFF_BAR = OFF_MISC + MISC;
-    static constexpr int SMEM = OFF_BAR + W * NS * 8;
+    static constexpr int SMEM = OFF_BAR + W * NS * 8 + 8;  // (+ the barrier of test_wait_cta)
     static_assert(NS >= (SPLIT ? 3 : 2), "ring");
     static_assert(OFF_BAR % 8 == 0 && OFF_MISC % 16 == 0, "alignment");
     // a warp's part of a finished piece lies in the stage it read last
@@ -555,7 +555,11 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
     unsigned char* ring = smem + warp * NS * C::STAGE;
     const uint32_t ring_u32 = smem_u32(ring);
     const uint32_t bars = smem_u32(smem + C::OFF_BAR) + warp * NS * 8;
-    if (threadIdx.x == 0) *abort_flag = 0;
+    const uint32_t test_bar = smem_u32(smem + C::OFF_BAR) + W * NS * 8;  // nothing ever arrives here
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        mbar_init(test_bar, 1);
+    }
     if (lane == 0) {
         for (int s = 0; s < NS; ++s) mbar_init(bars + 8 * s, 1);
         fence_barrier_init();
@@ -639,6 +643,8 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
             c_par ^= 1u;
         }
     };
+    if (a.test_wait_cta == c + 1 && warp == 0)
+        dead = !__all_sync(0xffffffffu, mbar_wait_bounded(test_bar, 0u, abort_flag, a.err, a.dbg, 42, 0, true, a.wait_limit));
     StepWarp<HD, GP, DT> sw;
     for (; more; more = cw.next(a, p)) {
         if (!p.coop && warp != p.rot) continue;
@@ -682,6 +688,8 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
             }
             if constexpr (C::SPLIT) {
                 advance();
+                __syncwarp();
+                refill(0);  // the K half at once: 131072 rows of the Mistral-7B shape 1.40 -> 1.33 ms
                 wait(c_st, c_par);
             }
             if (!dead) sw.values(smem_u32(vt), lane);

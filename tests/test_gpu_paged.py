@@ -473,6 +473,29 @@ def test_padded_rows_on_the_tensor_cores(dtype):
     p.run([(0, 0, 150)], True, pad=4)
 
 
+@pytest.mark.parametrize("HD", [64, 128])
+def test_a_wait_that_runs_out_is_reported(HD):
+    """A CTA whose wait runs out sets the error word; the kernel ends, and the next step is right."""
+    import torch
+    p = Pair(4, 2, HD, "int8", cap=2000, seed=3)
+    load_prompt(p, 0, p.inputs(1500))
+    q, k, v = p.inputs(1)
+    wide = [cuda(x) for x in (q, k, v)]
+    out = torch.empty_like(wide[0])
+    p.cache.set_option("wait_limit_ms", 20)
+    p.cache.set_option("test_wait_cta", 1)
+    jx.attn_step(p.cache, p.layers, *wide, out, [1500], 4, 2, neox=True)
+    torch.cuda.synchronize()
+    assert p.cache.check_device_error() == 1
+    assert p.cache.check_device_error() == 0
+    p.cache.set_option("test_wait_cta", 0)
+    p.cache.set_option("wait_limit_ms", 0)
+    p.cache.rollback(0, 1488)  # drops the block that step may have written
+    p.model.rows[0] = 1488
+    p.run([(0, 1488, 1)], False)
+    p.run([(0, 1489, 1)], False)
+
+
 def test_calls_in_a_row_share_their_buffers():
     """Prompts of several sizes, keeps and steps queued without a wait between them: lists, widened
     rows and totals are used in turn."""
