@@ -43,8 +43,10 @@ namespace jx {
 template <int HD, int GP>
 struct StepCfg {
     static constexpr int W = 4;  // warps per CTA
-    // Resident CTAs per SM, by the registers their accumulators need.
-    static constexpr int CTAS = HD == 256 ? 2 : (HD == 128 ? 3 : 4);
+    // Resident CTAs per SM, as many as the accumulators' registers allow.  (Groups of
+    // 5 to 8 heads, 131072 rows: head_dim 128 three CTAs with spills 159 us, two
+    // without 131; head_dim 64 four 80, three 73.)
+    static constexpr int CTAS = HD == 256 ? 2 : HD == 128 ? (GP == 8 ? 2 : 3) : HD == 64 && GP == 8 ? 3 : 4;
     // A stage holds a record, or (wide heads) half of one: scales and K, or V.
     static constexpr bool SPLIT = HD >= 128;
     static constexpr int STAGE = SPLIT ? tile_at(HD, 1) : record_bytes(HD);
