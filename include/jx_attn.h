@@ -338,7 +338,10 @@ JX_API int jx_pkv_attn_prefill(jx_pkv* kv, const jx_layer_desc* layers, uint32_t
 
 /* As jx_kv_check_device_error. */
 JX_API int jx_pkv_check_device_error(jx_pkv* kv, int* code, void* stream);
-/* "wait_limit_ms" and "test_wait_cta" (of a step): as in jx_kv_set_option. */
+/* "wait_limit_ms" and "test_wait_cta" (of a step): as in jx_kv_set_option;
+ * "prefill_tc": prompts on the tensor-core kernel where it takes their shape (1),
+ * in the step kernel's blocks (0), or by an estimate of both (-1, the default).
+ * The tensor-core kernel takes K and V beyond 8e6 in magnitude as that large. */
 JX_API int jx_pkv_set_option(jx_pkv* kv, const char* key, int value);
 /* Kernels the last jx_pkv_attn_step / jx_pkv_attn_prefill launched. */
 JX_API int jx_pkv_last_launch_count(const jx_pkv* kv, int* count);

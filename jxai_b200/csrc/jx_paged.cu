@@ -407,11 +407,14 @@ struct WidenArgs {
 static_assert(sizeof(WidenArgs) <= 4096, "kernel parameters");
 
 constexpr int kWidenRows = 64;
+constexpr int kMaxWideExp = 16;
 
 // A code times 2^(k - K), K so that the head's largest block exponent becomes 8:
 // exact in fp16 for blocks down to 2^-32 of the largest scale (below that a
-// value is off by 2^-33 of the largest), and never beyond 448 * 2^7.  The factor
-// 2^K of each head goes to the prompt kernel, which multiplies scores and
+// value is off by 2^-33 of the largest), and never beyond 448 * 2^7.  K is at most
+// 16 - 8: a row that holds infinities (2^62 in the cache) is taken as large as
+// 2^23, so that it cannot wipe out the rows of tokens that do not attend it.  The
+// factor 2^K of each head goes to the prompt kernel, which multiplies scores and
 // outputs by it.  One CTA per (64 rows, layer, kv head); the exponents of the
 // sequence's blocks (16 bytes per page) are read by every one of them.
 template <int HD, int DT>
@@ -436,10 +439,10 @@ __global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ Wide
     int ek = kMinExp, ev = kMinExp;
     for (int p = first + threadIdx.x; p <= last; p += 256) {
         const float4 sc = *reinterpret_cast<const float4*>(base + table[p] * a.page_bytes);
-        // a page's second block may begin behind the sequence's end
-        const bool two = p * kPageRows + kBlockRows < end;
-        ek = max(ek, max(scale_exp(sc.x), two ? scale_exp(sc.y) : kMinExp));
-        ev = max(ev, max(scale_exp(sc.z), two ? scale_exp(sc.w) : kMinExp));
+        // a page's first block may lie before the rows, its second behind them
+        const bool one = p * kPageRows + kBlockRows > lo, two = p * kPageRows + kBlockRows < end;
+        ek = max(ek, max(one ? scale_exp(sc.x) : kMinExp, two ? scale_exp(sc.y) : kMinExp));
+        ev = max(ev, max(one ? scale_exp(sc.z) : kMinExp, two ? scale_exp(sc.w) : kMinExp));
     }
     ek = __reduce_max_sync(0xffffffffu, ek);
     ev = __reduce_max_sync(0xffffffffu, ev);
@@ -452,8 +455,8 @@ __global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ Wide
         ek = max(ek, red[0][w]);
         ev = max(ev, red[1][w]);
     }
-    ek -= kTop;
-    ev -= kTop;
+    ek = min(ek, kMaxWideExp) - kTop;
+    ev = min(ev, kMaxWideExp) - kTop;
     if (blockIdx.x == static_cast<unsigned>(run.off) && threadIdx.x == 0)
         a.head_scale[(static_cast<long long>(s) * a.n_layers + l) * a.n_kv + h] = make_float2(exp2_int(ek), exp2_int(ev));
     constexpr int CPR = HD / 16;
@@ -474,7 +477,8 @@ __global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ Wide
         uint32_t w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const __half2 v = __floats2half2_rn(x[2 * j] * f, x[2 * j + 1] * f);
+            const __half2 v = __floats2half2_rn(fminf(fmaxf(x[2 * j] * f, -65504.0f), 65504.0f),
+                                                fminf(fmaxf(x[2 * j + 1] * f, -65504.0f), 65504.0f));
             w[j] = *reinterpret_cast<const uint32_t*>(&v);
         }
         dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -539,6 +543,7 @@ struct jx_pkv {
     int num_sms = 0;
     int opt_wait_limit_ms = 0;
     int opt_test_wait_cta = 0;
+    int opt_prefill_tc = -1;              // prompts on the tensor cores: 1 / 0, -1: by estimate
     int last_launches = 0;
 };
 
@@ -840,8 +845,6 @@ int step_rows(jx_pkv* kv, PagedArgs& A, const std::vector<PagedLayer>& part, con
     return JX_OK;
 }
 
-// Tokens of a sequence from which on a prompt goes to the tensor-core kernel.
-constexpr int kPromptTokens = 48;
 // fp16 rows held at one time.  A group of layers grows until its rows would
 // leave L2 (126 MB) before they are read, but not before its work items give
 // every CTA several; never beyond the second figure.
@@ -850,6 +853,39 @@ constexpr size_t kItemsPerCta = 8;
 // K/V streams (one kv head of a layer and sequence) that CTAs read at one time
 // where a group's rows exceed L2: as many as fit this.
 constexpr size_t kStreamL2 = size_t{32} << 20;
+
+// Whether a prompt goes to the tensor-core kernel or, in blocks of tokens, to the
+// step kernel: by what each takes, in microseconds.  The step kernel reads a
+// sequence's pages once per block, spread over all SMs (0.0135 ns per head_dim
+// element and unit); the prompt kernel walks the tiles of an item one by one on
+// one SM (3.4 us per 128 rows at head_dim 64, 4.6 at 128), after bringing the rows
+// to fp16.  Measured, one layer of 8 kv heads and 4 heads each, blocks / tensor
+// cores: head_dim 64, 256 tokens 35 / 32 us, behind 8192 rows 242 / 240 us, 64
+// tokens behind them 74 / 235 us; head_dim 128, 96 tokens behind 8192 rows 193 /
+// 310 us, 256 tokens 480 / 316 us.
+bool prompt_on_tensor_cores(const jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all,
+                            const std::vector<PagedRun>& runs) {
+    const int hd = static_cast<int>(kv->d.head_dim), nq = kStepCols / A.G, TQ = 2 * kPromptRows / A.G;
+    double windowed = 0.0;
+    for (const PagedLayer& L : all) windowed += (L.flags & kLayerWindow) ? 1.0 : 0.0;
+    const double full = static_cast<double>(all.size()) - windowed;
+    double units = 0.0, tiles = 0.0, longest = 0.0, rows = 0.0;
+    for (const PagedRun& r : runs) {
+        const double end = r.pos0 + r.n, mid = r.pos0 + 0.5 * r.n, win = A.window;
+        const double blocks = (r.n + nq - 1) / nq, items = (r.n + TQ - 1) / TQ;
+        units += blocks * (full * (mid / kPageRows + 1 + kPieceCost) +
+                           windowed * (std::min(mid, win) / kPageRows + 2 + kPieceCost));
+        tiles += items * (full * (mid / kPromptRows + 1) + windowed * ((std::min(mid, win) + TQ) / kPromptRows + 1));
+        longest = std::max(longest, (full > 0 ? end : std::min(end, win + TQ)) / kPromptRows + 1);
+        rows += full * end + windowed * std::min(end, win + r.n);
+    }
+    units *= A.n_kv;
+    tiles *= A.n_kv;
+    const double by_blocks = 12.0 + units * hd * 1.35e-5;
+    const double by_tiles = 18.0 + rows * A.n_kv * hd * 6 / 5e6 +
+                            std::max(longest, tiles / std::max(kv->num_sms, 1)) * (hd == 64 ? 3.4 : 4.6);
+    return by_tiles < by_blocks;
+}
 
 // Prompt attention on the tensor cores: the rows of a group of layers are
 // brought to fp16 (see widen_kernel), then paged_prompt_kernel runs over them.  Its work items are laid out for its persistent
@@ -1183,7 +1219,7 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
         // then attention: on the tensor cores, or (few tokens, or a shape that kernel
         // does not take) for blocks of as many tokens as fill the step kernel's columns
         if (paged_prompt_supported(static_cast<int>(D.head_dim), static_cast<int>(G)) && out_vec && a->scale > 0.0f &&
-            a->n_seqs >= kPromptTokens * runs.size()) {
+            (kv->opt_prefill_tc < 0 ? prompt_on_tensor_cores(kv, A, all, runs) : kv->opt_prefill_tc > 0)) {
             if (int rc = prompt_tc(kv, A, all, runs, st, &launches)) return rc;
             kv->last_launches = launches;
             return JX_OK;
@@ -1630,6 +1666,11 @@ int jx_pkv_check_device_error(jx_pkv* kv, int* code, void* stream) {
 
 int jx_pkv_set_option(jx_pkv* kv, const char* key, int value) {
     if (!kv || !key) return pfail(JX_ERR_INVALID, "null argument");
+    if (std::strcmp(key, "prefill_tc") == 0) {
+        if (value < -1 || value > 1) return pfail(JX_ERR_INVALID, "prefill_tc must be 1, 0 or -1");
+        kv->opt_prefill_tc = value;
+        return JX_OK;
+    }
     if (value < 0) return pfail(JX_ERR_INVALID, "%s must not be negative", key);
     if (std::strcmp(key, "wait_limit_ms") == 0) {
         kv->opt_wait_limit_ms = value;

@@ -20,10 +20,10 @@
 //    shared memory, which Q (two parts, both tiles) and the ring fill.
 //  * A tile's next S overwrites its P: it is issued once that P.V has completed,
 //    while the other tile's work is in the queue.
-//  * The running maximum moves only when a tile exceeds it by 2^8 (O is then
-//    rescaled in TMEM, its P.V known complete from the S that follows it); a
-//    weight of 1 is 2^7 in fp16, so weights reach 2^15 and the fp16 floor lies
-//    2^-32 below 1.
+//  * Weights are taken against a reference 2^7 below the largest score when it is
+//    set, and it moves only when a weight would exceed 2^15 (fp16 ends at 2^16; its
+//    floor then lies 2^-32 below the largest weight).  O is then rescaled in TMEM,
+//    its P.V known complete from the S that follows it.
 //  * The tensor cores cut the sum they add to towards zero (about 1e-8 of it per
 //    MMA of 16 rows), which over thousands of rows adds up to 1e-5.  So O sums
 //    a few tiles, then the softmax threads add it to an fp32 total of their own
@@ -40,6 +40,7 @@ namespace {
 
 constexpr int kThreads = 32 * 18;
 constexpr float kLog2 = 1.4426950408889634f;
+constexpr float kFar = 1048576.0f;  // scores beyond: a difference of a few is no longer exact
 
 
 template <int HD>
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                        a.scale_heads + tl.kvh);
             const float mul = a.scale * unscale * hs.x;  // raw S -> score
             const float mul2 = mul * kLog2;
-            float m = -INFINITY, l = 0.0f;  // the maximum in units of log2
+            float m = -INFINITY, l = 0.0f;  // what weights are taken against (in units of log2)
             float behind = 1.0f;            // what the total is to be multiplied by since it was written
             for (int t = 0; t < nt; ++t, ++g, ++pv) {
                 if (t > 0 && t % C::DRAIN == 0) {
@@ -368,13 +369,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mt = fmaxf(mt, swap(mt, false, false));  // both have read their scores, too
                 // the score's soft cap is monotone: the capped maximum is the maximum's cap
                 mt = capped ? (mt == -INFINITY ? mt : a.cap_out * tanhf(mt * mul2 * a.cap_in)) : mt * mul2;
-                const bool move = mt > m + 8.0f || (m == -INFINITY && mt > -INFINITY);
+                const bool move = mt - m > 15.0f;  // (an empty m is -inf, an empty tile's maximum, too)
                 if (__any_sync(0xffffffffu, move)) {
-                    const float f = !move ? 1.0f : (m == -INFINITY ? 0.0f : ex2_approx(m - mt));
+                    const float ref = mt - (fabsf(mt) > kFar ? 0.0f : 7.0f);
+                    const float f = !move ? 1.0f : (m == -INFINITY ? 0.0f : ex2_approx(m - ref));
                     if (move) {
                         l *= f;
                         behind *= f;
-                        m = mt;
+                        m = ref;
                     }
                     // this S was issued after the P.V before it had completed
                     if (t % C::DRAIN != 0) {
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                const float add = m == -INFINITY ? 0.0f : 7.0f - m;
+                const float add = m == -INFINITY ? 0.0f : -m;
                 float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 if (capped) {
                     // (masked scores stay -inf: their weight is 0)
@@ -397,7 +399,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (s[i] != 0xFF800000u)
                             s[i] = __float_as_uint(a.cap_out * tanhf(__uint_as_float(s[i]) * mul2 * a.cap_in));
                 }
-                const float k = capped ? 1.0f : mul2;
+                // The fused product below is exact where m is a rounded number: far from
+                // zero the difference could leave fp16's range, so such scores are
+                // rounded first, as m was.
+                const bool far = !capped && __any_sync(0xffffffffu, fabsf(m) > kFar && m > -INFINITY);
+                if (far) {
+#pragma unroll
+                    for (int i = 0; i < SW; ++i) s[i] = __float_as_uint(__fmul_rn(__uint_as_float(s[i]), mul2));
+                }
+                const float k = capped || far ? 1.0f : mul2;
 #pragma unroll
                 for (int c = 0; c < SW; c += 32) {
                     uint32_t hw[16], lw[16];

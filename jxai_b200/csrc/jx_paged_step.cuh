@@ -175,8 +175,10 @@ template <int HD, int GP, int DT>
 struct StepWarp {
     static constexpr int NBC = (2 * GP + 7) / 8;  // column blocks: (part, head) pairs
     static constexpr int KS = HD / 16;
-    static constexpr int kBase = 10;              // a weight of 1 is 2^10 in fp16 (at most 2^15)
-    static constexpr float kLazy = 5.0f;          // the maximum moves when exceeded by 2^5
+    // Weights are taken against a reference m, 2^10 below the largest when it is set
+    // and moved when a weight would exceed 2^15 (fp16 ends at 2^16).  Beyond 2^20 it
+    // is the largest itself: 10 is no longer exact next to it.
+    static constexpr float kBase = 10.0f, kTop = 15.0f, kFar = 1048576.0f;
 
     uint32_t qf[KS][NBC][2];
     float o[KS][NBC][4];
@@ -345,12 +347,13 @@ struct StepWarp {
             mt[j] = fmaxf(mt[j], __shfl_xor_sync(0xffffffffu, mt[j], 4));
             mt[j] = fmaxf(mt[j], __shfl_xor_sync(0xffffffffu, mt[j], 8));
             mt[j] = fmaxf(mt[j], __shfl_xor_sync(0xffffffffu, mt[j], 16));
-            move = move || mt[j] > m[j] + kLazy || (m[j] == -INFINITY && mt[j] > -INFINITY);
+            move = move || mt[j] - m[j] > kTop;  // (an empty m is -inf, an empty page's maximum, too)
         }
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const float mn = fmaxf(m[j], mt[j]);
+                const float to = mt[j] - (fabsf(mt[j]) > kFar ? 0.0f : kBase);
+                const float mn = mt[j] > -INFINITY ? fmaxf(m[j], to) : m[j];
                 const float f = m[j] == -INFINITY ? 0.0f : ex2_approx(m[j] - mn);
                 m[j] = mn;
                 l[j] *= f;
@@ -365,7 +368,7 @@ struct StepWarp {
         }
         float mb[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) mb[j] = m[j] == -INFINITY ? 0.0f : static_cast<float>(kBase) - m[j];
+        for (int j = 0; j < 2; ++j) mb[j] = m[j] == -INFINITY ? 0.0f : -m[j];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             float pr[4];

@@ -23,6 +23,7 @@ class Pair:
     def __init__(self, H, HK, HD, dtype, n_seqs=1, L=1, cap=256, n_pages=None, seed=0, **kw):
         self.H, self.HK, self.HD, self.L = H, HK, HD, L
         self.cache = jx.PagedKVCache(n_seqs, L, cap, HK, HD, n_pages=n_pages, dtype=dtype)
+        self.cache.set_option("prefill_tc", kw.get("tc", 1))
         self.model = Model(n_seqs, L, cap, HK, HD, dtype)
         self.rng = np.random.default_rng(seed)
         self.kw = dict(rope_dim=kw.get("rope_dim", HD), base=kw.get("base", 1e4), neox=kw.get("neox", True))
@@ -96,10 +97,11 @@ SHAPES = [(4, 1, 64), (14, 2, 64), (8, 8, 64), (8, 1, 128), (6, 2, 128), (4, 2, 
           (8, 1, 256), (8, 4, 32), (5, 1, 32)]
 
 
+@pytest.mark.parametrize("tc", [0, 1])
 @pytest.mark.parametrize("dtype", ["int8", "e4m3"])
 @pytest.mark.parametrize("H,HK,HD", SHAPES)
-def test_steps_after_a_prompt(H, HK, HD, dtype):
-    p = Pair(H, HK, HD, dtype, n_seqs=2, cap=160, seed=H * HD)
+def test_steps_after_a_prompt(H, HK, HD, dtype, tc):
+    p = Pair(H, HK, HD, dtype, n_seqs=2, cap=160, seed=H * HD, tc=tc)
     p.run([(1, 0, 37)], True)
     p.run([(0, 0, 1), (1, 37, 1)], False)
     p.run([(1, 38, 1), (0, 1, 1)], False, spread=3.0)
@@ -107,10 +109,11 @@ def test_steps_after_a_prompt(H, HK, HD, dtype):
     p.run([(0, 16, 1), (1, 109, 1)], False)
 
 
+@pytest.mark.parametrize("tc", [0, 1])
 @pytest.mark.parametrize("dtype", ["int8", "e4m3"])
 @pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200])
-def test_prompt_lengths(n, dtype):
-    p = Pair(4, 1, 64, dtype, cap=256, seed=n)
+def test_prompt_lengths(n, dtype, tc):
+    p = Pair(4, 1, 64, dtype, cap=256, seed=n, tc=tc)
     p.run([(0, 0, n)], True)
     p.run([(0, n, 1)], False)
 
@@ -149,11 +152,12 @@ def load_prompt(p, s, x):
     p.check_rows(s)
 
 
+@pytest.mark.parametrize("tc", [0, 1])
 @pytest.mark.parametrize("dtype", ["int8", "e4m3"])
 @pytest.mark.parametrize("HD,G", [(64, 4), (128, 2), (256, 4), (32, 3)])
-def test_window_softcap_and_shared_layers(HD, G, dtype):
+def test_window_softcap_and_shared_layers(HD, G, dtype, tc):
     p = Pair(G * 2, 2, HD, dtype, L=4, cap=300, swa=[True, False, True, False], window=40,
-             softcap=20.0, shares={2: 0, 3: 1}, neox=False, rope_dim=HD // 2, seed=HD)
+             softcap=20.0, shares={2: 0, 3: 1}, neox=False, rope_dim=HD // 2, seed=HD, tc=tc)
     p.run([(0, 0, 150)], True)
     p.run([(0, 150, 1)], False)
     p.run([(0, 151, 20)], True)
@@ -212,33 +216,73 @@ def test_scales_grow_row_by_row(dtype):
         at += n
 
 
-def test_extreme_values():
+@pytest.mark.parametrize("tc", [0, 1])
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+def test_extreme_values(dtype, tc):
     """NaN counts as 0, infinities and magnitudes over 2^62 as 2^62, tiny values and zeros stay in
-    the format; a block that holds them does not reach the rows that are masked or of other blocks."""
+    the format; what attends them is finite."""
+    import torch
+    from tests.paged_model import rotate
+    p = Pair(2, 1, 64, dtype, cap=128, seed=3, tc=tc)
+    q, k, v = p.inputs(40)
+    k[0, 0, :8] = [np.nan, np.inf, -np.inf, 0, 1e30, -1e-40, 1e-30, 3e38]
+    v[1, 0, :8] = [np.nan, np.inf, -np.inf, 0, 1e30, -1e-40, 1e-30, 3e38]
+    k[16:32] = 0.0
+    v[16:32] = 0.0
+    q[0:16] = 0.0
+    wide = [cuda(x) for x in (q, k, v)]
+    out = torch.zeros_like(wide[0])
+    jx.attn_prefill(p.cache, p.layers, *wide, out, list(range(40)), 2, 1, neox=True)
+    p.model.write(0, 0, 0, 0, rotate(k[:, 0].reshape(40, 1, 64), np.arange(40), **p.kw))
+    p.model.write(0, 0, 1, 0, v[:, 0].reshape(40, 1, 64))
+    p.model.rows[0] = 40
+    p.check_rows(0)
+    assert np.isfinite(out.cpu().numpy()).all()
+
+
+@pytest.mark.parametrize("tc", [0, 1])
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e12])
+def test_scores_far_from_zero(size, tc):
+    """Scores of any size: the softmax becomes a choice of the largest, and stays a softmax where
+    two are equal."""
+    p = Pair(2, 1, 64, "int8", cap=300, seed=8, tc=tc)
+    q, k, v = p.inputs(200)
+    k[:] = k[:1] * 0.25                # equal keys but for the position's rotation
+    p.layers[0].rope_dim = 0           # none: all scores of a query are equal
+    p.kw = dict(p.kw, rope_dim=0)
+    q = (q * size).astype(np.float32)
+    p.run([(0, 0, 200)], True, inputs=[q, k, v])
+    p.run([(0, 200, 1)], False, inputs=[q[:1], k[:1], v[:1]])
+
+
+@pytest.mark.parametrize("tc", [0, 1])
+def test_later_rows_do_not_reach_earlier_ones(tc):
+    """A token whose key and value are infinite or NaN: the tokens before it are right."""
+    import torch
     for dtype in ("int8", "e4m3"):
-        p = Pair(2, 1, 64, dtype, cap=128, seed=3)
-        q, k, v = p.inputs(40)
-        k[0, 0, :8] = [np.nan, np.inf, -np.inf, 0, 1e30, -1e-40, 1e-30, 3e38]
-        v[1, 0, :8] = [np.nan, np.inf, -np.inf, 0, 1e30, -1e-40, 1e-30, 3e38]
-        k[16:32] = 0.0
-        v[16:32] = 0.0
-        q[0:16] = 0.0
-        for s in range(1):
-            import torch
-            wide = [cuda(x) for x in (q, k, v)]
-            out = torch.zeros_like(wide[0])
-            jx.attn_prefill(p.cache, p.layers, *wide, out, list(range(40)), 2, 1, neox=True)
-            from tests.paged_model import rotate
-            p.model.write(0, 0, 0, 0, rotate(k[:, 0].reshape(40, 1, 64), np.arange(40), **p.kw))
-            p.model.write(0, 0, 1, 0, v[:, 0].reshape(40, 1, 64))
-            p.model.rows[0] = 40
-            p.check_rows(0)
-            assert np.isfinite(out.cpu().numpy()).all()
+        p, ok = (Pair(4, 1, 64, dtype, cap=256, seed=14, tc=tc) for _ in range(2))
+        q, k, v = p.inputs(200)
+        ok.run([(0, 0, 200)], True, inputs=(q, k, v))
+        bad_k, bad_v = k.copy(), v.copy()
+        bad_k[150], bad_v[150] = np.inf, -np.inf
+        bad_k[170], bad_v[171] = np.nan, np.nan
+        outs = []
+        for pair, kv in ((p, (bad_k, bad_v)), (ok, (k, v))):
+            pair.cache.clear(0)
+            wide = [cuda(x) for x in (q, *kv)]
+            out = torch.empty_like(wide[0])
+            jx.attn_prefill(pair.cache, pair.layers, *wide, out, list(range(200)), 4, 1, neox=True)
+            outs.append(out.cpu().numpy())
+        # rows before the block that holds the token: the same, but for the exponent the
+        # sums are taken against
+        assert np.abs(outs[0][:144] - outs[1][:144]).max() <= 2.0 ** -18 * np.abs(v).max()
+        assert np.isfinite(outs[0]).all()
 
 
-def test_rows_behind_a_window_do_not_reach_it():
+@pytest.mark.parametrize("tc", [0, 1])
+def test_rows_behind_a_window_do_not_reach_it(tc):
     """Rows with infinities and NaN in front of a sliding window leave its output alone."""
-    p = Pair(4, 1, 64, "e4m3", cap=128, swa=[True], window=16, seed=4)
+    p = Pair(4, 1, 64, "e4m3", cap=128, swa=[True], window=16, seed=4, tc=tc)
     x = p.inputs(64)
     x[1][:48], x[2][:48] = np.inf, np.nan
     load_prompt(p, 0, x)
@@ -409,7 +453,7 @@ def test_a_serving_run():
     their own."""
     import torch
     p = Pair(8, 2, 64, "int8", n_seqs=3, L=3, cap=256, n_pages=20, swa=[True, False, True],
-             window=48, seed=21)
+             window=48, seed=21, tc=-1)
     st = torch.cuda.Stream()
     with torch.cuda.stream(st):
         p.run([(0, 0, 61), (2, 0, 90)], True)
@@ -458,10 +502,10 @@ def test_layer_by_layer(dtype):
             p.check_rows(s)
 
 
-@pytest.mark.parametrize("tokens", [3, 50])
-def test_more_sequences_than_a_launch_takes(tokens):
+@pytest.mark.parametrize("tokens,tc", [(3, 0), (3, 1), (50, 1)])
+def test_more_sequences_than_a_launch_takes(tokens, tc):
     """Prompts and steps of 131 sequences of unlike lengths, with a window."""
-    p = Pair(2, 1, 64, "int8", n_seqs=131, L=2, cap=64, swa=[False, True], window=20, seed=5)
+    p = Pair(2, 1, 64, "int8", n_seqs=131, L=2, cap=64, swa=[False, True], window=20, seed=5, tc=tc)
     jobs = [(s, 0, tokens + s % 4) for s in range(131)]
     p.run(jobs, True)
     p.run([(s, n, 1) for s, _, n in reversed(jobs)], False)
@@ -502,6 +546,8 @@ def test_calls_in_a_row_share_their_buffers():
     import torch
     H, HK, HD = 8, 2, 64
     caches = [jx.PagedKVCache(2, 2, 600, HK, HD, dtype="int8") for _ in range(2)]
+    for c in caches:
+        c.set_option("prefill_tc", 1)
     layers = [jx.Layer(HD, HD, 1e4, l) for l in range(2)]
     g = torch.Generator(device="cuda").manual_seed(0)
     sizes = [300, 64, 500, 65, 600, 130]
@@ -564,6 +610,9 @@ def test_refusals():
     refuses(_lib.JX_ERR_NOMEM, step, list(range(40)), seqs=[1] * 40, call=jx.attn_prefill)
     assert p.cache.seq_pos(1) == 0 and p.cache.free_pages == 1
     refuses(_lib.JX_ERR_RANGE, p.cache.set_seq_pos, 0, 41)
+    refuses(_lib.JX_ERR_INVALID, p.cache.set_option, "prefill_tc", 2)
+    refuses(_lib.JX_ERR_INVALID, p.cache.set_option, "wait_limit_ms", -1)
+    refuses(_lib.JX_ERR_INVALID, p.cache.set_option, "no_such_option", 1)
     refuses(_lib.JX_ERR_INVALID, p.cache.fork, 0, 0)
     refuses(_lib.JX_ERR_RANGE, p.cache.fork, 0, 1, 41)
     refuses(_lib.JX_ERR_NOMEM, p.cache.copy, 0, 1)
