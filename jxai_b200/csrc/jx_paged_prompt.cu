@@ -392,20 +392,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const float add = m == -INFINITY ? 0.0f : -m;
                 float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (capped) {
-                    // (masked scores stay -inf: their weight is 0)
-#pragma unroll
-                    for (int i = 0; i < SW; ++i)
-                        if (s[i] != 0xFF800000u)
-                            s[i] = __float_as_uint(a.cap_out * tanhf(__uint_as_float(s[i]) * mul2 * a.cap_in));
-                }
                 // The fused product below is exact where m is a rounded number: far from
                 // zero the difference could leave fp16's range, so such scores are
                 // rounded first, as m was.
-                const bool far = !capped && __any_sync(0xffffffffu, fabsf(m) > kFar && m > -INFINITY);
-                if (far) {
+                const bool far = __any_sync(0xffffffffu, fabsf(m) > kFar && m > -INFINITY);
+                if (capped || far) {
 #pragma unroll
-                    for (int i = 0; i < SW; ++i) s[i] = __float_as_uint(__fmul_rn(__uint_as_float(s[i]), mul2));
+                    for (int i = 0; i < SW; ++i) {
+                        float v = __fmul_rn(__uint_as_float(s[i]), mul2);
+                        if (capped) v = v == -INFINITY ? v : a.cap_out * tanhf(v * a.cap_in);
+                        s[i] = __float_as_uint(v);
+                    }
                 }
                 const float k = capped || far ? 1.0f : mul2;
 #pragma unroll
