@@ -15,6 +15,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <map>
 #include <memory>
 #include <mutex>
 #include <new>
@@ -632,10 +633,20 @@ struct Span {  // rows [begin, end) of a sequence that a call writes
 // (the page is shared by a fork: the writer gets its own).  All or nothing.
 int make_room(jx_pkv* kv, const std::vector<Span>& spans, cudaStream_t st) {
     size_t need = 0;
+    std::map<int, int> left;  // holders of a shared page after those before have their own
     for (const Span& s : spans) {
         const auto& pg = kv->pages[s.seq];
-        for (uint32_t i = s.begin / kPageRows; i < pages_for(s.end); ++i)
-            if (i >= pg.size() || kv->refs[pg[i]] > 1) ++need;
+        for (uint32_t i = s.begin / kPageRows; i < pages_for(s.end); ++i) {
+            if (i >= pg.size()) {
+                ++need;
+            } else if (kv->refs[pg[i]] > 1) {
+                int& holders = left.emplace(pg[i], kv->refs[pg[i]]).first->second;
+                if (holders > 1) {
+                    ++need;
+                    --holders;
+                }
+            }
+        }
     }
     if (need > kv->free_pages.size())
         return pfail(JX_ERR_NOMEM, "%zu pages are needed, %zu of %u are free", need,

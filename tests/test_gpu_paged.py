@@ -341,6 +341,17 @@ def test_fork_writes_do_not_meet(dtype):
     assert p.cache.free_pages == p.cache.n_pages
 
 
+def test_a_page_shared_by_all_writers_of_a_call():
+    """The last holder of a shared page keeps it: two writers need one free page."""
+    p = Pair(2, 1, 32, "int8", n_seqs=2, cap=64, n_pages=2)
+    p.run([(0, 0, 20)], True)
+    p.cache.fork(0, 1)
+    p.model.fork(0, 1)
+    p.run([(0, 20, 1), (1, 20, 1)], False)
+    assert p.cache.free_pages == 0
+    p.check_rows(0)
+
+
 def test_a_fork_onto_its_own_fork():
     p = Pair(2, 1, 32, "int8", n_seqs=2, cap=96, n_pages=4)
     p.run([(0, 0, 70)], True)
