@@ -118,13 +118,16 @@ class PagedKVCache:
         check(self.lib.jx_pkv_compact(self.handle, seq, keep_recent, _stream_ptr(stream, self.device)))
 
     # contents ---------------------------------------------------------------
-    def _tensor(self, t, name: str, shape, dtypes):
+    def _tensor(self, t, name: str, shape, dtypes, stream):
         import torch
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise JxError(-1, f"{name} must be a CUDA tensor")
         if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes:
             raise JxError(-1, f"{name} must be {tuple(shape)} of {dtypes[0]}, got {tuple(t.shape)} "
                               f"of {t.dtype}")
+        if stream is not None and not t.is_contiguous():
+            # the copy would be made on torch's current stream
+            raise JxError(-1, f"{name} must be contiguous where a stream is given")
         return t.contiguous()
 
     def load(self, seq: int, row0: int, k_codes, k_scales, v_codes, v_scales, stream=None) -> None:
@@ -136,10 +139,10 @@ class PagedKVCache:
         kinds = (torch.int8 if self.dtype == JX_I8 else torch.float8_e4m3fn, torch.uint8)
         codes = (self.n_layers, n, self.n_kv_heads, self.head_dim)
         scales = (self.n_layers, -(-n // self.BLOCK), self.n_kv_heads)
-        keep = [self._tensor(k_codes, "k_codes", codes, kinds),
-                self._tensor(k_scales, "k_scales", scales, (torch.float32,)),
-                self._tensor(v_codes, "v_codes", codes, kinds),
-                self._tensor(v_scales, "v_scales", scales, (torch.float32,))]
+        keep = [self._tensor(k_codes, "k_codes", codes, kinds, stream),
+                self._tensor(k_scales, "k_scales", scales, (torch.float32,), stream),
+                self._tensor(v_codes, "v_codes", codes, kinds, stream),
+                self._tensor(v_scales, "v_scales", scales, (torch.float32,), stream)]
         check(self.lib.jx_pkv_load_rows(self.handle, seq, row0, n, *(t.data_ptr() for t in keep),
                                         _stream_ptr(stream, self.device)))
 
@@ -147,7 +150,7 @@ class PagedKVCache:
              stream=None):
         """Values of rows [row0[i], row0[i] + n_rows) of each listed sequence: a tensor [len(seqs),
         n_layers, 2, n_rows, n_kv_heads, head_dim] (K, then V) of bfloat16 (default) or float32;
-        both hold every value exactly."""
+        both hold every value exactly.  With `stream`, `out` has to be given."""
         import torch
         ids, first = _i32_array(seqs), _i32_array(row0)
         if len(ids) != len(first):
@@ -156,6 +159,8 @@ class PagedKVCache:
         if dtype not in (None, torch.bfloat16, torch.float32):
             raise JxError(-1, "rows are read as bfloat16 or float32")
         if out is None:
+            if stream is not None:
+                raise JxError(-1, "read: give out where a stream is given")
             out = torch.empty(shape, dtype=dtype or torch.bfloat16,
                               device=torch.device("cuda", self.device))
         elif (not out.is_cuda or tuple(out.shape) != shape or not out.is_contiguous()

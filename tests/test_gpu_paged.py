@@ -352,6 +352,22 @@ def test_a_page_shared_by_all_writers_of_a_call():
     p.check_rows(0)
 
 
+def test_streams_and_tensors():
+    import torch
+    cache = jx.PagedKVCache(1, 1, 64, 1, 32, dtype="int8")
+    st = torch.cuda.Stream()
+    codes = torch.randint(-127, 128, (1, 2 * 40, 1, 32), dtype=torch.int8, device="cuda")
+    scales = torch.ones(1, 3, 1, device="cuda")
+    refuses(_lib.JX_ERR_INVALID, cache.load, 0, 0, codes[:, ::2], scales, codes[:, 1::2], scales, stream=st)
+    cache.load(0, 0, codes[:, ::2], scales, codes[:, 1::2], scales)
+    refuses(_lib.JX_ERR_INVALID, cache.read, [0], [0], 40, stream=st)
+    out = torch.empty(1, 1, 2, 40, 1, 32, device="cuda")
+    torch.cuda.synchronize()
+    cache.read([0], [0], 40, out=out, stream=st)
+    st.synchronize()
+    assert torch.equal(out[0, 0, 0], codes[0, ::2].float()) and torch.equal(out[0, 0, 1], codes[0, 1::2].float())
+
+
 def test_a_fork_onto_its_own_fork():
     p = Pair(2, 1, 32, "int8", n_seqs=2, cap=96, n_pages=4)
     p.run([(0, 0, 70)], True)
