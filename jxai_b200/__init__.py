@@ -3,7 +3,8 @@
 The path: RoPE on q/k, append of k/v into the per-layer KV cache, and
 grouped-query decode attention over every cached position
 (jacxishipping/jxai src/transformer.cpp:2497-2567), run as one fused CUDA
-launch per step from libjxattn.so (C ABI: include/jx_attn.h).
+launch per step from libjxattn.so (C ABI: include/jx_attn.h).  PagedKVCache holds
+the rows in 8 bits, in pages that sequences share.
 """
 from ._lib import (JX_BF16, JX_E4M3, JX_F16_TRUNC, JX_F32, JX_I8, JxError, EXPORTS, load as load_library,
                    lib_path)

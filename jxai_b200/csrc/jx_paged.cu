@@ -4,8 +4,9 @@
 // Pages, their reference counts and the page table live on the host; a device
 // copy of the table ([n_seqs][max_pages]) is brought up to date by small kernels
 // on the caller's stream.  A launch's plan (which sequences, positions and
-// layers) travels in the kernel's parameters: nothing is uploaded, and no buffer
-// has to outlive the call.
+// layers) travels in the kernel's parameters; only the work items of a
+// tensor-core prompt and the row list of a keep are uploaded, from two buffers
+// that are used in turn.
 #include "jx_paged.h"
 
 #include <cudaTypedefs.h>
@@ -105,7 +106,8 @@ struct PageCopies {
 static_assert(sizeof(PageCopies) <= 4096, "kernel parameters");
 
 // Whole pages, 16 bytes per thread and turn: a page is one contiguous run, so
-// this is a plain copy at memory speed whatever the layers and heads are.
+// this is a plain copy whatever the layers and heads are (67 MB and back: 24 us =
+// 5.6 TB/s; the call with its table entries 38 us).
 __global__ void page_copy_kernel(const __grid_constant__ PageCopies c) {
     const long long n16 = c.page_bytes / 16;
     for (int p = blockIdx.y; p < c.n; p += gridDim.y) {
@@ -154,7 +156,9 @@ __device__ __forceinline__ float half_max(float v, float* red, int n) {
 // Rows of a call written to the cache.  One CTA per (block of 16 rows, layer,
 // kv head): its first half takes K, its second V, one thread per 16 values of
 // a row.  The block's largest magnitude gives the scale; rows that were in the
-// block before the call are re-rounded where the scale grows.
+// block before the call are re-rounded where the scale grows.  Reads 4 bytes and
+// writes 1 per element: 2048 tokens of four Llama-3.2-1B-shaped layers (42 MB) in
+// 15 us (16-byte loads; with scalar ones 41).
 template <int HD, int DT>
 __global__ void __launch_bounds__(2 * HD) append_kernel(const __grid_constant__ PagedArgs a) {
     constexpr int CPR = HD / 16;  // threads per row
@@ -229,7 +233,10 @@ constexpr int kKeepRecords = 4;  // records of a block that a CTA moves together
 // row lies is looked up once for all records, and their loads are in flight
 // together: a block alone is 8 KB behind three dependent loads.  Row i of the
 // result comes from a row >= i, and a CTA reads all of a block before it writes
-// it: in place (serial) no row is overwritten before it has been read.
+// it: in place (serial) no row is overwritten before it has been read.  5000 of
+// 16384 rows, 16 Mistral-7B-shaped layers (328 MB both ways): 77 us = 4.3 TB/s (one
+// record at a time and conversion instructions: 126); the call 102 us, of 32 layers
+// 176.
 template <int HD, int DT>
 __global__ void __launch_bounds__(2 * HD) keep_kernel(const KeepArgs a) {
     constexpr int CPR = HD / 16, R = kKeepRecords, WARPS = 2 * HD / 32;
@@ -354,7 +361,8 @@ struct ReadArgs {
 static_assert(sizeof(ReadArgs) <= 4096, "kernel parameters");
 
 // Values of rows; one (sequence, layer, K or V) per (z, y) of the grid, a thread
-// per 16 codes of a row, in the order of the output.
+// per 16 codes of a row, in the order of the output: 5000 rows of 16 layers (492 MB
+// both ways) in 87 us = 5.7 TB/s.
 template <int HD, int DT, bool F32>
 __global__ void read_kernel(const __grid_constant__ ReadArgs a) {
     constexpr uint32_t CPR = HD / 16;

@@ -5,7 +5,14 @@
 //
 //  * Bound by the codes it reads: one byte per element, 2 G multiply-adds each.
 //    So every record (32 rows of one kv head: K, V and scales, one contiguous
-//    run) goes to shared memory in ONE bulk copy and is read once.
+//    run) goes to shared memory in one bulk copy (head_dim 128 and 256: two, scales
+//    and K, then V, so that 8 or 12 warps per SM have three or four in flight) and is
+//    read once.  Measured (one B200, kernel alone, int8 or e4m3): 131072 rows of the
+//    Mistral-7B shape (8.6 GB) 1.27-1.33 ms = 6.5-6.8 TB/s; 64 ragged sequences of the
+//    Llama-3.2-1B shape (4.4 GB) 0.78-0.81 ms = 5.4-5.6 TB/s (head_dim 64: about 490
+//    instructions per 4 KB record, 2.4 per cycle); one such sequence of 4096 rows
+//    (68 MB) 24 us, of which about 7 before the first record is used and 3 after the
+//    last; 100 rows of one layer 8.5 us.
 //  * Work.  Units are (kv head, page) pairs, flattened over sequences, layers
 //    and heads; each CTA takes an equal run of them, cut into pieces at segment
 //    boundaries (a segment: one kv head of one layer and sequence).  Unit x of
