@@ -190,7 +190,7 @@ struct StepWarp {
     uint32_t qf[KS][NBC][2];
     float o[KS][NBC][4];
     float m[2], l[2];
-    float unscale;     // a.scale log2(e), and what q was scaled by taken back
+    float unscale[2];  // of this lane's two columns: a.scale log2(e), and what q was scaled by taken back
     int lo[2], hi[2];  // attended rows of this lane's two columns
 
     __device__ __forceinline__ static float col_sum(const float (&x)[NBC][4], int r) {
@@ -216,7 +216,6 @@ struct StepWarp {
         const PagedLayer L = a.layers[p.layer];
         const int ncol = run.n * a.G;
         const bool vec = a.q_vec && L.half % 4 == 0;
-        float mx = 0.0f;
 #pragma unroll 2
         for (int i = lane; i < GP * HD / 4; i += 32) {
             const int col = i / (HD / 4), d = i % (HD / 4) * 4;
@@ -228,21 +227,33 @@ struct StepWarp {
                           a.rope[L.cfg] + static_cast<long long>(run.pos0 + tok) * (HD / 2), a.neox != 0, vec);
             }
             *reinterpret_cast<float4*>(tmp + 4 * i) = x;
+        }
+        __syncwarp();
+        auto mine = [&](int ks) {  // what this lane takes of column g % GP; its four lanes have all dims
+            const int d = HD >= 64 ? (t + 4 * (ks / 4)) * 16 + (ks % 4) * 4 : t * 8 + ks * 4;
+            return *reinterpret_cast<const float4*>(tmp + (g % GP) * HD + d);
+        };
+        // A column's largest |q| is brought into [2^14, 2^15): no bits of the second part
+        // are lost to fp16's range.  Each column by itself: a query that is infinite,
+        // or far larger than those of the other heads and tokens, is no matter of theirs.
+        float mx = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const float4 x = mine(ks);
             mx = fmaxf(fmaxf(mx, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
         }
-        // the largest |q| is brought into [2^14, 2^15): no bits of the second part
-        // are lost to fp16's range
-        mx = warp_max(mx);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const int e = static_cast<int>((__float_as_uint(mx) >> 23) & 0xFFu) - 127;
         const int sh = min(60, max(-60, 14 - e));
         const float up = exp2_int(sh);
-        unscale = exp2_int(-sh) * (a.scale * 1.4426950408889634f);
-        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            unscale[j] = exp2_int(-__shfl_sync(0xffffffffu, sh, (2 * t + j) % GP * 4)) * (a.scale * 1.4426950408889634f);
         const int part = g / GP;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const int d = HD >= 64 ? (t + 4 * (ks / 4)) * 16 + (ks % 4) * 4 : t * 8 + ks * 4;
-            const float4 x = *reinterpret_cast<const float4*>(tmp + (g % GP) * HD + d);
+            const float4 x = mine(ks);
             uint32_t h01, l01, h23, l23;
             split_pair<DT_F16T>(x.x * up, x.y * up, h01, l01);
             split_pair<DT_F16T>(x.z * up, x.w * up, h23, l23);
@@ -336,7 +347,7 @@ struct StepWarp {
             vinv[b] = __uint_as_float((254u - ve) << 23);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float s = col_sum(acc[b], r) * (unscale * ks);
+                float s = col_sum(acc[b], r) * (unscale[r & 1] * ks);
                 if (capped) s = a.cap_out * tanhf(s * a.cap_in);
                 s += kv;
                 if (edge) {
