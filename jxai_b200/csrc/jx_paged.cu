@@ -1398,7 +1398,7 @@ int jx_pkv_create(const jx_pkv_desc* desc, jx_pkv** out) {
             return pfail(JX_ERR_NOMEM, "page pool of %zu bytes failed", bytes);
         }
         const size_t ctas = static_cast<size_t>(sms) * kStepCtasPerSm;
-        const size_t part = 2 * ctas * kStepCols * (d.head_dim + 2) * sizeof(float);
+        const size_t part = 2 * ctas * kStepCols * (d.head_dim + 4) * sizeof(float);
         if (cudaMalloc(&kv->d_scratch, part) != cudaSuccess || cudaMalloc(&kv->d_counters, ctas * sizeof(int)) != cudaSuccess ||
             cudaMemset(kv->d_counters, 0, ctas * sizeof(int)) != cudaSuccess) {
             cudaGetLastError();

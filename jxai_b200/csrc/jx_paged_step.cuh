@@ -30,13 +30,16 @@
 //    elements are pairs of codes, and the permute that builds fp16 numbers also
 //    separates the pair: no transposition is paid for.
 //  * Scales.  s = q.k 2^kK enters as a factor of the exponent; the weight of a
-//    row is taken as 2^(s log2e + kV - m) with kV the exponent of its V block,
-//    and the running maximum m is over that sum.  P stays at most 2^15 in
-//    fp16 whatever the scales are, O needs no factor per row, and the softmax
-//    sum takes back 2^-kV in fp32, once per block.
+//    row is taken as 2^(s log2e + kV - m) with kV the exponent of its V block and m
+//    a whole number, so that kV - m is exact and one fused multiply-add gives the
+//    exponent.  Where scores are beyond 2^22 the reference is a pair, a score m and
+//    an exponent c, and the weight 2^((s log2e - m) + (kV - c)): kV would be rounded
+//    away in a sum with such a score.  P stays at most 2^15 in fp16 whatever the
+//    scales are, O needs no factor per row, and the softmax sum takes back 2^-kV in
+//    fp32, once per block.
 //  * Split segments: a CTA has at most two pieces that are not whole segments
 //    (its first and its last), so two slots of scratch per CTA hold their
-//    (o, m, l); the CTA that counts in last joins them.
+//    (o, m, l, c); the CTA that counts in last joins them.
 #pragma once
 
 #include <algorithm>
@@ -57,13 +60,13 @@ struct StepCfg {
     // A stage holds a record, or (wide heads) half of one: scales and K, or V.
     static constexpr bool SPLIT = HD >= 128;
     static constexpr int STAGE = SPLIT ? tile_at(HD, 1) : record_bytes(HD);
-    static constexpr int MISC = W * GP * 2 * 4 + 64;  // (m, l) of each warp and column; flags
+    static constexpr int MISC = W * GP * 4 * 4 + 64;  // (m, l, c) of each warp and column; flags
     static constexpr int budget = (227 * 1024) / CTAS - 1024 - MISC - 8;
     static constexpr int fit = budget / (W * (STAGE + 8));
     static constexpr int NS = fit > 8 ? 8 : fit;  // stages per warp
-    // floats of a partial result: o [GP][HD], then (m, l) [GP]; 16-byte aligned
-    static constexpr int PART = (GP * (HD + 2) + 3) / 4 * 4;
-    static_assert(PART <= kStepCols * (HD + 2), "scratch");
+    // floats of a partial result: o [GP][HD], then (m, l, c, -) [GP]; 16-byte aligned
+    static constexpr int PART = GP * (HD + 4);
+    static_assert(PART <= kStepCols * (HD + 4), "scratch");
     static constexpr int OFF_MISC = W * NS * STAGE;
     static constexpr int OFF_BAR = OFF_MISC + MISC;
     static constexpr int SMEM = OFF_BAR + W * NS * 8 + 8;  // (+ the barrier of test_wait_cta)
@@ -182,16 +185,18 @@ template <int HD, int GP, int DT>
 struct StepWarp {
     static constexpr int NBC = (2 * GP + 7) / 8;  // column blocks: (part, head) pairs
     static constexpr int KS = HD / 16;
-    // Weights are taken against a reference m, 2^10 below the largest when it is set
-    // and moved when a weight would exceed 2^15 (fp16 ends at 2^16).  Beyond 2^20 it
-    // is the largest itself: 10 is no longer exact next to it.
-    static constexpr float kBase = 10.0f, kTop = 15.0f, kFar = 1048576.0f;
+    // Weights are taken against a reference m + c, about 2^10 below the largest when it
+    // is set and moved when a weight would exceed 2^15 (fp16 ends at 2^16).  m is a whole
+    // number and c 0, or, scores beyond kFar, m the largest of them.
+    static constexpr float kBase = 10.0f, kTop = 15.0f, kFar = 4194304.0f;
 
     uint32_t qf[KS][NBC][2];
     float o[KS][NBC][4];
-    float m[2], l[2];
+    float m[2], l[2];  // m is 0 before the column's first row
+    float top[2];      // what a weight's exponent may be: kTop, or -inf before the first row
     float unscale[2];  // of this lane's two columns: a.scale log2(e), and what q was scaled by taken back
     int lo[2], hi[2];  // attended rows of this lane's two columns
+    bool far;          // a column of the warp has scores beyond kFar; then each has a c, in shared memory
 
     __device__ __forceinline__ static float col_sum(const float (&x)[NBC][4], int r) {
         float v = x[0][r];
@@ -274,9 +279,11 @@ struct StepWarp {
             const int pos = run.pos0 + min(col, ncol - 1) / a.G;
             hi[j] = pos;
             lo[j] = (L.flags & kLayerWindow) ? max(0, pos - a.window + 1) : 0;
-            m[j] = -INFINITY;
+            m[j] = 0.0f;
+            top[j] = -INFINITY;
             l[j] = 0.0f;
         }
+        far = false;
 #pragma unroll
         for (int mh = 0; mh < KS; ++mh)
 #pragma unroll
@@ -287,9 +294,65 @@ struct StepWarp {
 
     uint32_t bp[2][NBC][2];  // weights of a page as operands
 
-    // Weights of rows row0 .. row0+31 from their K tile and scales.
+    // l and O by a factor of each column.
+    __device__ __forceinline__ void rescale(const float (&w)[2]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            l[j] *= w[j];
+#pragma unroll
+            for (int mh = 0; mh < KS; ++mh)
+#pragma unroll
+                for (int nb = 0; nb < NBC; ++nb) {
+                    o[mh][nb][j] *= w[j];
+                    o[mh][nb][j + 2] *= w[j];
+                }
+        }
+    }
+
+    // The largest of a column's rows of a page.
+    __device__ __forceinline__ static float largest(const float (&v)[2][4], int j) {
+        float t = fmaxf(fmaxf(v[0][j], v[0][j + 2]), fmaxf(v[1][j], v[1][j + 2]));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+        return fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+    }
+
+    // What a page does to the references where scores are beyond kFar: x [block][row]
+    // (scores) becomes the weights' exponents, w what l and O are to be multiplied by.  A
+    // call of its own: inline it would cost the ordinary page registers.
+    struct FarPage {
+        float x[2][4], kv[2], m[2], c[2], top[2], w[2];
+    };
+    __device__ __noinline__ static void far_page(FarPage& p) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float z[2][4];
+            auto against = [&](float mj, float cj) {
+                for (int b = 0; b < 2; ++b)
+                    for (int r = j; r < 4; r += 2) z[b][r] = (p.x[b][r] - mj) + (p.kv[b] - cj);
+                return largest(z, j);
+            };
+            const float mx = largest(p.x, j);
+            const bool move = against(p.m[j], p.c[j]) > p.top[j], beyond = fabsf(mx) > kFar;
+            p.w[j] = 1.0f;
+            const float e = against(beyond ? mx : 0.0f, 0.0f);
+            if (move) {
+                const float m1 = beyond ? mx : rintf(e) - kBase, c1 = beyond ? e - kBase : 0.0f;
+                p.w[j] = p.top[j] == -INFINITY ? 0.0f : ex2_approx((p.m[j] - m1) + (p.c[j] - c1));
+                p.m[j] = m1;
+                p.c[j] = c1;
+                p.top[j] = kTop;
+            }
+            against(p.m[j], p.c[j]);
+            for (int b = 0; b < 2; ++b)
+                for (int r = j; r < 4; r += 2) p.x[b][r] = z[b][r];
+        }
+    }
+
+    // Weights of rows row0 .. row0+31 from their K tile and scales.  mlc: where the
+    // warp's columns keep their c while `far`.
     __device__ __forceinline__ void scores(const PagedArgs& a, const unsigned char* rec, const float4 sc, int row0,
-                                           bool edge, int lane) {
+                                           bool edge, float4* mlc, int lane) {
         const int g = lane >> 2, t = lane & 3;
         float acc[2][NBC][4];
 #pragma unroll
@@ -335,65 +398,86 @@ struct StepWarp {
                 }
             }
         }
-        // exponents: x = s log2e + kV; rows b*16 + (r>>1)*8 + perm(g), column slot r&1
-        float x[2][4];
-        float vinv[2];
+        // s log2e = d * f; rows b*16 + (r>>1)*8 + perm(g), column slot r&1
+        float d[2][4], f[2][2], kv[2], vinv[2], y[2][4];
         const bool capped = a.softcap > 0.0f;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const float ks = b ? sc.y : sc.x;
             const uint32_t ve = __float_as_uint(b ? sc.w : sc.z) >> 23;
-            const float kv = static_cast<float>(static_cast<int>(ve) - 127);
+            kv[b] = static_cast<float>(static_cast<int>(ve) - 127);
             vinv[b] = __uint_as_float((254u - ve) << 23);
+            f[b][0] = unscale[0] * (b ? sc.y : sc.x);
+            f[b][1] = unscale[1] * (b ? sc.y : sc.x);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float s = col_sum(acc[b], r) * (unscale[r & 1] * ks);
-                if (capped) s = a.cap_out * tanhf(s * a.cap_in);
-                s += kv;
-                if (edge) {
-                    const int row = row0 + b * 16 + (r >> 1) * 8 + rp;
-                    if (row < lo[r & 1] || row > hi[r & 1]) s = -INFINITY;
-                }
-                x[b][r] = s;
+                d[b][r] = col_sum(acc[b], r);
+                if (capped) d[b][r] = a.cap_out * tanhf(d[b][r] * f[b][r & 1] * a.cap_in);
             }
+            if (capped) f[b][0] = f[b][1] = 1.0f;
         }
-        float mt[2];
-        bool move = false;
+        auto exponents = [&]() {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            mt[j] = fmaxf(fmaxf(x[0][j], x[0][j + 2]), fmaxf(x[1][j], x[1][j + 2]));
-            mt[j] = fmaxf(mt[j], __shfl_xor_sync(0xffffffffu, mt[j], 4));
-            mt[j] = fmaxf(mt[j], __shfl_xor_sync(0xffffffffu, mt[j], 8));
-            mt[j] = fmaxf(mt[j], __shfl_xor_sync(0xffffffffu, mt[j], 16));
-            move = move || mt[j] - m[j] > kTop;  // (an empty m is -inf, an empty page's maximum, too)
-        }
-        if (__any_sync(0xffffffffu, move)) {
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    y[b][r] = fmaf(d[b][r], f[b][r & 1], kv[b] - m[r & 1]);
+                    if (edge) {
+                        const int row = row0 + b * 16 + (r >> 1) * 8 + rp;
+                        if (row < lo[r & 1] || row > hi[r & 1]) y[b][r] = -INFINITY;
+                    }
+                }
+        };
+        exponents();
+        const float big[2] = {largest(y, 0), largest(y, 1)};
+        if (__any_sync(0xffffffffu, far || big[0] > top[0] || big[1] > top[1])) {
+            float w[2], mn[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const float to = mt[j] - (fabsf(mt[j]) > kFar ? 0.0f : kBase);
-                const float mn = mt[j] > -INFINITY ? fmaxf(m[j], to) : m[j];
-                const float f = m[j] == -INFINITY ? 0.0f : ex2_approx(m[j] - mn);
-                m[j] = mn;
-                l[j] *= f;
+                mn[j] = big[j] > top[j] ? rintf(m[j] + big[j]) - kBase : m[j];
+                w[j] = top[j] == -INFINITY ? 0.0f : ex2_approx(m[j] - mn[j]);
+            }
+            if (__any_sync(0xffffffffu, far || fabsf(mn[0]) > kFar || fabsf(mn[1]) > kFar)) {
+                FarPage p;
 #pragma unroll
-                for (int mh = 0; mh < KS; ++mh)
+                for (int j = 0; j < 2; ++j) {
+                    p.m[j] = m[j];
+                    p.c[j] = far ? mlc[(2 * t + j) % GP].z : 0.0f;
+                    p.top[j] = top[j];
+                    p.kv[j] = kv[j];
 #pragma unroll
-                    for (int nb = 0; nb < NBC; ++nb) {
-                        o[mh][nb][j] *= f;
-                        o[mh][nb][j + 2] *= f;
-                    }
+                    for (int r = 0; r < 4; ++r)  // scores as rounded numbers (a fused product would
+                        // tell equal ones apart from their rounded maximum)
+                        p.x[j][r] = y[j][r] == -INFINITY ? -INFINITY : __fmul_rn(d[j][r], f[j][r & 1]);
+                }
+                far_page(p);
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    m[j] = p.m[j];
+                    top[j] = p.top[j];
+                    w[j] = p.w[j];
+                    mlc[(2 * t + j) % GP].z = p.c[j];  // (the lanes of a column write the same)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[j][r] = p.x[j][r];
+                }
+                __syncwarp();
+                far = __any_sync(0xffffffffu, fabsf(m[0]) > kFar || fabsf(m[1]) > kFar);
+                rescale(w);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    m[j] = mn[j];
+                    if (big[j] > top[j]) top[j] = kTop;
+                }
+                rescale(w);
+                exponents();
             }
         }
-        float mb[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) mb[j] = m[j] == -INFINITY ? 0.0f : -m[j];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             float pr[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                pr[r] = ex2_approx(x[b][r] + mb[r & 1]);
-            }
+            for (int r = 0; r < 4; ++r) pr[r] = ex2_approx(y[b][r]);
             l[0] = fmaf(pr[0] + pr[2], vinv[b], l[0]);
             l[1] = fmaf(pr[1] + pr[3], vinv[b], l[1]);
 #pragma unroll
@@ -445,8 +529,9 @@ struct StepWarp {
         }
     }
 
-    // This warp's part of a piece to shared memory: o_s [col][HD], ml_s [col][2].
-    __device__ __forceinline__ void finish(float* o_s, float* ml_s, int lane) {
+    // This warp's part of a piece to shared memory: o_s [col][HD], mlc [col](m, l, c), m
+    // -inf of a column without rows.
+    __device__ __forceinline__ void finish(float* o_s, float4* mlc, int lane) {
         const int g = lane >> 2, t = lane & 3;
         const bool w0 = GP == 8 || (GP == 4 && t < 2) || (GP <= 2 && t == 0);
         const bool w1 = w0 && GP != 1;
@@ -464,8 +549,8 @@ struct StepWarp {
             v += __shfl_xor_sync(0xffffffffu, v, 8);
             v += __shfl_xor_sync(0xffffffffu, v, 16);
             if (g == 0 && (j == 0 ? w0 : w1)) {
-                ml_s[((2 * t + j) % GP) * 2] = m[j];
-                ml_s[((2 * t + j) % GP) * 2 + 1] = v;
+                float4& at = mlc[(2 * t + j) % GP];
+                at = make_float4(top[j] == -INFINITY ? -INFINITY : m[j], v, far ? at.z : 0.0f, 0.0f);
             }
         }
     }
@@ -563,16 +648,41 @@ __device__ __forceinline__ void warm_inputs(const PagedArgs& a, const Piece& p, 
     }
 }
 
+// Elements e .. e+3 of a split segment's sum where its scores are beyond kFar: each
+// part's c counts, too.  Rare, so one part after the other, in a call of its own.
+template <int HD, int GP>
+__device__ __noinline__ float4 join_far(const float* scratch, int c0, int c1, int e, float* sum) {
+    float M = -INFINITY, Cm = 0.0f, Ls = 0.0f;
+    float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int c = c0; c <= c1; ++c) {
+        const float* src = scratch + static_cast<long long>(c == c0 ? 2 * c0 + 1 : 2 * c) * StepCfg<HD, GP>::PART;
+        const float4 mlc = __ldcg(reinterpret_cast<const float4*>(src + GP * HD + 4 * (e / HD)));
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(src + e));
+        if (mlc.x == -INFINITY) continue;
+        const float Mn = fmaxf(M, mlc.x);
+        const float x = (M - Mn) + Cm, y = (mlc.x - Mn) + mlc.z, Cn = fmaxf(x, y);
+        const float f0 = ex2_approx(x - Cn), f = ex2_approx(y - Cn);
+        Ls = fmaf(mlc.y, f, Ls * f0);
+        O = make_float4(fmaf(o.x, f, O.x * f0), fmaf(o.y, f, O.y * f0), fmaf(o.z, f, O.z * f0), fmaf(o.w, f, O.w * f0));
+        M = Mn;
+        Cm = Cn;
+    }
+    *sum = Ls;
+    return O;
+}
+
 template <int HD, int GP, int DT>
 __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS)
     paged_step_kernel(const __grid_constant__ PagedArgs a) {
     using C = StepCfg<HD, GP>;
+    using SW = StepWarp<HD, GP, DT>;
     constexpr int W = C::W, NS = C::NS;
     static_assert(W == 4, "PieceWalk's rotation");
     extern __shared__ __align__(16) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float* ml_s = reinterpret_cast<float*>(smem + C::OFF_MISC);                 // [warp][col](m, l)
-    int* o_at = reinterpret_cast<int*>(smem + C::OFF_MISC + W * GP * 2 * 4);    // [warp]: its o in smem
+    float4* mlc_s = reinterpret_cast<float4*>(smem + C::OFF_MISC);              // [warp][col](m, l, c)
+    int* o_at = reinterpret_cast<int*>(smem + C::OFF_MISC + W * GP * 4 * 4);    // [warp]: its o in smem
     volatile int* abort_flag = o_at + W;
     int* flag = o_at + W + 1;
     unsigned char* ring = smem + warp * NS * C::STAGE;
@@ -668,7 +778,7 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
     };
     if (a.test_wait_cta == c + 1 && warp == 0)
         dead = !__all_sync(0xffffffffu, mbar_wait_bounded(test_bar, 0u, abort_flag, a.err, a.dbg, 42, 0, true, a.wait_limit));
-    StepWarp<HD, GP, DT> sw;
+    SW sw;
     for (; more; more = cw.next(a, p)) {
         if (!p.coop && warp != p.rot) continue;
         // the stage kept back: the one read last (at the start, the last one)
@@ -707,7 +817,7 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
                                             static_cast<long long>(p.h) * record_bytes(HD), lane);
                 }
                 sw.scores(a, rec + tile_at(HD, 0), *reinterpret_cast<const float4*>(rec), row0,
-                          row0 < lo_all || row0 + kPageRows - 1 > run.pos0, lane);
+                          row0 < lo_all || row0 + kPageRows - 1 > run.pos0, mlc_s + warp * GP, lane);
             }
             if constexpr (C::SPLIT) {
                 advance();
@@ -731,20 +841,19 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
         };
         if (!p.coop) {
             // a whole segment, read by this warp alone
-            float* ml = ml_s + warp * GP * 2;
-            sw.finish(reinterpret_cast<float*>(o_mine), ml, lane);
+            float4* mlc = mlc_s + warp * GP;
+            sw.finish(reinterpret_cast<float*>(o_mine), mlc, lane);
             __syncwarp();
             for (int e = lane; e < ncol * HD; e += 32) {
-                *out_at(e / HD, e % HD) = __fdividef(reinterpret_cast<const float*>(o_mine)[e], ml[e / HD * 2 + 1]);
+                *out_at(e / HD, e % HD) = __fdividef(reinterpret_cast<const float*>(o_mine)[e], mlc[e / HD].y);
             }
             __syncwarp();
             continue;
         }
         if (any) {
-            sw.finish(reinterpret_cast<float*>(o_mine), ml_s + warp * GP * 2, lane);
+            sw.finish(reinterpret_cast<float*>(o_mine), mlc_s + warp * GP, lane);
         } else if (lane < GP) {
-            ml_s[(warp * GP + lane) * 2] = -INFINITY;
-            ml_s[(warp * GP + lane) * 2 + 1] = 0.0f;
+            mlc_s[warp * GP + lane] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         }
         if (lane == 0) o_at[warp] = any ? static_cast<int>(o_mine - smem) : -1;
         __syncthreads();
@@ -758,15 +867,28 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
             float M = -INFINITY;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                ml[w] = *reinterpret_cast<const float2*>(ml_s + (w * GP + col) * 2);
+                ml[w] = *reinterpret_cast<const float2*>(mlc_s + w * GP + col);
                 M = fmaxf(M, ml[w].x);
+            }
+#pragma unroll
+            for (int w = 0; w < W; ++w) ml[w].x = ml[w].x == -INFINITY ? -INFINITY : ml[w].x - M;
+            float Cm = 0.0f;  // of the sum, as M
+            if (fabsf(M) > SW::kFar && M > -INFINITY) {  // (else a part with a c of its own has no weight)
+                Cm = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    ml[w].x += mlc_s[w * GP + col].z;
+                    Cm = fmaxf(Cm, ml[w].x);
+                }
+#pragma unroll
+                for (int w = 0; w < W; ++w) ml[w].x -= Cm;
             }
             float Ls = 0.0f;
             float2 O = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                if (ml[w].x == -INFINITY) continue;
-                const float f = ex2_approx(ml[w].x - M);
+                if (o_at[w] < 0 || ml[w].x == -INFINITY) continue;  // no pages, or no rows of them
+                const float f = ex2_approx(ml[w].x);
                 const float2 o = *reinterpret_cast<const float2*>(smem + o_at[w] + e * 4);
                 Ls = fmaf(ml[w].y, f, Ls);
                 O = make_float2(fmaf(o.x, f, O.x), fmaf(o.y, f, O.y));
@@ -778,7 +900,7 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
                 dst[1] = O.y * inv;
             } else {
                 *reinterpret_cast<float2*>(part + e) = O;
-                if (d == 0) *reinterpret_cast<float2*>(part + GP * HD + 2 * col) = make_float2(M, Ls);
+                if (d == 0) *reinterpret_cast<float4*>(part + GP * HD + 4 * col) = make_float4(M, Ls, Cm, 0.0f);
             }
         }
         if (!whole) {
@@ -804,7 +926,7 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
                             // beyond the last part: the last one again, with no weight
                             const int cq = min(q0 + q, c1);
                             const float* src = a.scratch + static_cast<long long>(cq == c0 ? 2 * c0 + 1 : 2 * cq) * C::PART;
-                            ml[q] = __ldcg(reinterpret_cast<const float2*>(src + GP * HD + 2 * col));
+                            ml[q] = __ldcg(reinterpret_cast<const float2*>(src + GP * HD + 4 * col));
                             ov[q] = __ldcg(reinterpret_cast<const float4*>(src + e));
                             if (q0 + q > c1) ml[q].x = -INFINITY;
                         }
@@ -824,6 +946,7 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
                         }
                         M = Mn;
                     }
+                    if (fabsf(M) > SW::kFar && M > -INFINITY) O = join_far<HD, GP>(a.scratch, c0, c1, e, &Ls);
                     float* dst = out_at(col, d);
                     const float inv = __fdividef(1.0f, Ls);
                     dst[0] = O.x * inv;
@@ -833,7 +956,7 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
                 }
             }
         }
-        __syncthreads();  // o, ml_s and flag are read before they are written again
+        __syncthreads();  // o, mlc_s and flag are read before they are written again
     }
     // every copy has landed before the CTA exits, after a wait that ran out too
     for (int k = max(0, issued - NS); k < issued; ++k)

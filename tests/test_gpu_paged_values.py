@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import jxai_b200 as jx
-from tests.test_gpu_paged import Pair, cuda
+from tests.test_gpu_paged import Pair, cuda, load_prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +72,83 @@ def test_small_queries_beside_large_ones_keep_their_bits(tc):
     got = attend(p, 0, 0, q, k, v, True)
     ref, tol = expect(p, 0, 0, 0, q, k, v)
     assert (np.abs(got[:, 0] - ref) <= tol)[:, ::2].all()
+
+
+def far_case(rng, n, HD, H, HK, spread):
+    """Keys that are one direction times 1, 0.5 or -1 (each block of 16 holds a 1), and values whose
+    blocks are 2^-spread .. 2^spread large.  No rotation."""
+    f = rng.choice([1.0, 0.5, -1.0], n)
+    f[::16] = 1.0
+    u = rng.standard_normal((HK, HD)).astype(np.float32)
+    k = (f[:, None, None] * u).reshape(n, 1, HK * HD)
+    v = rng.standard_normal((n, 1, HK * HD))
+    v *= np.exp2(rng.integers(-spread, spread + 1, n // 16 + 1))[np.arange(n) // 16][:, None, None]
+    q = rng.standard_normal((n, 1, H * HD))
+    return f, u, [x.astype(np.float32) for x in (q, k, v)]
+
+
+@pytest.mark.parametrize("tc", [0, 1])
+@pytest.mark.parametrize("size", [1e4, 1e6, 2.0 ** 26, 1e12, 1e18])
+@pytest.mark.parametrize("H,HK,HD,dtype", [(2, 1, 64, "int8"), (4, 2, 128, "e4m3"), (4, 1, 256, "int8"),
+                                           (8, 4, 32, "e4m3"), (7, 1, 64, "e4m3")])
+def test_scores_of_any_size(H, HK, HD, dtype, size, tc):
+    """Scores so far apart that the largest wins alone, and several equal largest: the output is the
+    mean of their values, whatever the scales of the blocks that these lie in."""
+    rng = np.random.default_rng(int(np.log2(size)) + HD)
+    n = 150
+    f, u, (q, k, v) = far_case(rng, n, HD, H, HK, 10)
+    G = H // HK
+    # every query at an angle to the keys that keeps |q.u| near its largest
+    q = np.sign(rng.standard_normal((n, 1, HK, G, 1))) * (u[:, None] + 0.1 * q.reshape(n, 1, HK, G, HD))
+    q = (q * np.float32(size)).astype(np.float32).reshape(n, 1, H * HD)
+    p = Pair(H, HK, HD, dtype, cap=256, seed=1, tc=tc, rope_dim=0)
+
+    def check(got, at, q):
+        V = p.model.values(0, 0, 1, 0, at + len(got))
+        for i in range(len(got)):
+            for h in range(H):
+                g = h // G
+                s = np.sign(q[i].reshape(H, HD)[h].astype(np.float64) @ u[g])
+                x = s * f[:at + i + 1]
+                w = x == x.max()
+                want = V[:at + i + 1, g][w].mean(0)
+                # Weights of equal scores: 2^-22 from exp2 and 2^-22 as two fp16 parts; what the
+                # second part loses below the largest weight, 2^-25 each; the sums over rows, one
+                # rounding (2^-23) per 16 rows and a few more.
+                tol = np.abs(V[:at + i + 1, g][w]).max() * (2.0 ** -21 + (at + i + 1) * 2.0 ** -25
+                                                           + ((at + i + 1) / 16 + 4) * 2.0 ** -23)
+                assert (np.abs(got[i, 0, h] - want) <= tol).all(), (i, h)
+    got = attend(p, 0, 0, q, k, v, True)
+    p.model.write(0, 0, 0, 0, k.reshape(n, HK, HD))
+    p.model.write(0, 0, 1, 0, v.reshape(n, HK, HD))
+    check(got, 0, q)
+    f = np.append(f, 1.0)
+    one = [q[:1], u.reshape(1, 1, HK * HD), v[-1:]]
+    got = attend(p, 0, n, *one, False)
+    p.model.write(0, 0, 0, n, u.reshape(1, HK, HD))
+    p.model.write(0, 0, 1, n, v[-1:].reshape(1, HK, HD))
+    check(got, n, one[0])
+
+
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+def test_far_scores_over_a_split_segment(dtype):
+    """A long row whose parts are joined over CTAs: equal far scores count alike, and a part without
+    any of the largest counts for nothing."""
+    rng = np.random.default_rng(5)
+    n, HD = 6000, 64
+    f, u, (_, k, v) = far_case(rng, n, HD, 1, 1, 8)
+    f[:2000] = np.where(f[:2000] == 1.0, 0.5, f[:2000])  # the first third holds none of the largest
+    f[:2000:16] = -1.0
+    k = (f[:, None, None] * u).reshape(n, 1, HD).astype(np.float32)
+    p = Pair(1, 1, HD, dtype, cap=6016, seed=1, rope_dim=0)
+    load_prompt(p, 0, (None, k, v))
+    V = p.model.values(0, 0, 1, 0, n)[:, 0]
+    w = f == 1.0
+    for size in (1.0, 2.0 ** 20, 2.0 ** 27, 2.0 ** 60):
+        q = (u * np.float32(size * 30)).reshape(1, 1, HD)
+        # a new key that scores least, dropped again
+        got = attend(p, 0, n, q, -u.reshape(1, 1, HD), v[:1], False)[0, 0, 0]
+        p.cache.rollback(0, n)
+        # the largest score is at least 30 |u|^2 / 8 / 2 above the next: e^-100 and less of the rest
+        tol = np.abs(V[w]).max() * (2.0 ** -21 + n * 2.0 ** -25 + (n / 16 + 4) * 2.0 ** -23)
+        assert (np.abs(got - V[w].mean(0)) <= tol).all(), size
