@@ -138,6 +138,20 @@ __device__ __forceinline__ int scale_exp(float s) {  // k of a stored scale 2^k
     return static_cast<int>(__float_as_uint(s) >> 23) - 127;
 }
 
+// Exponent of the power of two that brings a query whose largest magnitude is `amax`
+// into [2^14, 2^15), to the end of fp32's range; at most 2^60 for small ones, of which
+// what lies below 2^-84 is lost.
+__device__ __forceinline__ int query_exp(float amax) {
+    return min(60, 14 - (static_cast<int>((__float_as_uint(amax) >> 23) & 0xFFu) - 127));
+}
+// What takes that (and the scale of scores) back, no larger than 2^70: times a block's
+// scale it then stays in range, and scores that it cuts are 2^30 apart and more.
+__device__ __forceinline__ float query_unit(int sh, float scale) {
+    constexpr float kMost = 1.180591620717411303424e21f;
+    const float u = exp2_int(-sh) * scale;
+    return u > kMost ? kMost : u < -kMost ? -kMost : u;
+}
+
 // One element of a rotated head; each operation's result is an fp32 number
 // (no fused multiply-add), so that what the cache holds does not depend on
 // how the compiler contracts.  cs[j] = (cos, sin).

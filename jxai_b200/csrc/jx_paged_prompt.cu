@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t to = tmem + lane_addr + C::COL_O + x * 128;
         const bool capped = a.softcap > 0.0f;
         // This row of item tl's Q tile: rotated, brought into [2^14, 2^15), split into
-        // two fp16 parts.  Returns the power of two that undoes it.
+        // two fp16 parts.  Returns what undoes it, times the scale of scores.
         auto stage_q = [&](const PrefillTile& tl) -> float {
             const int tok = x * TQ + j;
             float qr[HW];
@@ -286,8 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int d = 0; d < HW; ++d) mx = fmaxf(mx, fabsf(qr[d]));
             mx = fmaxf(mx, swap(mx, true, false));
-            const int e = static_cast<int>((__float_as_uint(mx) >> 23) & 0xFFu) - 127;
-            const int sh = min(60, max(-60, 14 - e));
+            const int sh = query_exp(mx);
             const float up = exp2_int(sh);
             unsigned char* q = base + C::OFF_Q + 2 * x * C::TILE;
 #pragma unroll
@@ -304,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             fence_proxy_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(BAR(C::B_QF + x));
-            return exp2_int(-sh);
+            return query_unit(sh, a.scale * kLog2);
         };
         int g = 0, pv = 0;  // phases of S, and of P.V, so far
         float unscale = it_begin < it_end ? stage_q(a.tiles[it_begin]) : 1.0f;
@@ -319,8 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int lo_all = tl.window > 0 ? max(0, row_n - tl.window + 1) : 0;
             const float2 hs = __ldg(a.head_scale + (static_cast<long long>(tl.seq) * a.scale_layers + tl.cache_layer) *
                                                        a.scale_heads + tl.kvh);
-            const float mul = a.scale * unscale * hs.x;  // raw S -> score
-            const float mul2 = mul * kLog2;
+            const float mul2 = unscale * hs.x;  // raw S -> score, in units of log2
             float m = -INFINITY, l = 0.0f;  // what weights are taken against (in units of log2)
             float behind = 1.0f;            // what the total is to be multiplied by since it was written
             for (int t = 0; t < nt; ++t, ++g, ++pv) {

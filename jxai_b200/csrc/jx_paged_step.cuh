@@ -249,12 +249,11 @@ struct StepWarp {
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const int e = static_cast<int>((__float_as_uint(mx) >> 23) & 0xFFu) - 127;
-        const int sh = min(60, max(-60, 14 - e));
+        const int sh = query_exp(mx);
         const float up = exp2_int(sh);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-            unscale[j] = exp2_int(-__shfl_sync(0xffffffffu, sh, (2 * t + j) % GP * 4)) * (a.scale * 1.4426950408889634f);
+            unscale[j] = query_unit(__shfl_sync(0xffffffffu, sh, (2 * t + j) % GP * 4), a.scale * 1.4426950408889634f);
         const int part = g / GP;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {

@@ -88,7 +88,7 @@ def far_case(rng, n, HD, H, HK, spread):
 
 
 @pytest.mark.parametrize("tc", [0, 1])
-@pytest.mark.parametrize("size", [1e4, 1e6, 2.0 ** 26, 1e12, 1e18])
+@pytest.mark.parametrize("size", [1e4, 1e6, 2.0 ** 26, 1e12, 1e18, 1e24, 1e33])
 @pytest.mark.parametrize("H,HK,HD,dtype", [(2, 1, 64, "int8"), (4, 2, 128, "e4m3"), (4, 1, 256, "int8"),
                                            (8, 4, 32, "e4m3"), (7, 1, 64, "e4m3")])
 def test_scores_of_any_size(H, HK, HD, dtype, size, tc):
