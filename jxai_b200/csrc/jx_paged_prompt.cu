@@ -318,7 +318,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int lo_all = tl.window > 0 ? max(0, row_n - tl.window + 1) : 0;
             const float2 hs = __ldg(a.head_scale + (static_cast<long long>(tl.seq) * a.scale_layers + tl.cache_layer) *
                                                        a.scale_heads + tl.kvh);
-            const float mul2 = unscale * hs.x;  // raw S -> score, in units of log2
+            // raw S -> score, in units of log2; not 0, which times a masked -inf is NaN
+            const float mul2 = fmaxf(unscale * hs.x, 1.17549435e-38f);
             float m = -INFINITY, l = 0.0f;  // what weights are taken against (in units of log2)
             float behind = 1.0f;            // what the total is to be multiplied by since it was written
             for (int t = 0; t < nt; ++t, ++g, ++pv) {

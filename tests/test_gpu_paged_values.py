@@ -152,3 +152,18 @@ def test_far_scores_over_a_split_segment(dtype):
         # the largest score is at least 30 |u|^2 / 8 / 2 above the next: e^-100 and less of the rest
         tol = np.abs(V[w]).max() * (2.0 ** -21 + n * 2.0 ** -25 + (n / 16 + 4) * 2.0 ** -23)
         assert (np.abs(got - V[w].mean(0)) <= tol).all(), size
+
+
+def test_a_scale_that_almost_vanishes():
+    """Scores that underflow are zeros, not NaN where a later row is masked."""
+    for tc in (0, 1):
+        p = Pair(2, 1, 64, "int8", cap=256, seed=6, tc=tc)
+        q, k, v = p.inputs(200)
+        for scale in (1e-30, 1e-38, 1e-45):
+            p.cache.clear(0)
+            got = attend(p, 0, 0, q, k, v, True, scale=scale)[:, 0]
+            p.model.write(0, 0, 1, 0, v.reshape(200, 1, 64))
+            V = p.model.values(0, 0, 1, 0, 200)[:, 0]
+            mean = np.cumsum(V, 0) / np.arange(1, 201)[:, None]
+            tol = np.abs(V).max() * (2.0 ** -21 + 200 * 2.0 ** -25 + (200 / 16 + 4) * 2.0 ** -23)
+            assert (np.abs(got - mean[:, None]) <= tol).all()
