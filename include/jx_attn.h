@@ -330,7 +330,8 @@ JX_API int jx_pkv_read_rows(jx_pkv* kv, const int32_t* seq_ids, const int32_t* r
  * the cache's head_dim, the call its n_kv_heads; at most 8 RoPE settings per
  * handle (rope_dim, base, factors, yarn_scale).  In a prompt, the rows of one sequence
  * stand together and ascend by one.  New pages come from the pool; with too few
- * left, JX_ERR_NOMEM and nothing is changed. */
+ * left, or where a prompt's workspaces cannot be allocated, JX_ERR_NOMEM and
+ * nothing is changed. */
 JX_API int jx_pkv_attn_step(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers,
                             const jx_step_args* args, void* stream);
 JX_API int jx_pkv_attn_prefill(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers,
@@ -341,7 +342,9 @@ JX_API int jx_pkv_check_device_error(jx_pkv* kv, int* code, void* stream);
 /* "wait_limit_ms" and "test_wait_cta" (of a step): as in jx_kv_set_option;
  * "prefill_tc": prompts on the tensor-core kernel where it takes their shape (1),
  * in the step kernel's blocks (0), or by an estimate of both (-1, the default).
- * The tensor-core kernel takes K and V beyond 8e6 in magnitude as that large. */
+ * The tensor-core kernel takes K and V beyond 8e6 in magnitude as that large.
+ * "test_fail" 1: a workspace that a prompt or a keep would have to allocate
+ * cannot be had -- a test of that error path (0 = off). */
 JX_API int jx_pkv_set_option(jx_pkv* kv, const char* key, int value);
 /* Kernels the last jx_pkv_attn_step / jx_pkv_attn_prefill launched. */
 JX_API int jx_pkv_last_launch_count(const jx_pkv* kv, int* count);

@@ -552,6 +552,7 @@ struct jx_pkv {
     int num_sms = 0;
     int opt_wait_limit_ms = 0;
     int opt_test_wait_cta = 0;
+    int opt_test_fail = 0;          // test hook: a call's workspaces cannot be had
     int opt_prefill_tc = -1;              // prompts on the tensor cores: 1 / 0, -1: by estimate
     int last_launches = 0;
 };
@@ -638,12 +639,14 @@ struct Span {  // rows [begin, end) of a sequence that a call writes
 };
 
 // Pages for the rows that a call writes: new ones, and copies of shared ones
-// (the page is shared by a fork: the writer gets its own).  All or nothing.
+// (the page is shared by a fork: the writer gets its own).  All or nothing: what can
+// fail for lack of memory comes before the first page moves.
 int make_room(jx_pkv* kv, const std::vector<Span>& spans, cudaStream_t st) {
     size_t need = 0;
     std::map<int, int> left;  // holders of a shared page after those before have their own
     for (const Span& s : spans) {
-        const auto& pg = kv->pages[s.seq];
+        auto& pg = kv->pages[s.seq];
+        pg.reserve(pages_for(s.end));
         for (uint32_t i = s.begin / kPageRows; i < pages_for(s.end); ++i) {
             if (i >= pg.size()) {
                 ++need;
@@ -661,6 +664,8 @@ int make_room(jx_pkv* kv, const std::vector<Span>& spans, cudaStream_t st) {
                      kv->free_pages.size(), kv->d.n_pages);
     std::vector<TableEntry> table;
     std::vector<std::pair<int, int>> copies;
+    table.reserve(need);
+    copies.reserve(need);
     for (const Span& s : spans) {
         auto& pg = kv->pages[s.seq];
         for (uint32_t i = s.begin / kPageRows; i < pages_for(s.end); ++i) {
@@ -746,6 +751,7 @@ int take_upload(jx_pkv* kv, size_t bytes, jx_pkv::Upload** out) {
     if (u.pending) PKV_CUDA(cudaEventSynchronize(u.done));
     u.pending = false;
     if (u.bytes < bytes) {
+        if (kv->opt_test_fail) return pfail(JX_ERR_NOMEM, "list of %zu bytes failed (test_fail)", bytes);
         if (u.h) PKV_CUDA(cudaFreeHost(u.h));
         u.h = nullptr;
         if (u.d) PKV_CUDA(cudaFree(u.d));
@@ -762,19 +768,23 @@ int take_upload(jx_pkv* kv, size_t bytes, jx_pkv::Upload** out) {
     return JX_OK;
 }
 
-// Queues the copy, and after the kernels that read it, the buffer's release.
-int send_upload(jx_pkv::Upload* u, size_t bytes, cudaStream_t st) {
-    PKV_CUDA(cudaMemcpyAsync(u->d, u->h, bytes, cudaMemcpyHostToDevice, st));
-    return JX_OK;
-}
-int release_upload(jx_pkv::Upload* u, cudaStream_t st) {
-    PKV_CUDA(cudaEventRecord(u->done, st));
-    u->pending = true;
-    return JX_OK;
-}
+// A list on its way: copied to the device, and the buffer's release queued behind the
+// kernels that read it, whichever way the call ends.
+struct SentUpload {
+    jx_pkv::Upload* u;
+    cudaStream_t st;
+    SentUpload(jx_pkv::Upload* u_, cudaStream_t st_) : u(u_), st(st_) {}
+    SentUpload(const SentUpload&) = delete;
+    ~SentUpload() { u->pending = cudaEventRecord(u->done, st) == cudaSuccess; }
+    int copy(size_t bytes) const {
+        PKV_CUDA(cudaMemcpyAsync(u->d, u->h, bytes, cudaMemcpyHostToDevice, st));
+        return JX_OK;
+    }
+};
 
-int grow_device(void** p, size_t* have, size_t need, const char* what) {
+int grow_device(jx_pkv* kv, void** p, size_t* have, size_t need, const char* what) {
     if (*have >= need) return JX_OK;
+    if (kv->opt_test_fail) return pfail(JX_ERR_NOMEM, "%s of %zu bytes failed (test_fail)", what, need);
     if (*p) {
         PKV_CUDA(cudaDeviceSynchronize());  // earlier calls may still be reading it
         PKV_CUDA(cudaFree(*p));
@@ -817,12 +827,17 @@ int append_rows(jx_pkv* kv, PagedArgs& A, const std::vector<PagedLayer>& part, c
 }
 
 // The step kernel over the given layers and runs (of at most 8 / G tokens),
-// in as many launches as their plan takes.
+// in as many launches as their plan takes: at most 64 layers, 128 runs and 2^30
+// units (of one layer a sequence cannot have more: 2^30 records are 2 TB).
 int step_rows(jx_pkv* kv, PagedArgs& A, const std::vector<PagedLayer>& part, const std::vector<PagedRun>& runs,
               cudaStream_t st, int* launches) {
     constexpr long long kMaxUnits = 1ll << 30;
-    for (size_t l0 = 0; l0 < part.size(); l0 += kMaxCallLayers) {
-        A.n_layers = static_cast<int>(std::min<size_t>(kMaxCallLayers, part.size() - l0));
+    long long longest = 1;
+    for (const PagedRun& r : runs) longest = std::max<long long>(longest, (r.pos0 + r.n - 1) / kPageRows + 1 + kPieceCost);
+    const size_t most = static_cast<size_t>(
+        std::min<long long>(kMaxCallLayers, std::max<long long>(1, kMaxUnits / (longest * A.n_kv))));
+    for (size_t l0 = 0; l0 < part.size(); l0 += most) {
+        A.n_layers = static_cast<int>(std::min(most, part.size() - l0));
         std::copy_n(part.begin() + l0, A.n_layers, A.layers);
         std::stable_partition(A.layers, A.layers + A.n_layers,
                               [](const PagedLayer& L) { return !(L.flags & kLayerWindow); });
@@ -840,10 +855,7 @@ int step_rows(jx_pkv* kv, PagedArgs& A, const std::vector<PagedLayer>& part, con
                 const int last = r.pos0 + r.n - 1;
                 const int n0 = last / kPageRows + 1 + kPieceCost;
                 const int n1 = last / kPageRows - std::max(0, r.pos0 - A.window + 1) / kPageRows + 1 + kPieceCost;
-                if ((p0 + n0) * seg0 + (p1 + n1) * seg1 > kMaxUnits) {
-                    if (A.n_runs > 0) break;
-                    return pfail(JX_ERR_UNSUPPORTED, "a step over %d rows of %d layers is too large", last + 1, A.n_layers);
-                }
+                if (A.n_runs > 0 && (p0 + n0) * seg0 + (p1 + n1) * seg1 > kMaxUnits) break;
                 r.off = static_cast<int>(p0);
                 r.off1 = static_cast<int>(p1);
                 p0 += n0;
@@ -907,14 +919,8 @@ bool prompt_on_tensor_cores(const jx_pkv* kv, const PagedArgs& A, const std::vec
 }
 
 // Prompt attention on the tensor cores: the rows of a group of layers are
-// brought to fp16 (see widen_kernel), then paged_prompt_kernel runs over them.  Its work items are laid out for its persistent
-// CTAs here: longest first, dealt in turn and back.
-int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all, const std::vector<PagedRun>& runs,
-              cudaStream_t st, int* launches) {
-    const jx_pkv_desc& D = kv->d;
-    const int hd = static_cast<int>(D.head_dim), G = A.G, TQ = 2 * kPromptRows / G, BN = kPromptRows;
-    const TensorMapEncode enc = tensor_map_encode();
-    if (!enc) return pfail(JX_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+// brought to fp16 (see widen_kernel), then paged_prompt_kernel runs over them.
+struct PromptPlan {
     struct Group {
         size_t r0, nr;
         std::vector<PagedLayer> layers;
@@ -923,6 +929,20 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
         int grid;
     };
     std::vector<Group> groups;
+    jx_pkv::Upload* list = nullptr;  // items, then each CTA's first, of all groups
+    size_t bytes = 0, first_at = 0;
+};
+
+// Groups, work items (laid out for the persistent CTAs: longest first, dealt in
+// turn and back) and workspaces: all that can fail for lack of memory.  Changes
+// nothing of the cache.
+int plan_prompt(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all, const std::vector<PagedRun>& runs,
+                PromptPlan* plan) {
+    const jx_pkv_desc& D = kv->d;
+    const int hd = static_cast<int>(D.head_dim), G = A.G, TQ = 2 * kPromptRows / G, BN = kPromptRows;
+    if (!tensor_map_encode()) return pfail(JX_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    using Group = PromptPlan::Group;
+    std::vector<Group>& groups = plan->groups;
     const size_t row_bytes = static_cast<size_t>(D.n_kv_heads) * hd * 2;
     for (size_t r0 = 0; r0 < runs.size();) {
         // sequences whose rows of one layer fit the budget go together (one at least)
@@ -1017,24 +1037,34 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
         }
         firsts.push_back(static_cast<int>(at - g.at_items));
     }
-    const size_t first_at = items.size() * sizeof(PrefillTile);
-    const size_t bytes = first_at + firsts.size() * sizeof(int);
+    const size_t first_at = plan->first_at = items.size() * sizeof(PrefillTile);
+    const size_t bytes = plan->bytes = first_at + firsts.size() * sizeof(int);
     size_t wide = 0, heads = 0;
     for (const Group& g : groups) {
         wide = std::max<size_t>(wide, 2 * row_bytes * g.rows * g.nr * g.layers.size());
         heads = std::max<size_t>(heads, g.nr * g.layers.size() * D.n_kv_heads);
     }
-    if (int rc = grow_device(reinterpret_cast<void**>(&kv->d_wide), &kv->wide_bytes, wide, "fp16 rows")) return rc;
-    if (int rc = grow_device(reinterpret_cast<void**>(&kv->d_head_scale), &kv->head_scales, heads * sizeof(float2), "head scales")) return rc;
-    if (int rc = grow_device(reinterpret_cast<void**>(&kv->d_totals), &kv->totals_bytes,
+    if (int rc = grow_device(kv, reinterpret_cast<void**>(&kv->d_wide), &kv->wide_bytes, wide, "fp16 rows")) return rc;
+    if (int rc = grow_device(kv, reinterpret_cast<void**>(&kv->d_head_scale), &kv->head_scales, heads * sizeof(float2), "head scales")) return rc;
+    if (int rc = grow_device(kv, reinterpret_cast<void**>(&kv->d_totals), &kv->totals_bytes,
                              static_cast<size_t>(std::max(kv->num_sms, 1)) * 2 * hd * kPromptRows * sizeof(float), "totals"))
         return rc;
-    jx_pkv::Upload* u = nullptr;
-    if (int rc = take_upload(kv, bytes, &u)) return rc;
-    std::memcpy(u->h, items.data(), first_at);
-    std::memcpy(static_cast<char*>(u->h) + first_at, firsts.data(), firsts.size() * sizeof(int));
-    if (int rc = send_upload(u, bytes, st)) return rc;
-    for (const Group& g : groups) {
+    if (int rc = take_upload(kv, bytes, &plan->list)) return rc;
+    std::memcpy(plan->list->h, items.data(), first_at);
+    std::memcpy(static_cast<char*>(plan->list->h) + first_at, firsts.data(), firsts.size() * sizeof(int));
+    return JX_OK;
+}
+
+int run_prompt(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedRun>& runs, const PromptPlan& plan,
+               cudaStream_t st, int* launches) {
+    const jx_pkv_desc& D = kv->d;
+    const int hd = static_cast<int>(D.head_dim), G = A.G, BN = kPromptRows;
+    const size_t row_bytes = static_cast<size_t>(D.n_kv_heads) * hd * 2;
+    const TensorMapEncode enc = tensor_map_encode();
+    jx_pkv::Upload* u = plan.list;
+    const SentUpload sent(u, st);
+    if (int rc = sent.copy(plan.bytes)) return rc;
+    for (const PromptPlan::Group& g : plan.groups) {
         const size_t nl = g.layers.size();
         WidenArgs w{};
         w.pool = kv->pool;
@@ -1074,7 +1104,7 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
                 return pfail(JX_ERR_CUDA, "cuTensorMapEncodeTiled failed");
         PromptArgs p{};
         p.tiles = reinterpret_cast<const PrefillTile*>(u->d) + g.at_items;
-        p.cta_first = reinterpret_cast<const int*>(static_cast<const char*>(u->d) + first_at) + g.at_first;
+        p.cta_first = reinterpret_cast<const int*>(static_cast<const char*>(u->d) + plan.first_at) + g.at_first;
         p.q = A.q;
         p.out = A.out;
         p.q_stride = A.q_stride;
@@ -1096,7 +1126,7 @@ int prompt_tc(jx_pkv* kv, const PagedArgs& A, const std::vector<PagedLayer>& all
         if (e != cudaSuccess) return pfail(JX_ERR_CUDA, "prompt launch failed: %s", cudaGetErrorString(e));
         *launches += 2;
     }
-    return release_upload(u, st);
+    return JX_OK;
 }
 
 int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const jx_step_args* a,
@@ -1189,13 +1219,6 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
         all[l].flags = static_cast<uint8_t>((L.is_swa && a->sliding_window > 0 ? kLayerWindow : 0) |
                                             (L.shares_kv ? 0 : kLayerAppend));
     }
-    if (any_write) {
-        if (int rc = make_room(kv, spans, st)) return rc;
-        for (const Span& s : spans) {
-            drop_rows(kv, s.seq, s.end);
-            kv->rows[s.seq] = s.end;
-        }
-    }
     for (size_t i = 0; i < kv->ropes.size(); ++i) A.rope[i] = kv->ropes[i].d_tab;
     A.pool = kv->pool;
     A.table = kv->d_table;
@@ -1228,38 +1251,48 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
     const bool out_vec = reinterpret_cast<uintptr_t>(a->out) % 16 == 0 && a->q_stride % 4 == 0;
     A.scratch = kv->d_scratch;
     A.counters = kv->d_counters;
-    int launches = 0;
-    if (prompt) {
-        // all rows of the call first
-        std::vector<PagedLayer> part;
-        for (const PagedLayer& L : all)
-            if (L.flags & kLayerAppend) part.push_back(L);
-        if (int rc = append_rows(kv, A, part, runs, st, &launches)) return rc;
-        // then attention: on the tensor cores, or (few tokens, or a shape that kernel
-        // does not take) for blocks of as many tokens as fill the step kernel's columns
-        if (paged_prompt_supported(static_cast<int>(D.head_dim), static_cast<int>(G)) && out_vec && a->scale > 0.0f &&
-            (kv->opt_prefill_tc < 0 ? prompt_on_tensor_cores(kv, A, all, runs) : kv->opt_prefill_tc > 0)) {
-            if (int rc = prompt_tc(kv, A, all, runs, st, &launches)) return rc;
-            kv->last_launches = launches;
-            return JX_OK;
+    // Attention of a prompt: on the tensor cores, or (few tokens, or a shape that kernel
+    // does not take) for blocks of as many tokens as fill the step kernel's columns.
+    const bool tc = prompt && paged_prompt_supported(static_cast<int>(D.head_dim), static_cast<int>(G)) && out_vec &&
+                    a->scale > 0.0f &&
+                    (kv->opt_prefill_tc < 0 ? prompt_on_tensor_cores(kv, A, all, runs) : kv->opt_prefill_tc > 0);
+    // What can fail for lack of memory comes before the rows of the call are claimed.
+    PromptPlan plan;
+    std::vector<PagedLayer> first, second;
+    std::vector<PagedRun> blocks;
+    if (tc)
+        if (int rc = plan_prompt(kv, A, all, runs, &plan)) return rc;
+    for (const PagedLayer& L : all) {
+        if (prompt) {
+            if (L.flags & kLayerAppend) first.push_back(L);  // written before any attention
+        } else {
+            // a layer that reads rows another layer of the call writes goes second
+            const bool later = !(L.flags & kLayerAppend) && writer[L.cache_layer] >= 0;
+            (later ? second : first).push_back(L);
         }
+    }
+    if (prompt && !tc) {
         const int nq = std::max(1, kStepCols / static_cast<int>(G));
-        std::vector<PagedRun> blocks;
         for (const PagedRun& r : runs)
             for (int j = 0; j < r.n; j += nq)
                 blocks.push_back(PagedRun{r.seq, r.pos0 + j, std::min(nq, r.n - j), r.io0 + j, 0, 0});
-        if (int rc = step_rows(kv, A, all, blocks, st, &launches)) return rc;
-    } else {
-        // a layer that reads rows another layer of the call writes goes second
-        A.append = 1;
-        for (int wave = 0; wave < 2; ++wave) {
-            std::vector<PagedLayer> part;
-            for (const PagedLayer& L : all) {
-                const bool later = !(L.flags & kLayerAppend) && writer[L.cache_layer] >= 0;
-                if (later == (wave == 1)) part.push_back(L);
-            }
-            if (int rc = step_rows(kv, A, part, runs, st, &launches)) return rc;
+    }
+    if (any_write) {
+        if (int rc = make_room(kv, spans, st)) return rc;
+        for (const Span& s : spans) {
+            drop_rows(kv, s.seq, s.end);
+            kv->rows[s.seq] = s.end;
         }
+    }
+    int launches = 0;
+    if (prompt) {
+        if (int rc = append_rows(kv, A, first, runs, st, &launches)) return rc;
+        if (int rc = tc ? run_prompt(kv, A, runs, plan, st, &launches) : step_rows(kv, A, all, blocks, st, &launches))
+            return rc;
+    } else {
+        A.append = 1;
+        if (int rc = step_rows(kv, A, first, runs, st, &launches)) return rc;
+        if (int rc = step_rows(kv, A, second, runs, st, &launches)) return rc;
     }
     kv->last_launches = launches;
     return JX_OK;
@@ -1296,7 +1329,8 @@ int keep_impl(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, cu
     if (!in_place)
         for (uint32_t i = keep_pages; i < n_pages; ++i) result[i] = take_page(kv);
     std::memcpy(list + n_rows + n_src, result.data(), n_pages * sizeof(int));
-    if (int rc = send_upload(u, n_list * sizeof(int), st)) return rc;
+    const SentUpload sent(u, st);
+    if (int rc = sent.copy(n_list * sizeof(int))) return rc;
     const int* d_list = static_cast<const int*>(u->d);
     KeepArgs k{};
     k.pool = kv->pool;
@@ -1314,7 +1348,6 @@ int keep_impl(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, cu
         keep_kernel<hd.value, dt.value><<<grid, 2 * hd.value, 0, st>>>(k);
     });
     if (int rc = launched("keep")) return rc;
-    if (int rc = release_upload(u, st)) return rc;
     if (in_place) {
         drop_rows(kv, seq, n_rows);
         return JX_OK;
@@ -1518,9 +1551,12 @@ int jx_pkv_copy(jx_pkv* kv, uint32_t src, uint32_t dst, void* stream) {
         if (from.size() > kv->free_pages.size() + freed)
             return pfail(JX_ERR_NOMEM, "%zu pages are needed, %zu of %u are free", from.size(),
                          kv->free_pages.size() + freed, kv->d.n_pages);
-        drop_rows(kv, dst, 0);
         std::vector<TableEntry> table;
         std::vector<std::pair<int, int>> copies;
+        table.reserve(from.size());
+        copies.reserve(from.size());
+        kv->pages[dst].reserve(from.size());
+        drop_rows(kv, dst, 0);
         for (size_t i = 0; i < from.size(); ++i) {
             const int p = take_page(kv);
             kv->pages[dst].push_back(p);
@@ -1693,6 +1729,10 @@ int jx_pkv_set_option(jx_pkv* kv, const char* key, int value) {
     if (value < 0) return pfail(JX_ERR_INVALID, "%s must not be negative", key);
     if (std::strcmp(key, "wait_limit_ms") == 0) {
         kv->opt_wait_limit_ms = value;
+        return JX_OK;
+    }
+    if (std::strcmp(key, "test_fail") == 0) {
+        kv->opt_test_fail = value;
         return JX_OK;
     }
     if (std::strcmp(key, "test_wait_cta") == 0) {
