@@ -344,7 +344,7 @@ JX_API int jx_pkv_check_device_error(jx_pkv* kv, int* code, void* stream);
  * in the step kernel's blocks (0), or by an estimate of both (-1, the default).
  * The tensor-core kernel takes K and V beyond 8e6 in magnitude as that large.
  * "test_fail" 1: a workspace that a prompt or a keep would have to allocate
- * cannot be had -- a test of that error path (0 = off). */
+ * cannot be had; 2: a keep's launch fails -- tests of those error paths (0 = off). */
 JX_API int jx_pkv_set_option(jx_pkv* kv, const char* key, int value);
 /* Kernels the last jx_pkv_attn_step / jx_pkv_attn_prefill launched. */
 JX_API int jx_pkv_last_launch_count(const jx_pkv* kv, int* count);

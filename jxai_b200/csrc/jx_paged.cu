@@ -552,7 +552,7 @@ struct jx_pkv {
     int num_sms = 0;
     int opt_wait_limit_ms = 0;
     int opt_test_wait_cta = 0;
-    int opt_test_fail = 0;          // test hook: a call's workspaces cannot be had
+    int opt_test_fail = 0;                // test hook: workspaces (1), a keep's launch (2) fail
     int opt_prefill_tc = -1;              // prompts on the tensor cores: 1 / 0, -1: by estimate
     int last_launches = 0;
 };
@@ -751,7 +751,7 @@ int take_upload(jx_pkv* kv, size_t bytes, jx_pkv::Upload** out) {
     if (u.pending) PKV_CUDA(cudaEventSynchronize(u.done));
     u.pending = false;
     if (u.bytes < bytes) {
-        if (kv->opt_test_fail) return pfail(JX_ERR_NOMEM, "list of %zu bytes failed (test_fail)", bytes);
+        if (kv->opt_test_fail == 1) return pfail(JX_ERR_NOMEM, "list of %zu bytes failed (test_fail)", bytes);
         if (u.h) PKV_CUDA(cudaFreeHost(u.h));
         u.h = nullptr;
         if (u.d) PKV_CUDA(cudaFree(u.d));
@@ -784,7 +784,7 @@ struct SentUpload {
 
 int grow_device(jx_pkv* kv, void** p, size_t* have, size_t need, const char* what) {
     if (*have >= need) return JX_OK;
-    if (kv->opt_test_fail) return pfail(JX_ERR_NOMEM, "%s of %zu bytes failed (test_fail)", what, need);
+    if (kv->opt_test_fail == 1) return pfail(JX_ERR_NOMEM, "%s of %zu bytes failed (test_fail)", what, need);
     if (*p) {
         PKV_CUDA(cudaDeviceSynchronize());  // earlier calls may still be reading it
         PKV_CUDA(cudaFree(*p));
@@ -1326,8 +1326,22 @@ int keep_impl(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, cu
     std::memcpy(list, rows, n_rows * sizeof(int));
     std::memcpy(list + n_rows, pg.data(), n_src * sizeof(int));
     std::vector<int> result(pg.begin(), pg.begin() + n_pages);
-    if (!in_place)
+    std::vector<TableEntry> table;
+    table.reserve(fresh);
+    struct Fresh {  // pages taken for the result, given back unless the call succeeds
+        jx_pkv* kv;
+        std::vector<int>& result;
+        uint32_t first;
+        bool taken;
+        ~Fresh() {
+            if (taken)
+                for (size_t i = result.size(); i > first; --i) give_back(kv, result[i - 1]);
+        }
+    } hold{kv, result, keep_pages, false};
+    if (!in_place) {
         for (uint32_t i = keep_pages; i < n_pages; ++i) result[i] = take_page(kv);
+        hold.taken = true;
+    }
     std::memcpy(list + n_rows + n_src, result.data(), n_pages * sizeof(int));
     const SentUpload sent(u, st);
     if (int rc = sent.copy(n_list * sizeof(int))) return rc;
@@ -1343,6 +1357,7 @@ int keep_impl(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, cu
     k.blk0 = static_cast<int>(keep_pages * (kPageRows / kBlockRows));
     k.n_blk = static_cast<int>((n_rows + kBlockRows - 1) / kBlockRows) - k.blk0;
     k.serial = in_place ? 1 : 0;
+    if (kv->opt_test_fail == 2) return pfail(JX_ERR_CUDA, "keep launch failed (test_fail)");
     const dim3 grid(in_place ? 1 : k.n_blk, (k.n_rec + kKeepRecords - 1) / kKeepRecords);
     dispatch(D, [&](auto hd, auto dt) {
         keep_kernel<hd.value, dt.value><<<grid, 2 * hd.value, 0, st>>>(k);
@@ -1352,7 +1367,7 @@ int keep_impl(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, cu
         drop_rows(kv, seq, n_rows);
         return JX_OK;
     }
-    std::vector<TableEntry> table;
+    hold.taken = false;
     for (uint32_t i = keep_pages; i < n_pages; ++i) table.push_back({seq, i, result[i]});
     for (size_t i = keep_pages; i < pg.size(); ++i) give_back(kv, pg[i]);
     pg = std::move(result);

@@ -68,3 +68,22 @@ def test_a_keep_without_its_list_changes_nothing():
     p.cache.keep(0, np.array(rows))
     p.model.keep(0, rows)
     p.check_rows(0)
+
+
+@pytest.mark.parametrize("pages", [4, 8])
+def test_a_keep_that_fails_late_loses_no_page(pages):
+    """After the pages for the result were taken (or, in a full pool, in place)."""
+    p = Pair(4, 2, 64, "int8", cap=128, n_pages=pages, seed=4)
+    p.run([(0, 0, 100)], True)
+    before = state(p)
+    rows = list(range(0, 100, 2))
+    p.cache.set_option("test_fail", 2)
+    for _ in range(3):
+        refuses(_lib.JX_ERR_CUDA, p.cache.keep, 0, rows)
+        assert state(p) == before
+    p.check_rows(0)
+    p.cache.set_option("test_fail", 0)
+    p.cache.keep(0, rows)
+    p.model.keep(0, rows)
+    p.check_rows(0)
+    p.run([(0, 50, 1)], False)
