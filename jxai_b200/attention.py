@@ -97,6 +97,14 @@ def _i32_array(x):
     return (C.c_int32 * a.size).from_buffer_copy(np.ascontiguousarray(a, dtype=np.int32))
 
 
+def _call_ints(x):
+    """Positions or sequences of a call: as _i32_array, and arrays that it refuses (of floats or
+    truth values, of more dimensions) element by element, as lists are."""
+    if isinstance(x, np.ndarray) and (x.ndim != 1 or x.dtype.kind not in "iu"):
+        x = list(x)
+    return _i32_array(x)
+
+
 class KVCache:
     """Device KV cache: K and V each [n_seqs][n_layers][capacity][row_stride]."""
 
@@ -292,10 +300,12 @@ def _step_args(cache, layers, q, k, v, out, pos, n_heads, n_kv_heads, scale, sof
     rows = n * len(layers)
     if scale is None:
         scale = 1.0 / math.sqrt(hd)
-    pos_a = _i32_array(pos)
+    pos_a = _call_ints(pos)
     sid = None
     if seq_ids is not None:
-        sid = _i32_array(seq_ids)
+        sid = _call_ints(seq_ids)
+        if len(sid) < n and isinstance(cache, KVCache):
+            sid = (C.c_int32 * n)(*sid)  # the rows that it does not list: sequence 0
         if len(sid) != n:
             raise JxError(-1, "seq_ids: one sequence per row")
     a = StepArgs()
