@@ -730,7 +730,8 @@ int rope_table(jx_pkv* kv, const jx_layer_desc& L, float yarn, bool neox, cudaSt
     return JX_OK;
 }
 
-int check_device_ptr(const void* p, const char* name, int device) {
+int check_device_ptr(const void* p, const char* name, int device, int align) {
+    if (reinterpret_cast<uintptr_t>(p) % align != 0) return pfail(JX_ERR_INVALID, "%s must be aligned to %d bytes", name, align);
     cudaPointerAttributes at{};
     const cudaError_t e = cudaPointerGetAttributes(&at, p);
     if (e != cudaSuccess) {
@@ -1204,7 +1205,7 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
     OnDevice on(D.device);
     if (!on.ok) return pfail(JX_ERR_CUDA, "cannot select device %d", D.device);
     for (int i = 0; i < 4; ++i)
-        if (int rc = check_device_ptr(ptrs[i], names[i], D.device)) return rc;
+        if (int rc = check_device_ptr(ptrs[i], names[i], D.device, 4)) return rc;
     if (int rc = refuse_capture(st)) return rc;
     std::vector<PagedLayer> all(n_layers);
     PagedArgs A{};
@@ -1621,11 +1622,8 @@ int jx_pkv_load_rows(jx_pkv* kv, uint32_t seq, uint32_t row0, uint32_t n_rows, c
         if (!on.ok) return pfail(JX_ERR_CUDA, "cannot select device %d", D.device);
         const void* ptrs[4] = {k_codes, k_scales, v_codes, v_scales};
         const char* names[4] = {"k_codes", "k_scales", "v_codes", "v_scales"};
-        for (int i = 0; i < 4; ++i) {
-            if (int rc = check_device_ptr(ptrs[i], names[i], D.device)) return rc;
-            if (reinterpret_cast<uintptr_t>(ptrs[i]) % (i % 2 ? 4 : 16) != 0)
-                return pfail(JX_ERR_INVALID, "%s must be aligned to %d bytes", names[i], i % 2 ? 4 : 16);
-        }
+        for (int i = 0; i < 4; ++i)
+            if (int rc = check_device_ptr(ptrs[i], names[i], D.device, i % 2 ? 4 : 16)) return rc;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         if (int rc = refuse_capture(st)) return rc;
         if (int rc = make_room(kv, {Span{seq, row0, row0 + n_rows}}, st)) return rc;
@@ -1666,8 +1664,7 @@ int jx_pkv_read_rows(jx_pkv* kv, const int32_t* seq_ids, const int32_t* row0, ui
         if (n == 0 || n_rows == 0) return JX_OK;
         OnDevice on(D.device);
         if (!on.ok) return pfail(JX_ERR_CUDA, "cannot select device %d", D.device);
-        if (int rc = check_device_ptr(out, "out", D.device)) return rc;
-        if (reinterpret_cast<uintptr_t>(out) % 16 != 0) return pfail(JX_ERR_INVALID, "out must be aligned to 16 bytes");
+        if (int rc = check_device_ptr(out, "out", D.device, 16)) return rc;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         if (int rc = refuse_capture(st)) return rc;
         ReadArgs a{};

@@ -1,4 +1,5 @@
-"""Calls on the paged cache that find too little memory, on the GPU: they say so and change nothing."""
+"""Calls on the paged cache that find too little memory, or memory that they cannot use, on the GPU:
+they say so and change nothing."""
 import numpy as np
 import pytest
 
@@ -87,3 +88,25 @@ def test_a_keep_that_fails_late_loses_no_page(pages):
     p.model.keep(0, rows)
     p.check_rows(0)
     p.run([(0, 50, 1)], False)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("which", ["q", "k", "v", "out"])
+def test_misaligned_rows_are_refused(which, prompt):
+    """Addresses that no float has are refused on the host; those that only lack the alignment of
+    wide loads are taken."""
+    import torch
+    p = Pair(2, 1, 64, "int8", cap=64, seed=4)
+    p.run([(0, 0, 40)], True)
+    before = state(p)
+    z = [torch.zeros(2, 1, w * 64, device="cuda") for w in (2, 1, 1, 2)]
+    plan = jx.StepPlan(p.cache, p.layers, *z, [40], 2, 1, seq_ids=[0], prefill=prompt)
+    at = getattr(plan.args, which)
+    for offset in (1, 2, 3):
+        setattr(plan.args, which, at + offset)
+        refuses(_lib.JX_ERR_INVALID, plan.run)
+        assert state(p) == before
+    setattr(plan.args, which, at + 4)
+    plan.run()
+    torch.cuda.synchronize()
+    assert p.cache.check_device_error() == 0 and p.cache.seq_pos(0) == 41
