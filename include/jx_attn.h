@@ -331,7 +331,14 @@ JX_API int jx_pkv_read_rows(jx_pkv* kv, const int32_t* seq_ids, const int32_t* r
  * handle (rope_dim, base, factors, yarn_scale).  In a prompt, the rows of one sequence
  * stand together and ascend by one.  New pages come from the pool; with too few
  * left, or where a prompt's workspaces cannot be allocated, JX_ERR_NOMEM and
- * nothing is changed. */
+ * nothing is changed.
+ *
+ * A prompt runs in the step kernel's blocks or on the tensor cores (see the option
+ * "prefill_tc").  The latter attends rows brought to fp16 with one power of two per
+ * call, layer and kv head: values are exact where the head's block scales lie within
+ * 2^32 (JX_I8) or 2^22 (JX_E4M3) of the largest and else off by at most 2^-32 of it;
+ * beyond 1.7e7 (JX_I8) or 3.4e7 (JX_E4M3) a value counts as that large, and
+ * others of its head are then off by at most 2^-16. */
 JX_API int jx_pkv_attn_step(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers,
                             const jx_step_args* args, void* stream);
 JX_API int jx_pkv_attn_prefill(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers,
@@ -342,7 +349,6 @@ JX_API int jx_pkv_check_device_error(jx_pkv* kv, int* code, void* stream);
 /* "wait_limit_ms" and "test_wait_cta" (of a step): as in jx_kv_set_option;
  * "prefill_tc": prompts on the tensor-core kernel where it takes their shape (1),
  * in the step kernel's blocks (0), or by an estimate of both (-1, the default).
- * The tensor-core kernel takes K and V beyond 8e6 in magnitude as that large.
  * "test_fail" 1: a workspace that a prompt or a keep would have to allocate
  * cannot be had; 2: a keep's launch fails -- tests of those error paths (0 = off). */
 JX_API int jx_pkv_set_option(jx_pkv* kv, const char* key, int value);

@@ -418,12 +418,13 @@ static_assert(sizeof(WidenArgs) <= 4096, "kernel parameters");
 constexpr int kWidenRows = 64;
 constexpr int kMaxWideExp = 16;
 
-// A code times 2^(k - K), K so that the head's largest block exponent becomes 8:
-// exact in fp16 for blocks down to 2^-32 of the largest scale (below that a
-// value is off by 2^-33 of the largest), and never beyond 448 * 2^7.  K is at most
-// 16 - 8: a row that holds infinities (2^62 in the cache) is taken as large as
-// 2^23, so that it cannot wipe out the rows of tokens that do not attend it.  The
-// factor 2^K of each head goes to the prompt kernel, which multiplies scores and
+// A code times 2^(k - K), K so that the head's largest block exponent becomes 8
+// (int8; e4m3: 7) and no value exceeds 448 * 2^7.  fp16 has bits down to 2^-24, an
+// e4m3 code down to 2^-9: exact for blocks down to 2^-32 (e4m3: 2^-22) of the largest
+// scale, below that off by at most 2^-33 (2^-32) of it.  K is at most 8 (9): a row
+// that holds infinities (2^62 in the cache) is taken as 65504 * 2^8 = 1.7e7 (3.4e7),
+// so that it cannot wipe out the rows of tokens that do not attend it; beside it a
+// value is off by at most 2^-17 (2^-16).  The factor 2^K of each head goes to the prompt kernel, which multiplies scores and
 // outputs by it.  One CTA per (64 rows, layer, kv head); the exponents of the
 // sequence's blocks (16 bytes per page) are read by every one of them.
 template <int HD, int DT>

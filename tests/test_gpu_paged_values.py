@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import jxai_b200 as jx
+from tests.paged_model import Model, rotate
 from tests.test_gpu_paged import Pair, cuda, load_prompt
 
 pytestmark = pytest.mark.gpu
@@ -152,6 +153,67 @@ def test_far_scores_over_a_split_segment(dtype):
         # the largest score is at least 30 |u|^2 / 8 / 2 above the next: e^-100 and less of the rest
         tol = np.abs(V[w]).max() * (2.0 ** -21 + n * 2.0 ** -25 + (n / 16 + 4) * 2.0 ** -23)
         assert (np.abs(got - V[w].mean(0)) <= tol).all(), size
+
+
+class Clipped(Model):
+    """The model with values cut at `top`, as prompts on the tensor cores take them."""
+    top = np.inf
+
+    def values(self, *a):
+        return np.clip(super().values(*a), -self.top, self.top)
+
+
+@pytest.mark.parametrize("tc", [0, 1])
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+def test_rows_with_infinities_count_as_they_are_held(dtype, tc):
+    """NaN, infinities, huge and tiny values and blocks of zeros in K and V: every output is the
+    model's, over the rows as they are held."""
+    p = Pair(2, 1, 64, dtype, cap=128, seed=3, tc=tc)
+    p.model = Clipped(1, 1, 128, 1, 64, dtype)
+    if tc:
+        # fp16 ends at 65504; the unit of a head's rows is at most 2^8 (int8) or 2^9
+        p.model.top = 65504.0 * 2.0 ** (8 if dtype == "int8" else 9)
+    q, k, v = p.inputs(60)
+    k[0, 0, :8] = [np.nan, np.inf, -np.inf, 0, 1e30, -1e-40, 1e-30, 3e38]
+    v[1, 0, :8] = [np.nan, np.inf, -np.inf, 0, 1e30, -1e-40, 1e-30, 3e38]
+    k[16:32] = 0.0
+    v[16:32] = 0.0
+    q[0:16] = 0.0
+    got = attend(p, 0, 0, q, k, v, True)[:, 0]
+    ref, _ = expect(p, 0, 0, 0, q, k, v)
+    V = np.abs(p.model.values(0, 0, 1, 0, 60)[:, 0])
+    K = p.model.values(0, 0, 0, 0, 60)[:, 0]
+    qr = rotate(q.reshape(60, 2, 64), np.arange(60), **p.kw).astype(np.float64)
+    checked = 0
+    for i in range(60):
+        for h in range(2):
+            e = K[:i + 1] @ qr[i, h] * p.scale
+            if abs(e[0]) < 1e4 and abs(e[0]) > 1e-9:
+                continue  # (the infinite row's score is not far from the others')
+            # Scores but the first row's are ordinary: 64 products of 2^-21 and less.  Values
+            # that lie more than 2^22 below the head's largest are rounded when an e4m3 row is
+            # widened: by 2^-25 of the unit 2^9.
+            wide = 2.0 ** -16 if tc and dtype == "e4m3" else 0.0
+            ds = np.abs(qr[i, h]).sum() * p.scale * (wide + np.abs(K[1:i + 1]).max(initial=0.0) * 2.0 ** -20)
+            tol = V[:i + 1].max(0) * (4 * ds + 2.0 ** -18) + wide
+            assert (np.abs(got[i, h] - ref[i, h]) <= tol).all(), (i, h)
+            checked += 1
+    assert checked > 100
+
+
+@pytest.mark.parametrize("tc", [0, 1])
+@pytest.mark.parametrize("dtype,spread", [("int8", 30), ("e4m3", 20), ("e4m3", 30)])
+def test_values_far_below_those_of_later_rows(dtype, spread, tc):
+    """Tokens that attend small values alone, 2^spread below those of later rows: right to the last
+    bit of their own size, as far as one fp16 unit per head holds both."""
+    p = Pair(4, 1, 64, dtype, cap=256, seed=spread, tc=tc)
+    q, k, v = p.inputs(200)
+    v[:128] *= np.float32(2.0 ** -spread)
+    got = attend(p, 0, 0, q, k, v, True)[:, 0]
+    ref, tol = expect(p, 0, 0, 0, q, k, v)
+    # e4m3 beyond 2^22: off by at most 2^-32 of the largest scale
+    wide = 2.0 ** (p.model.k[0, 0, 1, :12].max() - 32) if tc and dtype == "e4m3" and spread > 22 else 0.0
+    assert (np.abs(got - ref) <= tol + wide).all()
 
 
 def test_a_scale_that_almost_vanishes():
