@@ -229,3 +229,27 @@ def test_a_scale_that_almost_vanishes():
             mean = np.cumsum(V, 0) / np.arange(1, 201)[:, None]
             tol = np.abs(V).max() * (2.0 ** -21 + 200 * 2.0 ** -25 + (200 / 16 + 4) * 2.0 ** -23)
             assert (np.abs(got - mean[:, None]) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+@pytest.mark.parametrize("H,HK,HD,rows", [(4, 1, 64, 1100), (8, 1, 64, 700), (2, 1, 128, 1700), (8, 1, 128, 2300)])
+def test_prompts_behind_many_rows(H, HK, HD, rows, dtype):
+    """Several partial sums of the tensor-core kernel are added up (every 4 or 6 tiles of 128 rows),
+    the reference moving between them: keys that grow along the rows."""
+    p = Pair(H, HK, HD, dtype, cap=rows + 100, seed=rows, tc=1)
+    q, k, v = p.inputs(rows)
+    k *= (0.05 + 6.0 * (np.arange(rows) / rows) ** 2).astype(np.float32)[:, None, None]
+    load_prompt(p, 0, (q, k, v))
+    p.run([(0, rows, 5)], True, spread=8.0)
+    p.run([(0, rows + 5, 70)], True, spread=0.5)
+
+
+@pytest.mark.parametrize("H", [8, 16])
+def test_prompts_of_many_layers_behind_many_rows(H):
+    """More fp16 rows than stay in L2 (items ordered by stream), more layers than one group takes,
+    several items per CTA."""
+    rows, L = 1150, 70
+    p = Pair(H, 8, 64, "int8", L=L, cap=1184, seed=H, tc=1)
+    x = p.inputs(rows)
+    load_prompt(p, 0, x)
+    p.run([(0, rows, 9)], True)
