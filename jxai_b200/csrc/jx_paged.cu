@@ -688,7 +688,7 @@ int make_room(jx_pkv* kv, const std::vector<Span>& spans, cudaStream_t st) {
 
 // The table of (cos, sin) rows for a layer's RoPE setting, built on first use.
 int rope_table(jx_pkv* kv, const jx_layer_desc& L, float yarn, bool neox, cudaStream_t st, int* cfg) {
-    const uint32_t rdim = std::min(L.head_dim, L.rope_dim) / 2 * 2;
+    const uint32_t rdim = std::min(L.head_dim, L.rope_dim);  // (odd: its frequencies, one pair fewer)
     const float* rf = neox && !L.is_swa ? L.rope_freqs : nullptr;
     uint32_t bb, yb;
     std::memcpy(&bb, &L.rope_freq_base, 4);
