@@ -1158,7 +1158,7 @@ int attn_call(jx_pkv* kv, const jx_layer_desc* layers, uint32_t n_layers, const 
             return pfail(JX_ERR_UNSUPPORTED, "layer %u: head_dim %u, the cache has %u", l, L.head_dim, D.head_dim);
         if (L.kv_source_layer >= D.n_layers)
             return pfail(JX_ERR_INVALID, "layer %u: kv_source_layer %u >= %u", l, L.kv_source_layer, D.n_layers);
-        if (!(L.rope_freq_base > 0.0f) || !std::isfinite(L.rope_freq_base))
+        if (std::min(L.head_dim, L.rope_dim) >= 2 && (!(L.rope_freq_base > 0.0f) || !std::isfinite(L.rope_freq_base)))
             return pfail(JX_ERR_INVALID, "layer %u: rope_freq_base must be positive", l);
         if (!L.shares_kv) {
             if (writer[L.kv_source_layer] >= 0)

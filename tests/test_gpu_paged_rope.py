@@ -37,3 +37,12 @@ def test_odd_numbers_of_rotated_dims(rope_dim, neox):
     m = Model(1, 1, 64, 1, 64, "int8")
     m.write(0, 0, 0, 0, x[:, None])
     assert np.array_equal(got.astype(np.float64), m.values(0, 0, 0, 0, 20))
+
+
+@pytest.mark.parametrize("rope_dim", [0, 1])
+@pytest.mark.parametrize("base", [0.0, -1.0, float("nan")])
+def test_a_layer_without_rotation_needs_no_base(rope_dim, base):
+    got, k = keys_after(rope_dim, base, True)
+    m = Model(1, 1, 64, 1, 64, "int8")
+    m.write(0, 0, 0, 0, k)
+    assert np.array_equal(got.astype(np.float64), m.values(0, 0, 0, 0, 20))
