@@ -262,9 +262,10 @@ JX_API int jx_noalloc_set_option(const char* key, int value);
  * A sequence holds the rows [0, seq_pos).  A call that writes rows may begin at
  * any position up to seq_pos; the sequence then ends at the row after the last
  * one written, in every layer (an engine that calls layer by layer passes the
- * same positions for each; a layer that no call wrote holds undefined rows).  Calls on one jx_pkv are ordered on one stream, like those on a
- * jx_kv.  None of them can be captured into a CUDA graph (JX_ERR_UNSUPPORTED):
- * which page a row goes to is decided on the host, call by call. */
+ * same positions for each; a layer that no call wrote holds undefined rows).
+ * Calls on one jx_pkv are ordered on one stream, like those on a jx_kv.  None of
+ * them can be captured into a CUDA graph (JX_ERR_UNSUPPORTED): which page a row
+ * goes to is decided on the host, call by call. */
 typedef struct jx_pkv jx_pkv;
 
 typedef struct {
@@ -301,10 +302,11 @@ JX_API int jx_pkv_fork(jx_pkv* kv, uint32_t src, uint32_t dst, uint32_t n_rows, 
 JX_API int jx_pkv_copy(jx_pkv* kv, uint32_t src, uint32_t dst, void* stream);
 /* Cuts a sequence down to the given rows (HOST array, ascending, each below
  * seq_pos): row i of the result is row rows[i], for every layer.  Blocks that
- * change are scaled and rounded anew from the values held.  Leading pages whose
- * rows all stay in place are kept as they are.  Needs free pages for the others,
- * or none where the pool has too few and the sequence shares none of them (the
- * rows are then moved in place, which is slower). */
+ * change are scaled and rounded anew from the values held.  Keys stay as they were
+ * rotated, and the next row stands at position n_rows, as after jx_kv_compact.
+ * Leading pages whose rows all stay in place are kept as they are.  Needs free pages
+ * for the others, or none where the pool has too few and the sequence shares none of
+ * them (the rows are then moved in place, which is slower). */
 JX_API int jx_pkv_keep(jx_pkv* kv, uint32_t seq, const int32_t* rows, uint32_t n_rows, void* stream);
 /* jx_kv_compact's rule: rows [0, 4) and the last keep_recent rows stay; no-op
  * when the sequence holds no more than those. */

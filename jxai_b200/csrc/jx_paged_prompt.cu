@@ -8,13 +8,11 @@
 //    and P.V (q and p in two fp16 parts; 1024 cycles each at head_dim 128, at 4096
 //    per cycle) against 16384 exponentials at 16 per cycle (1024 cycles) and about 6
 //    instructions per score on four schedulers.  Measured: 8192 tokens of two
-//    Mistral-7B-shaped layers 2.25 ms with append and widening (488 TFLOP/s by the
-//    attention's formula, twice that in products; tensor pipe 52 % active), 2048
-//    tokens of the Llama-3.2-1B shape 1.12 ms; per tile a thread takes about 700
-//    cycles to load scores and find the maximum, 390 to exchange it, 1350 for the
-//    weights, and waits the rest of about 6400 per pair of tiles.  The three overlap only if there
-//    is always a tile for each, so two tiles take turns: while one's softmax runs,
-//    the tensor cores work on the other.
+//    Mistral-7B-shaped layers 2.33 ms with append and widening (472 TFLOP/s by the
+//    attention's formula, twice that in products; tensor pipe 47 % active), 2048
+//    tokens of the Llama-3.2-1B shape 1.13 ms (tensor pipe 25 %).  The three overlap
+//    only if there is always a tile for each, so two tiles take turns: while one's
+//    softmax runs, the tensor cores work on the other.
 //  * Warp 0 streams K and V tiles (128 rows, TMA, 128-byte swizzle) through a
 //    ring.  Warp 1 issues the MMAs of both tiles from one thread.  Warps 2-9 and
 //    10-17 are the softmax of tile 0 and 1: two threads per row, each with half of

@@ -24,8 +24,8 @@ class PagedKVCache:
     """A pool of pages and the sequences that hold them.
 
     ``n_pages`` defaults to as many as all sequences need at ``capacity`` rows;
-    with fewer, a call that finds none free raises ``JxError`` (code -3) and
-    changes nothing.  A sequence holds the rows ``[0, seq_pos)``: a step or prompt
+    with fewer, a call that finds none free (or no memory for a prompt's
+    workspaces) raises ``JxError`` (code -3) and changes nothing.  A sequence holds the rows ``[0, seq_pos)``: a step or prompt
     writes from a position up to ``seq_pos`` on, and the sequence then ends at the
     row after the last one written.
     """
@@ -70,7 +70,9 @@ class PagedKVCache:
 
     @property
     def nbytes(self) -> int:
-        """Bytes of the page pool."""
+        """Bytes of the page pool.  The handle holds more: cosines and sines of every position
+        (capacity * head_dim * 4 bytes per RoPE setting) and, from the first tensor-core prompt on,
+        its fp16 rows (up to 1 GiB, or one sequence and layer where that is more)."""
         record = 2 * self.PAGE * self.head_dim + 16
         return self.n_pages * self.n_layers * self.n_kv_heads * record
 
@@ -110,7 +112,8 @@ class PagedKVCache:
         check(self.lib.jx_pkv_copy(self.handle, src, dst, _stream_ptr(stream, self.device)))
 
     def keep(self, seq: int, rows: Sequence[int], stream=None) -> None:
-        """Cuts the sequence down to the given rows (ascending), in every layer."""
+        """Cuts the sequence down to the given rows (ascending), in every layer.  Their keys stay as
+        they were rotated; the next row stands at position len(rows)."""
         arr = _i32_array(rows)
         check(self.lib.jx_pkv_keep(self.handle, seq, arr, len(arr), _stream_ptr(stream, self.device)))
 

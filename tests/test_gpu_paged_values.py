@@ -155,6 +155,38 @@ def test_far_scores_over_a_split_segment(dtype):
         assert (np.abs(got - V[w].mean(0)) <= tol).all(), size
 
 
+@pytest.mark.parametrize("tc", [0, 1])
+@pytest.mark.parametrize("window", [1, 40, 3000, 0])
+@pytest.mark.parametrize("size", [30.0, 2.0 ** 24, 2.0 ** 50])
+def test_far_scores_of_blocks_with_windows(size, window, tc):
+    """Tokens whose windows begin and end inside pages, behind rows that several CTAs read: pages and
+    parts without rows for some of the tokens, scores near zero and far from it."""
+    rng = np.random.default_rng(window)
+    n, more, HD, H = 3000, 21, 64, 2
+    f, u, (_, k, v) = far_case(rng, n + more, HD, H, 1, 6)
+    p = Pair(H, 1, HD, "int8", cap=3040, seed=1, tc=tc, rope_dim=0, swa=[window > 0], window=window)
+    load_prompt(p, 0, (None, k[:n], v[:n]))
+    at = n - n % 16
+    f[at:] = np.where(np.arange(at, n + more) % 16 == 0, 1.0, f[at:])
+    k[at:] = (f[at:, None, None] * u).reshape(-1, 1, HD)
+    p.cache.rollback(0, at)
+    q = (np.array([1.0, -1.0])[None, None, :, None] * u[:, None] * size).astype(np.float32)
+    q = np.ascontiguousarray(np.broadcast_to(q, (n + more - at, 1, H, HD))).reshape(-1, 1, H * HD)
+    got = attend(p, 0, at, q, k[at:], v[at:], True)[:, 0]
+    p.model.write(0, 0, 0, at, k[at:].reshape(-1, 1, HD))
+    p.model.write(0, 0, 1, at, v[at:].reshape(-1, 1, HD))
+    V = p.model.values(0, 0, 1, 0, n + more)[:, 0]
+    for i, pos in enumerate(range(at, n + more)):
+        lo = max(0, pos - window + 1) if window else 0
+        for h in range(H):
+            x = (1.0, -1.0)[h] * f[lo:pos + 1]
+            won = V[lo:pos + 1][x == x.max()]
+            # the next score is 30 |u|^2 / 16 = 100 or more below: e^-100 of the rest
+            m = pos + 1 - lo
+            tol = np.abs(won).max() * (2.0 ** -21 + m * 2.0 ** -25 + (m / 16 + 4) * 2.0 ** -23)
+            assert (np.abs(got[i, h] - won.mean(0)) <= tol).all(), (pos, h)
+
+
 class Clipped(Model):
     """The model with values cut at `top`, as prompts on the tensor cores take them."""
     top = np.inf
