@@ -424,9 +424,10 @@ constexpr int kMaxWideExp = 16;
 // scale, below that off by at most 2^-33 (2^-32) of it.  K is at most 8 (9): a row
 // that holds infinities (2^62 in the cache) is taken as 65504 * 2^8 = 1.7e7 (3.4e7),
 // so that it cannot wipe out the rows of tokens that do not attend it; beside it a
-// value is off by at most 2^-17 (2^-16).  The factor 2^K of each head goes to the prompt kernel, which multiplies scores and
-// outputs by it.  One CTA per (64 rows, layer, kv head); the exponents of the
-// sequence's blocks (16 bytes per page) are read by every one of them.
+// value is off by at most 2^-17 (2^-16).  The factor 2^K of each head goes to the
+// prompt kernel, which multiplies scores and outputs by it.  One CTA per (64 rows,
+// layer, kv head); the exponents of the sequence's blocks (16 bytes per page) are
+// read by every one of them.
 template <int HD, int DT>
 __global__ void __launch_bounds__(256) widen_kernel(const __grid_constant__ WidenArgs a) {
     constexpr int kTop = DT == DT_I8 ? 8 : 7;

@@ -145,7 +145,8 @@ __device__ __forceinline__ int query_exp(float amax) {
     return min(60, 14 - (static_cast<int>((__float_as_uint(amax) >> 23) & 0xFFu) - 127));
 }
 // What takes that (and the scale of scores) back, no larger than 2^70: times a block's
-// scale it then stays in range, and scores that it cuts are 2^30 apart and more.
+// scale it then stays in range.  (That cuts scores of queries beyond 2^84, by a common
+// factor: they stay far apart.)
 __device__ __forceinline__ float query_unit(int sh, float scale) {
     constexpr float kMost = 1.180591620717411303424e21f;
     const float u = exp2_int(-sh) * scale;

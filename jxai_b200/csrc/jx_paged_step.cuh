@@ -189,6 +189,9 @@ struct StepWarp {
     // is set and moved when a weight would exceed 2^15 (fp16 ends at 2^16).  m is a whole
     // number and c 0, or, scores beyond kFar, m the largest of them.
     static constexpr float kBase = 10.0f, kTop = 15.0f, kFar = 4194304.0f;
+    // Parts are joined with their c where the largest m is beyond this: a part whose m
+    // is beyond kFar has no weight otherwise.
+    static constexpr float kFarJoin = kFar / 2;
 
     uint32_t qf[KS][NBC][2];
     float o[KS][NBC][4];
@@ -647,7 +650,7 @@ __device__ __forceinline__ void warm_inputs(const PagedArgs& a, const Piece& p, 
     }
 }
 
-// Elements e .. e+3 of a split segment's sum where its scores are beyond kFar: each
+// Elements e .. e+3 of a split segment's sum where m is beyond kFarJoin: each
 // part's c counts, too.  Rare, so one part after the other, in a call of its own.
 template <int HD, int GP>
 __device__ __noinline__ float4 join_far(const float* scratch, int c0, int c1, int e, float* sum) {
@@ -872,7 +875,7 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
 #pragma unroll
             for (int w = 0; w < W; ++w) ml[w].x = ml[w].x == -INFINITY ? -INFINITY : ml[w].x - M;
             float Cm = 0.0f;  // of the sum, as M
-            if (fabsf(M) > SW::kFar && M > -INFINITY) {  // (else a part with a c of its own has no weight)
+            if (fabsf(M) > SW::kFarJoin && M > -INFINITY) {
                 Cm = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
@@ -945,7 +948,7 @@ __global__ void __launch_bounds__(StepCfg<HD, GP>::W * 32, StepCfg<HD, GP>::CTAS
                         }
                         M = Mn;
                     }
-                    if (fabsf(M) > SW::kFar && M > -INFINITY) O = join_far<HD, GP>(a.scratch, c0, c1, e, &Ls);
+                    if (fabsf(M) > SW::kFarJoin && M > -INFINITY) O = join_far<HD, GP>(a.scratch, c0, c1, e, &Ls);
                     float* dst = out_at(col, d);
                     const float inv = __fdividef(1.0f, Ls);
                     dst[0] = O.x * inv;

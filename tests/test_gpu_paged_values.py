@@ -187,6 +187,37 @@ def test_far_scores_of_blocks_with_windows(size, window, tc):
             assert (np.abs(got[i, h] - won.mean(0)) <= tol).all(), (pos, h)
 
 
+@pytest.mark.parametrize("flip", [False, True])
+@pytest.mark.parametrize("at,up,down", [(0, 6, -6), (2 ** 21, 6, -6), (2 ** 22, 6, -6), (2 ** 22, 3, -12),
+                                        (2 ** 22, 13, 2), (-2 ** 22, 2, -9)])
+def test_parts_on_both_sides_of_far_scores(at, up, down, flip):
+    """Scores of -at + up and -at + down (in powers of two) in the two halves of a long row, the
+    lower ones with larger values: parts whose sums are taken against references near zero and far
+    from it count alike."""
+    n, HD = 6000, 64
+    j = np.where((np.arange(n) < n // 2) ^ flip, float(up), float(down))
+    k, v = np.zeros((n, 1, HD), np.float32), np.random.default_rng(abs(at)).standard_normal((n, 1, HD))
+    k[:, 0, 0], k[:, 0, 1] = 64.0, j
+    v = (v * np.where(j == up, 2.0 ** 13, 2.0 ** 25)[:, None, None]).astype(np.float32)
+    p = Pair(1, 1, HD, "int8", cap=6016, seed=1, rope_dim=0)
+    load_prompt(p, 0, (None, k, v))
+    K, V = (p.model.values(0, 0, w, 0, n)[:, 0] for w in range(2))
+    assert np.array_equal(K[:, :2], k[:, 0, :2])
+    q, new = np.zeros((1, 1, HD), np.float32), np.zeros((1, 1, HD), np.float32)
+    q[0, 0, :3] = -at / 64, 1.0, -1.0
+    new[0, 0, :3] = 64.0, 0.0, 100.0  # the new row's score: -at - 100
+    # times log2(e) in fp32, the scale is 1: every score a whole number
+    scale = np.float32(np.log(2))
+    assert np.float32(scale * np.float32(1.4426950408889634)) == 1.0
+    got = attend(p, 0, n, q, new, v[:1], False, scale=float(scale))[0, 0, 0]
+    w = np.exp2(j - up)
+    want = (w @ V) / w.sum()
+    # a weight, in the sum of values and in that of weights: 2^-22 from exp2, 2^-22 as two parts;
+    # each sum over rows: one rounding (2^-23) per 16 rows and a few more
+    tol = (w @ np.abs(V)) / w.sum() * 2 * (2.0 ** -21 + (n / 16 + 8) * 2.0 ** -23)
+    assert (np.abs(got - want) <= tol).all(), np.abs(got / want - 1).max()
+
+
 class Clipped(Model):
     """The model with values cut at `top`, as prompts on the tensor cores take them."""
     top = np.inf
