@@ -413,21 +413,30 @@ struct StepWarp {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 d[b][r] = col_sum(acc[b], r);
-                if (capped) d[b][r] = a.cap_out * tanhf(d[b][r] * f[b][r & 1] * a.cap_in);
             }
-            if (capped) f[b][0] = f[b][1] = 1.0f;
+        }
+        if (capped) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) d[b][r] = a.cap_out * tanhf(d[b][r] * f[b][r & 1] * a.cap_in);
+                f[b][0] = f[b][1] = 1.0f;
+            }
         }
         auto exponents = [&]() {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    y[b][r] = fmaf(d[b][r], f[b][r & 1], kv[b] - m[r & 1]);
-                    if (edge) {
+                for (int r = 0; r < 4; ++r) y[b][r] = fmaf(d[b][r], f[b][r & 1], kv[b] - m[r & 1]);
+            if (edge) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
                         const int row = row0 + b * 16 + (r >> 1) * 8 + rp;
                         if (row < lo[r & 1] || row > hi[r & 1]) y[b][r] = -INFINITY;
                     }
-                }
+            }
         };
         exponents();
         const float big[2] = {largest(y, 0), largest(y, 1)};
