@@ -8,10 +8,10 @@
 //    run) goes to shared memory in one bulk copy (head_dim 128 and 256: two, scales
 //    and K, then V, so that 8 or 12 warps per SM have three or four in flight) and is
 //    read once.  Measured (one B200, kernel alone, int8 or e4m3): 131072 rows of the
-//    Mistral-7B shape (8.6 GB) 1.32 ms = 6.5 TB/s; 64 ragged sequences of the
-//    Llama-3.2-1B shape (4.4 GB) 0.79 ms = 5.5 TB/s (head_dim 64: 470 instructions
-//    per 4 KB record, 2.35 per cycle; 128: 820 per 8 KB record, 2.2); one such
-//    sequence of 4096 rows (68 MB) 25 us; 100 rows of one layer 8.4 to 11 us.
+//    Mistral-7B shape (8.6 GB) 1.32-1.35 ms = 6.4-6.5 TB/s; 64 ragged sequences of
+//    the Llama-3.2-1B shape (4.4 GB) 0.73 ms = 5.95 TB/s (head_dim 64: 420 instructions
+//    per 4 KB record, 2.35 per cycle; 128: 770 per 8 KB record, 2.15); one such
+//    sequence of 4096 rows (68 MB) 23 us; 100 rows of one layer 8.4 to 11 us.
 //  * Work.  Units are (kv head, page) pairs, flattened over sequences, layers
 //    and heads; each CTA takes an equal run of them, cut into pieces at segment
 //    boundaries (a segment: one kv head of one layer and sequence).  Unit x of
@@ -55,7 +55,7 @@ struct StepCfg {
     // Resident CTAs per SM, as many as the accumulators' registers allow.  (Groups of
     // 5 to 8 heads, 131072 rows: head_dim 128 three CTAs with spills 159 us, two
     // without 131; head_dim 64 four 80, three 73.  Eight columns of head_dim 256 spill
-    // 460 bytes all the same.)
+    // 470 bytes all the same.)
     static constexpr int CTAS = HD == 256 ? 2 : HD == 128 ? (GP == 8 ? 2 : 3) : HD == 64 && GP == 8 ? 3 : 4;
     // A stage holds a record, or (wide heads) half of one: scales and K, or V.
     static constexpr bool SPLIT = HD >= 128;
